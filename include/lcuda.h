@@ -484,6 +484,99 @@ LC_API int lc_paged_kv_gather(const void* key_pages, const void* value_pages, in
                        void* k_out, void* v_out, int64_t B, int64_t Hkv, int64_t L, int64_t D,
                        int64_t page_size, int dtype, void* stream);
 
+/* Bytes of workspace lc_shared_prefix_decode_fwd needs (fp32 outputs and
+ * logsumexps of the token ranges); capacities are table width x page size. -1
+ * for invalid sizes. */
+LC_API int64_t lc_shared_prefix_decode_workspace_bytes(int64_t B, int64_t groups, int64_t Hq,
+                                                       int64_t Hkv, int64_t D,
+                                                       int64_t prefix_capacity,
+                                                       int64_t own_capacity);
+
+/* Paged GQA decode of a batch whose groups of sequences share a prefix: one
+ * query token per sequence. The B sequences are `groups` groups of W = B /
+ * groups consecutive ones; sequence b attends to the prefix_lens[b / W] tokens
+ * of row b / W of prefix_table and to the seq_lens[b] tokens of row b of
+ * block_table:
+ *   out[b,h,:] = softmax(q[b,h,:] . [K_prefix; K_b]^T * scale) [V_prefix; V_b]
+ * lse[b,h] (fp32, contiguous [B, Hq], may be NULL): natural-log logsumexp of the
+ * scaled scores. A sequence without any token gives out = 0, lse = -inf. A
+ * group's prefix is read and multiplied once for all of its sequences.
+ * No counterpart in the reference, whose cache holds one sequence
+ * (models/llama3/kv_cache.py:43-44).
+ * q, out: [B, Hq, D] with (batch, head) strides. key_pages, value_pages:
+ *   [num_pages, Hkv, page_size, D] pools with shared strides, which both tables
+ *   index; table entries outside [0, num_pages) are never dereferenced (their
+ *   tokens are skipped). prefix_table: int32 [groups, max_prefix_pages];
+ *   block_table: int32 [B, max_pages_per_seq]; either width may be 0.
+ *   prefix_lens int32 [groups] and seq_lens int32 [B] are clamped to the
+ *   tables' capacities.
+ * workspace: >= lc_shared_prefix_decode_workspace_bytes, 256-byte aligned; calls
+ *   that may overlap need their own. */
+LC_API int lc_shared_prefix_decode_fwd(
+    const void* q, int64_t q_sb, int64_t q_sh, const void* key_pages, const void* value_pages,
+    int64_t kv_s_page, int64_t kv_s_head, int64_t kv_s_tok, int64_t num_pages,
+    const int32_t* prefix_table, int64_t pt_stride, int64_t max_prefix_pages,
+    const int32_t* prefix_lens, const int32_t* block_table, int64_t bt_stride,
+    int64_t max_pages_per_seq, const int32_t* seq_lens, void* out, int64_t o_sb, int64_t o_sh,
+    float* lse, void* workspace, int64_t workspace_bytes, int64_t B, int64_t groups, int64_t Hq,
+    int64_t Hkv, int64_t D, int64_t page_size, float scale, int dtype, void* stream);
+
+/* Bytes of workspace lc_beam_select needs, or -1 for invalid sizes. */
+LC_API int64_t lc_beam_select_workspace_bytes(int64_t groups, int64_t width, int64_t vocab,
+                                              int64_t count);
+
+/* Beam search's selection: the `count` best continuations of each group of
+ * `width` beams. With logits x [groups, width, vocab] (unit stride over vocab,
+ * strides of groups and beams given) and the beams' scores s fp32 [groups,
+ * width],
+ *   value(w, v) = s[w] + x[w, v] - ln sum_u exp(x[w, u])
+ * and out_scores (fp32), out_tokens (v) and out_parents (w), int64, all
+ * contiguous [groups, count], hold the largest values, largest first, ties by
+ * the lowest w * vocab + v. Values are formed and compared in 64 bits.
+ * finished (uint8 [groups, width], may be NULL): a beam that is set has one
+ * continuation, the token eos at the beam's own score (its logits are not
+ * read); its other tokens have -inf. out_finished (uint8 [groups, count], may
+ * be NULL): the parent is finished or the token is eos.
+ * A beam with no logit above -inf, or whose score is -inf, has -inf for every
+ * token; NaN or +inf among a beam's logits or in its score makes its values
+ * NaN, which rank above all others.
+ * 1 <= width <= 256, 1 <= count <= min(64, width * vocab), width * vocab <
+ * 2^31. workspace: 256-byte aligned; calls that may overlap need their own.
+ * No counterpart in the reference (models/llama3/model.py:200-218 decodes
+ * greedily). */
+LC_API int lc_beam_select(const void* logits, int64_t group_stride, int64_t beam_stride,
+                          const float* scores, const uint8_t* finished, int64_t eos,
+                          int64_t groups, int64_t width, int64_t vocab, int64_t count,
+                          float* out_scores, int64_t* out_tokens, int64_t* out_parents,
+                          uint8_t* out_finished, void* workspace, int64_t workspace_bytes,
+                          int dtype, void* stream);
+
+/* Reorders paged K/V caches after a selection: sequence w of group n (row n *
+ * width + w of the table) continues what sequence parents[n, w] of the group
+ * holds. The sequences of a group hold the same number of tokens, t =
+ * seq_lens[n * width] (clamped to the table's capacity); let c = t / page_size.
+ * Whole pages are shared, not copied: out_table takes the parent's entries in
+ * the columns before c. If t % page_size > 0, a parent's first child keeps its
+ * page of column c, and its i-th other child over the group takes the page of
+ * column c of the i-th sequence that is nobody's parent, into which the first t
+ * % page_size slots of the parent's page are copied, in every layer. All other
+ * entries of out_table are the sequence's own. So the pages from column c on
+ * stay distinct within the group if they were before, which the call needs.
+ * parents: int64 contiguous [groups, width]; entries outside [0, width) stand
+ * for the sequence itself. key_pages, value_pages: [layers, num_pages, Hkv,
+ * page_size, D] pools with shared strides (head_dim contiguous), one table for
+ * all layers; pages with entries outside [0, num_pages) are not copied.
+ * out_table: int32 [groups * width, max_pages_per_seq]; must not overlap
+ * block_table. width <= 256.
+ * No counterpart in the reference (see lc_beam_select). */
+LC_API int lc_paged_kv_reorder(void* key_pages, void* value_pages, int64_t kv_s_layer,
+                               int64_t kv_s_page, int64_t kv_s_head, int64_t kv_s_tok,
+                               int64_t layers, int64_t num_pages, const int32_t* block_table,
+                               int64_t bt_stride, int32_t* out_table, int64_t out_stride,
+                               int64_t max_pages_per_seq, const int32_t* seq_lens,
+                               const int64_t* parents, int64_t groups, int64_t width, int64_t Hkv,
+                               int64_t D, int64_t page_size, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -149,6 +149,24 @@ _SIGNATURES = {
         [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p],
     ),
+    "lc_shared_prefix_decode_workspace_bytes": (_c_i64, [_c_i64] * 7),
+    "lc_shared_prefix_decode_fwd": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
+         _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_int, _c_p],
+    ),
+    "lc_beam_select_workspace_bytes": (_c_i64, [_c_i64] * 4),
+    "lc_beam_select": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p,
+         _c_p, _c_p, _c_p, _c_i64, ctypes.c_int, _c_p],
+    ),
+    "lc_paged_kv_reorder": (
+        ctypes.c_int,
+        [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64,
+         _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p],
+    ),
 }
 
 EXPORTS = tuple(_SIGNATURES)

@@ -1335,3 +1335,215 @@ def kv_gather(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: t
             B, Hkv, length, D, P, nat.lc_dtype(key_pages), _stream(dev))
     nat.check(rc, "lc_paged_kv_gather")
     return k_out, v_out
+
+
+# ---------------------------------------------------------------------------
+# Beam search: attention of sequences that share a prefix, selection, reordering
+# (no counterpart in the reference, which decodes greedily: model.py:200-218)
+# ---------------------------------------------------------------------------
+def shared_prefix_decode(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                         prefix_table: torch.Tensor, prefix_lens: torch.Tensor,
+                         block_table: torch.Tensor, seq_lens: torch.Tensor,
+                         scale: float | None = None, return_lse: bool = False):
+    """One-token GQA attention over the paged cache of a batch whose groups of
+    W = B / N consecutive sequences share a prefix (forward only).
+
+    q [B, Hq, 1, D] or [B, Hq, D]; key_pages, value_pages [num_pages, Hkv, P, D];
+    prefix_table int32 [N, pages] and prefix_lens int32 [N]: the tokens that
+    every sequence of a group attends to first; block_table int32 [B, pages] and
+    seq_lens int32 [B]: each sequence's own tokens. Returns out with q's shape
+    (and lse [B, Hq] fp32 if return_lse).
+    """
+    args = (prefix_table, prefix_lens, block_table, seq_lens, scale, return_lse)
+    if _records_grad(q, key_pages, value_pages):
+        return _ForwardOnly.apply("shared_prefix_decode",
+                                  lambda a, k, v: _shared_prefix_decode(a, k, v, *args),
+                                  q, key_pages, value_pages)
+    return _shared_prefix_decode(q, key_pages, value_pages, *args)
+
+
+def _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, block_table,
+                          seq_lens, scale, return_lse):
+    squeeze = q.dim() == 3
+    q4 = q.unsqueeze(2) if squeeze else q
+    if q4.dim() != 4 or q4.shape[2] != 1:
+        raise ValueError(f"q must be [batch, heads, 1, head_dim], got {tuple(q.shape)}")
+    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape:
+        raise ValueError("key_pages and value_pages must both be [num_pages, kv_heads, page, dim]")
+    B, Hq, _, D = q4.shape
+    num_pages, Hkv, P, Dk = key_pages.shape
+    if Dk != D:
+        raise ValueError(f"head_dim mismatch: q {D}, pages {Dk}")
+    if Hkv == 0 or Hq % Hkv != 0:
+        raise ValueError(f"n_heads ({Hq}) must be a multiple of n_kv_heads ({Hkv})")
+    for t in (prefix_table, prefix_lens, block_table, seq_lens):
+        if t.dtype != torch.int32:
+            raise TypeError("prefix_table, prefix_lens, block_table and seq_lens must be int32")
+    if prefix_table.dim() != 2 or prefix_lens.shape != (prefix_table.shape[0],):
+        raise ValueError("prefix_table must be [groups, pages] and prefix_lens [groups]")
+    if block_table.dim() != 2 or block_table.shape[0] != B or seq_lens.shape != (B,):
+        raise ValueError("block_table must be [batch, max_pages] and seq_lens [batch]")
+    N = prefix_table.shape[0]
+    if (B % N != 0) if N else B != 0:
+        raise ValueError(f"a batch of {B} sequences is not a multiple of {N} prefix groups")
+    if q4.dtype != key_pages.dtype or q4.dtype != value_pages.dtype:
+        raise TypeError("q and the page pools must share a dtype")
+    dtype = nat.lc_dtype(q4)
+    dev = nat.require_device(q4, key_pages, value_pages, prefix_table, prefix_lens, block_table,
+                             seq_lens)
+    if key_pages.stride() != value_pages.stride() or key_pages.stride(-1) != 1:
+        key_pages, value_pages = key_pages.contiguous(), value_pages.contiguous()
+    if q4.stride(-1) != 1:
+        q4 = q4.contiguous()
+    prefix_table, block_table = (t if t.shape[1] < 2 or t.stride(1) == 1 else t.contiguous()
+                                 for t in (prefix_table, block_table))
+    prefix_lens, seq_lens = prefix_lens.contiguous(), seq_lens.contiguous()
+    out = torch.empty((B, Hq, 1, D), dtype=q4.dtype, device=dev)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    if B > 0:
+        lib = nat.load()
+        need = nat.size("lc_shared_prefix_decode_workspace_bytes", B, N, Hq, Hkv, D,
+                        prefix_table.shape[1] * P, block_table.shape[1] * P)
+        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+        with _guard(dev):
+            rc = lib.lc_shared_prefix_decode_fwd(
+                q4.data_ptr(), q4.stride(0), q4.stride(1), key_pages.data_ptr(),
+                value_pages.data_ptr(), key_pages.stride(0), key_pages.stride(1),
+                key_pages.stride(2), num_pages, prefix_table.data_ptr(),
+                max(prefix_table.stride(0), prefix_table.shape[1]), prefix_table.shape[1],
+                prefix_lens.data_ptr(), block_table.data_ptr(),
+                max(block_table.stride(0), block_table.shape[1]), block_table.shape[1],
+                seq_lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+                None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), B, N, Hq,
+                Hkv, D, P, float(1.0 / math.sqrt(D) if scale is None else scale), dtype,
+                _stream(dev))
+        nat.check(rc, "lc_shared_prefix_decode_fwd")
+    if squeeze:
+        out = out.squeeze(2)
+    return (out, lse) if return_lse else out
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_candidates: int | None = None,
+                finished: torch.Tensor | None = None, eos_token_id: int | None = None):
+    """The best continuations of each group of beams (forward only).
+
+    logits [N, W, V] (float32, float16 or bfloat16); scores fp32 [N, W]: the
+    beams' summed log-probabilities. Returns (scores fp32, tokens int64, parents
+    int64), each [N, K] with K = num_candidates (W by default; at most 64): the
+    largest scores[n, w] + log_softmax(logits[n, w])[v], largest first, ties by
+    the lowest w * V + v. With finished (bool [N, W]; needs eos_token_id) a
+    finished beam's only continuation is eos_token_id at its own score, and a
+    fourth tensor, bool [N, K], says which results are finished. A beam with no
+    logit above -inf or a score of -inf has continuations of -inf; NaN or +inf in
+    its logits or score gives NaN, which ranks first.
+    """
+    if _records_grad(logits, scores):
+        return _ForwardOnly.apply(
+            "beam_select", lambda a, s: _beam_select(a, s, num_candidates, finished, eos_token_id),
+            logits, scores)
+    return _beam_select(logits, scores, num_candidates, finished, eos_token_id)
+
+
+def _beam_select(logits, scores, num_candidates, finished, eos_token_id):
+    if logits.dim() != 3:
+        raise ValueError(f"logits must be [groups, beams, vocab], got {tuple(logits.shape)}")
+    N, W, V = logits.shape
+    if scores.shape != (N, W):
+        raise ValueError(f"scores must be {(N, W)}, got {tuple(scores.shape)}")
+    if scores.dtype != torch.float32:
+        raise TypeError(f"scores must be float32, got {scores.dtype}")
+    K = W if num_candidates is None else int(num_candidates)
+    if not (1 <= W <= 256 and V >= 1 and 1 <= K <= min(64, W * V)):
+        raise ValueError(f"{K} candidates of {W} beams x {V} tokens: beams are 1 to 256, "
+                         "candidates 1 to min(64, beams * vocab)")
+    if W * V >= 2 ** 31:
+        raise ValueError(f"{W} beams x {V} tokens: 2^31 or more")
+    if finished is not None:
+        if finished.dtype != torch.bool or finished.shape != (N, W):
+            raise TypeError(f"finished must be bool {(N, W)}")
+        if eos_token_id is None:
+            raise ValueError("finished needs eos_token_id")
+        if not 0 <= int(eos_token_id) < V:
+            raise ValueError(f"eos_token_id {eos_token_id} outside a vocabulary of {V}")
+    dtype = nat.lc_dtype(logits)
+    dev = nat.require_device(logits, scores, finished)
+    if V > 1 and logits.stride(2) != 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    finished = None if finished is None else finished.contiguous()
+    out_s = torch.empty((N, K), dtype=torch.float32, device=dev)
+    out_t = torch.empty((N, K), dtype=torch.int64, device=dev)
+    out_p = torch.empty((N, K), dtype=torch.int64, device=dev)
+    out_f = None if finished is None else torch.empty((N, K), dtype=torch.bool, device=dev)
+    if N > 0:
+        lib = nat.load()
+        ws = torch.empty(nat.size("lc_beam_select_workspace_bytes", N, W, V, K),
+                         dtype=torch.uint8, device=dev)
+        with _guard(dev):
+            rc = lib.lc_beam_select(
+                logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(),
+                nat.ptr(finished), 0 if finished is None else int(eos_token_id), N, W, V, K,
+                out_s.data_ptr(), out_t.data_ptr(), out_p.data_ptr(), nat.ptr(out_f),
+                ws.data_ptr(), ws.numel(), dtype, _stream(dev))
+        nat.check(rc, "lc_beam_select")
+    return (out_s, out_t, out_p) if finished is None else (out_s, out_t, out_p, out_f)
+
+
+def paged_kv_reorder(key_pages: torch.Tensor, value_pages: torch.Tensor,
+                     block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Make sequence w of group n continue what sequence parents[n, w] holds; returns
+    the new block table.
+
+    key_pages, value_pages [layers, num_pages, Hkv, P, D] (or 4-D: one layer),
+    which share one block_table int32 [B, pages]; parents int64 [N, W] with B =
+    N * W, each in [0, W) (others: the sequence itself). The sequences of a group
+    hold the same number of tokens, seq_lens[n * W] (int32 [B]), and own their
+    pages from the column being filled on. Whole pages are shared through the
+    table; of the page being filled, a parent's first child keeps it and the others
+    get copies, in the pages of sequences that nobody continues (written in place
+    in the pools). out: an int32 [B, pages] buffer for the new table that does not
+    overlap block_table.
+    """
+    one = key_pages.dim() == 4
+    if key_pages.dim() not in (4, 5) or key_pages.shape != value_pages.shape:
+        raise ValueError("key_pages and value_pages must both be [layers, num_pages, kv_heads, "
+                         "page, dim]")
+    if key_pages.dtype != value_pages.dtype:
+        raise TypeError("key_pages and value_pages must share a dtype")
+    if key_pages.requires_grad or value_pages.requires_grad:
+        raise NotImplementedError("paged_kv_reorder writes the pools in place: they cannot "
+                                  "require grad")
+    if key_pages.stride() != value_pages.stride() or key_pages.stride(-1) != 1:
+        raise ValueError("key_pages and value_pages must share a layout with unit dim stride")
+    kp, vp = (key_pages.unsqueeze(0), value_pages.unsqueeze(0)) if one else (key_pages, value_pages)
+    L, num_pages, Hkv, P, D = kp.shape
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise TypeError("block_table and seq_lens must be int32")
+    if parents.dtype != torch.int64 or parents.dim() != 2:
+        raise TypeError("parents must be int64 [groups, beams]")
+    N, W = parents.shape
+    if block_table.dim() != 2 or block_table.shape[0] != N * W or seq_lens.shape != (N * W,):
+        raise ValueError(f"block_table must be [{N * W}, pages] and seq_lens [{N * W}] for "
+                         f"parents {(N, W)}")
+    if N and not 1 <= W <= 256:
+        raise ValueError(f"{W} beams: 1 to 256")
+    M = block_table.shape[1]
+    dtype = nat.lc_dtype(kp)
+    dev = nat.require_device(kp, vp, block_table, seq_lens, parents, out)
+    block_table = block_table if M < 2 or block_table.stride(1) == 1 else block_table.contiguous()
+    seq_lens, parents = seq_lens.contiguous(), parents.contiguous()
+    if out is None:
+        out = torch.empty((N * W, M), dtype=torch.int32, device=dev)
+    elif out.dtype != torch.int32 or out.shape != (N * W, M) or (M > 1 and out.stride(1) != 1):
+        raise ValueError(f"out must be int32 {(N * W, M)} with contiguous rows")
+    if N * W and M:
+        lib = nat.load()
+        with _guard(dev):
+            rc = lib.lc_paged_kv_reorder(
+                kp.data_ptr(), vp.data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2),
+                kp.stride(3), L, num_pages, block_table.data_ptr(),
+                max(block_table.stride(0), M), out.data_ptr(), max(out.stride(0), M), M,
+                seq_lens.data_ptr(), parents.data_ptr(), N, W, Hkv, D, P, dtype, _stream(dev))
+        nat.check(rc, "lc_paged_kv_reorder")
+    return out

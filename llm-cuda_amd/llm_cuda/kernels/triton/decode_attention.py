@@ -9,8 +9,12 @@
   [N, Hkv, P, D] through an int32 block table [B, max_pages] with ragged
   int32 seq_lens [B] (the reference could only decode a contiguous copy of a
   batch-1 cache, models/llama3/kv_cache.py:43-44,65-83).
+* `shared_prefix_decode_attention(q, key_pages, value_pages, prefix_table,
+  prefix_lens, block_table, seq_lens)` decodes a batch whose groups of sequences
+  share a prefix (the beams of a prompt, requests behind one system prompt): the
+  prefix's pages are read and multiplied once per group, not once per sequence.
 
-Both return out shaped like q; `return_lse=True` adds the fp32 natural-log
+All return out shaped like q; `return_lse=True` adds the fp32 natural-log
 logsumexp [B, Hq] of the scaled scores. The paged entry also takes the
 reference's additive attention_mask (the reference's decode predicate refuses
 masks and falls back to torch; that predicate keeps its answer here).
@@ -120,3 +124,24 @@ def paged_decode_attention(
                              return_lse=return_lse, split_tokens=split_tokens,
                              workspace=workspace, attention_mask=attention_mask,
                              uniform_length=uniform_length)
+
+
+def shared_prefix_decode_attention(
+    q: torch.Tensor,
+    key_pages: torch.Tensor,
+    value_pages: torch.Tensor,
+    prefix_table: torch.Tensor,
+    prefix_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scale: float | None = None,
+    return_lse: bool = False,
+):
+    """q [B, Hq, 1, D]; the pools [num_pages, Hkv, P, D] hold the prefixes' pages
+    (prefix_table int32 [N, pages], prefix_lens int32 [N]) and the sequences' own
+    (block_table int32 [B, pages], seq_lens int32 [B]). The batch is N groups of
+    B / N consecutive sequences; each attends to its group's prefix and to its own
+    tokens, in one softmax. Table entries outside the pool are skipped; a sequence
+    without tokens gives zeros (lse -inf)."""
+    return _ops.shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens,
+                                     block_table, seq_lens, scale=scale, return_lse=return_lse)
