@@ -131,6 +131,329 @@ __global__ __launch_bounds__(64) void shared_generic_kernel(SharedArgs a) {
   if (lane == 0) a.part_lse[pidx] = l_run == 0.f ? -INFINITY : m_run + lc_log2(l_run);
 }
 
+// ---------------------------------------------------------------------------
+// MFMA kernel (bf16/f16, head_dim a multiple of 8 up to 128, pages of a power of two): one workgroup of 4
+// waves per (token range, 32 WR rows). A prefix's rows are the W G query heads of
+// its sequences that share a kv head, row r = w G + g; a sequence's own rows are
+// its G heads. Tiles of 64 tokens go through LDS (double-buffered, by DMA), so a
+// byte of K and V is read once for all rows of the workgroup:
+//   S^T[64 tok x 32 rows] = K Q^T, O^T[d x 32 rows] += V^T P^T   (32x32x16 MFMA)
+// The waves share the tile as WR row tiles x WK token halves: with 128 rows each
+// wave has 32 rows and all 64 tokens, with fewer rows the tokens are halved and
+// the halves' softmax states joined through LDS at the end.
+// Tokens are named by a table, so every lane finds the address of its own 16-byte
+// chunk of a DMA; lanes whose token is past the range, whose page entry is invalid
+// or whose chunk is past head_dim read zeros instead, and their scores are masked.
+// The weights P are rounded to the data type for the second product, as the
+// matrix instructions take it: 2^-8 relative each in bf16, far below the output's
+// own rounding after they are averaged; their sum stays in fp32.
+// ---------------------------------------------------------------------------
+constexpr int kTile = 64;  // tokens per tile
+constexpr float kSharedRescaleLog2 = 8.0f;
+
+__device__ __attribute__((aligned(16))) const uint32_t shared_zeros[4] = {0, 0, 0, 0};
+
+struct RangeItem {
+  const int32_t* table;  // the token range's table row
+  int b0, row0, rows;    // row r is sequence b0 + r / G, head r % G of the kv head
+  int kvh, t_begin, t_end, slot;
+};
+
+template <typename T, int DPAD, int WR>
+__device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeItem& it,
+                                             LC_LDS char* lds_k0, LC_LDS char* lds_k1,
+                                             LC_LDS char* lds_v0, LC_LDS char* lds_v1) {
+  typedef Mfma32<T> Ops;
+  typedef typename Ops::v8 v8;
+  constexpr int KS = DPAD / 16, DTL = DPAD / 32, CPR = DPAD / 8;
+  constexpr int RPI = 64 / CPR;           // token rows per DMA instruction
+  constexpr int NIW = kTile / (RPI * 4);  // DMA instructions per wave and tensor
+  constexpr int ROW_B = DPAD * (int)sizeof(T);
+  constexpr int NKT = WR == 4 ? 2 : 1;  // 32-token blocks per wave and tile
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wave_s = __builtin_amdgcn_readfirstlane(wave);
+  const int l32 = lane & 31, hh = lane >> 5;
+  const int wr = WR == 4 ? wave : WR == 2 ? (wave & 1) : 0;
+  const int wk = WR == 4 ? 0 : WR == 2 ? (wave >> 1) : wave;
+  const bool active = wk < 2 && it.row0 + wr * 32 < it.rows;  // (wave-uniform)
+
+  // This lane's query row.
+  const int r_abs = it.row0 + wr * 32 + l32;
+  const bool row_ok = r_abs < it.rows;
+  const int r_safe = row_ok ? r_abs : it.row0;
+  const int b = it.b0 + r_safe / a.G;
+  const int h = it.kvh * a.G + r_safe % a.G;
+  v8 qop[KS];
+  {
+    const T* qh = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = (hh * (CPR / 2) + s) * 8;
+      const bool ok = row_ok && d0 < a.D;
+      const v8 x = *reinterpret_cast<const v8*>(qh + (ok ? d0 : 0));
+      qop[s] = ok ? x : v8{};
+    }
+  }
+
+  const T* kp = static_cast<const T*>(a.kp) + (int64_t)it.kvh * a.s_head;
+  const T* vp = static_cast<const T*>(a.vp) + (int64_t)it.kvh * a.s_head;
+  const T* zeros = reinterpret_cast<const T*>(shared_zeros);
+  // Pages of this lane's DMA rows of the tile at t0, and of the token it masks
+  // (past the range: an entry that is not used).
+  const int last_page = (it.t_end - 1) >> a.p_shift;
+  auto fetch = [&](int t0, int (&pg)[NIW], int& own) {
+#pragma unroll
+    for (int u = 0; u < NIW; ++u) {
+      const int tok = t0 + (wave * NIW + u) * RPI + lane / CPR;
+      pg[u] = it.table[min(tok >> a.p_shift, last_page)];
+    }
+    const int tok = t0 + (NKT == 2 ? lane : wk * 32 + l32);
+    own = it.table[min(tok >> a.p_shift, last_page)];
+  };
+  auto issue = [&](int t0, const int (&pg)[NIW], LC_LDS char* kd, LC_LDS char* vd) {
+#pragma unroll
+    for (int u = 0; u < NIW; ++u) {
+      const int row = (wave * NIW + u) * RPI + lane / CPR;
+      const int ch = (lane % CPR) ^ pf_swz<CPR>(row);
+      const int tok = t0 + row;
+      const bool ok = static_cast<unsigned>(pg[u]) < static_cast<unsigned>(a.num_pages) &&
+                      tok < it.t_end && ch * 8 < a.D;
+      const int slot = tok & (a.P - 1);
+      const int64_t off = (int64_t)pg[u] * a.s_page + (int64_t)slot * a.s_tok + ch * 8;
+      const T* ks = ok ? kp + off : zeros;
+      const T* vs = ok ? vp + off : zeros;
+      const int dst = (wave_s * NIW + u) * RPI * ROW_B;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)ks,
+                                       (LC_LDS void*)(kd + dst), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vs,
+                                       (LC_LDS void*)(vd + dst), 16, 0, 0);
+    }
+  };
+
+  // LDS addresses of the operands (see the prefill kernel's).
+  int kaddr[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    kaddr[s] = (wk < 2 ? wk * 32 : 0) * ROW_B + l32 * ROW_B +
+               (((hh * (CPR / 2) + s) ^ pf_swz<CPR>(l32)) << 4);
+  int vaddr[2][DTL];
+  {
+    const int gq = lane >> 4, te = (lane & 15) >> 2, tc = lane & 3;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+      for (int dt = 0; dt < DTL; ++dt) {
+        const int kr = jj * 8 + hh * 4 + te;
+        const int d = dt * 32 + (gq & 1) * 16 + 4 * tc;
+        vaddr[jj][dt] = ((wk < 2 ? wk * 32 : 0) + kr) * ROW_B +
+                        ((((d >> 3) ^ pf_swz<CPR>(kr)) << 4) | ((d & 7) * (int)sizeof(T)));
+      }
+  }
+
+  f32x16_t o[DTL];
+#pragma unroll
+  for (int i = 0; i < DTL; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  float m_ref = -INFINITY, l_lane = 0.f;
+
+  auto compute = [&](LC_LDS const char* kt_lds, LC_LDS const char* vt_lds, uint64_t live) {
+    f32x16_t x[NKT];
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[kt][r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+        x[kt] = Ops::mma(*reinterpret_cast<LC_LDS const v8*>(kt_lds + kaddr[s] + kt * 32 * ROW_B),
+                         qop[s], x[kt]);
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[kt][r] *= a.scale_log2;
+    constexpr uint64_t kAll = NKT == 2 ? ~0ull : 0xffffffffull;
+    if ((live & kAll) != kAll) {
+      const uint64_t mine = live >> (hh * 4);
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((mine >> (kt * 32 + (r >> 2) * 8 + (r & 3))) & 1)) x[kt][r] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[kt][r]);
+    mx = pf_half_max(mx);
+    // The reference max only moves when some row's max grew by more than 2^8
+    // (exact: O and l share it).
+    if (__ballot(mx > m_ref + kSharedRescaleLog2)) {
+      const float m_new = fmaxf(m_ref, mx);
+      const float alpha = m_new == -INFINITY ? 1.f : lc_exp2(m_ref - m_new);
+      l_lane *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+      m_ref = m_new;
+    }
+    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+    v8 pop[NKT][2];
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = lc_exp2(x[kt][r] - m_use);
+        l_lane += p;
+        pop[kt][r >> 3][r & 7] = static_cast<T>(p);
+      }
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+      for (int jp = 0; jp < 2; ++jp)
+#pragma unroll
+        for (int dt = 0; dt < DTL; ++dt) {
+          const int rowoff = (kt * 32 + jp * 16) * ROW_B;
+          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (LC_LDS i16x4_t*)(vt_lds + vaddr[0][dt] + rowoff));
+          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (LC_LDS i16x4_t*)(vt_lds + vaddr[1][dt] + rowoff));
+          const i16x8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          o[dt] = Ops::mma(__builtin_bit_cast(v8, both), pop[kt][jp], o[dt]);
+        }
+  };
+
+  // Tile t computes from one buffer while tile t + 1 arrives in the other and the
+  // page entries of tile t + 2 are on their way.
+  int pg[NIW], own, own_next;
+  fetch(it.t_begin, pg, own);
+  issue(it.t_begin, pg, lds_k0, lds_v0);
+  fetch(it.t_begin + kTile, pg, own_next);
+  auto step = [&](int t, LC_LDS char* kc, LC_LDS char* vc, LC_LDS char* kn, LC_LDS char* vn) {
+    pf_barrier<true>();  // tile t is in LDS; the other buffer's reads are done
+    if (t + kTile < it.t_end) issue(t + kTile, pg, kn, vn);
+    const uint64_t live =
+        __ballot(static_cast<unsigned>(own) < static_cast<unsigned>(a.num_pages) &&
+                 t + (NKT == 2 ? lane : wk * 32 + l32) < it.t_end);
+    own = own_next;
+    fetch(t + 2 * kTile, pg, own_next);
+    if (active && live != 0) compute(kc, vc, live);
+  };
+  for (int t = it.t_begin; t < it.t_end; t += 2 * kTile) {
+    step(t, lds_k0, lds_v0, lds_k1, lds_v1);
+    if (t + kTile < it.t_end) step(t + kTile, lds_k1, lds_v1, lds_k0, lds_v0);
+  }
+
+  float l_tot = l_lane;
+  {
+    const unsigned u = __float_as_uint(l_lane);
+    const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    l_tot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  if constexpr (WR != 4) {
+    // The second token half's state goes to the first half's wave: O in the K
+    // buffers, [row tile][register][lane], then m and l.
+    __syncthreads();
+    LC_LDS float* rec = (LC_LDS float*)(wr == 0 ? lds_k0 : lds_k1);
+    LC_LDS float* ml = (LC_LDS float*)lds_v0 + wr * 128;
+    if (wk == 1) {
+#pragma unroll
+      for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) rec[(dt * 16 + r) * 64 + lane] = o[dt][r];
+      ml[lane] = m_ref;
+      ml[64 + lane] = l_tot;
+    }
+    __syncthreads();
+    if (wk != 0) return;
+    const float m2 = ml[lane], l2 = ml[64 + lane];
+    const float m = fmaxf(m_ref, m2);
+    const float w1 = m_ref == -INFINITY ? (l_tot == 0.f ? 0.f : 1.f) : lc_exp2(m_ref - m);
+    const float w2 = m2 == -INFINITY ? (l2 == 0.f ? 0.f : 1.f) : lc_exp2(m2 - m);
+    l_tot = l_tot * w1 + l2 * w2;
+#pragma unroll
+    for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = o[dt][r] * w1 + rec[(dt * 16 + r) * 64 + lane] * w2;
+    m_ref = m;
+  }
+  if (!row_ok) return;
+  const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
+  const float inv_l = l_tot == 0.f ? 0.f : 1.0f / l_tot;
+  float* po = a.part_o + pidx * a.D;
+#pragma unroll
+  for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d0 = dt * 32 + j * 8 + hh * 4;
+      if (d0 < a.D) {
+        f32x4_t w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = o[dt][j * 4 + e] * inv_l;
+        *reinterpret_cast<f32x4_t*>(po + d0) = w;
+      }
+    }
+  if (hh == 0) a.part_lse[pidx] = l_tot == 0.f ? -INFINITY : m_ref + lc_log2(l_tot);
+}
+
+// Workgroups below p_blocks take the prefixes' ranges, the others the sequences'
+// own. A prefix range's row tiles read the same K and V: they get block ids 8
+// apart, which run on one XCD, and find it in its L2.
+template <typename T, int DPAD, int WR>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
+  constexpr int TILE_B = kTile * DPAD * (int)sizeof(T);
+  // (separate arrays: the compiler tracks a DMA by the array that it writes)
+  __shared__ __align__(16) char lds_k0[TILE_B];
+  __shared__ __align__(16) char lds_k1[TILE_B];
+  __shared__ __align__(16) char lds_v0[TILE_B];
+  __shared__ __align__(16) char lds_v1[TILE_B];
+  RangeItem it;
+  const int id = blockIdx.x;
+  if (id < p_blocks) {
+    const int run = id / (8 * row_tiles), rest = id - run * 8 * row_tiles;
+    const int pair = run * 8 + (rest & 7), tile = rest >> 3;
+    const int units = (a.B / a.W) * a.Hkv;
+    const int split = pair / units, u = pair - split * units;
+    if (split >= a.p_splits) return;
+    const int n = u / a.Hkv;
+    const int len = clamp_len(a.plens[n], a.p_pages, a.P);
+    const int each = range_tokens(len, a.p_splits);
+    it.t_begin = split * each;
+    if (it.t_begin >= len) return;
+    it.t_end = min(len, it.t_begin + each);
+    it.table = a.ptab + (int64_t)n * a.ptab_stride;
+    it.kvh = u - n * a.Hkv;
+    it.b0 = n * a.W;
+    it.rows = a.W * a.G;
+    it.row0 = tile * 32 * WR;
+    it.slot = split;
+    shared_range<T, DPAD, WR>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
+                              (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1);
+  } else {
+    const int units = a.B * a.Hkv * head_groups;
+    const int split = (id - p_blocks) / units, u = id - p_blocks - split * units;
+    const int hg = u % head_groups, bk = u / head_groups;
+    const int b = bk / a.Hkv;
+    const int len = clamp_len(a.slens[b], a.s_pages, a.P);
+    const int each = range_tokens(len, a.s_splits);
+    it.t_begin = split * each;
+    if (it.t_begin >= len) return;
+    it.t_end = min(len, it.t_begin + each);
+    it.table = a.btab + (int64_t)b * a.btab_stride;
+    it.kvh = bk - b * a.Hkv;
+    it.b0 = b;
+    it.rows = a.G;
+    it.row0 = hg * 32;
+    it.slot = a.p_splits + split;
+    shared_range<T, DPAD, 1>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
+                              (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1);
+  }
+}
+
 // Merge: one wave per (sequence, query head) joins the live ranges of its
 // prefix and of its own tokens; each lane owns VPL consecutive floats of
 // head_dim. A row without tokens gets out = 0, lse = -inf.
@@ -199,24 +522,27 @@ __global__ __launch_bounds__(64) void shared_merge_kernel(SharedArgs a, T* __res
 }
 
 struct SharedPlan {
+  int wr;  // a prefix workgroup's row tiles of 32
   int p_splits, s_splits;
 };
 
-// Ranges per prefix and per sequence: about one round of the CUs over all
-// tokens, no range shorter than two steps.
+// Ranges per prefix and per sequence: about one round of the workgroups that the
+// CUs hold at once (two each) over all tokens, no range shorter than two tiles.
 SharedPlan shared_plan(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_cap,
                        int64_t s_cap) {
+  if (B == 0) return SharedPlan{1, 0, 0};
   const int64_t G = Hq / Hkv, W = B / N;
-  const int64_t up = N * Hkv * lc_cdiv(W * G, 128), us = B * Hkv * lc_cdiv(G, 32);
+  const int wr = W * G <= 32 ? 1 : W * G <= 64 ? 2 : 4;
+  const int64_t up = N * Hkv * lc_cdiv(W * G, 32 * wr), us = B * Hkv * lc_cdiv(G, 32);
   const int64_t total = up * p_cap + us * s_cap;
-  int64_t each = lc_cdiv(total, lc_cu_count());
+  int64_t each = lc_cdiv(total, 2 * lc_cu_count());
   if (each < 2 * kSharedStep) each = 2 * kSharedStep;
   auto splits = [&](int64_t cap) -> int {
     if (cap == 0) return 0;
     const int64_t s = lc_cdiv(cap, each);
     return static_cast<int>(s < 64 ? s : 64);
   };
-  return SharedPlan{splits(p_cap), splits(s_cap)};
+  return SharedPlan{wr, splits(p_cap), splits(s_cap)};
 }
 
 int64_t shared_bytes(int64_t rows, int64_t D, const SharedPlan& p) {
@@ -238,11 +564,36 @@ int launch_merge(const SharedArgs& a, void* out, int64_t o_sb, int64_t o_sh, flo
   return lc_check_launch("lc_shared_prefix_decode_fwd (merge)");
 }
 
+template <typename T, int DPAD>
+int launch_mfma(const SharedArgs& a, int wr, hipStream_t st) {
+  const int64_t row_tiles = lc_cdiv((int64_t)a.W * a.G, 32 * wr), head_groups = lc_cdiv(a.G, 32);
+  const int64_t pairs = (int64_t)(a.B / a.W) * a.Hkv * a.p_splits;
+  const int64_t p_blocks = lc_cdiv(pairs, 8) * 8 * row_tiles;
+  const int64_t blocks = p_blocks + (int64_t)a.B * a.Hkv * head_groups * a.s_splits;
+  LC_REQUIRE(blocks < (1LL << 24), "lc_shared_prefix_decode_fwd: %lld workgroups",
+             (long long)blocks);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  const int pb = static_cast<int>(p_blocks), rt = static_cast<int>(row_tiles),
+            hg = static_cast<int>(head_groups);
+  if (wr == 1)
+    shared_mfma_kernel<T, DPAD, 1><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+  else if (wr == 2)
+    shared_mfma_kernel<T, DPAD, 2><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+  else
+    shared_mfma_kernel<T, DPAD, 4><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+  return lc_check_launch("lc_shared_prefix_decode_fwd (mfma)");
+}
+
 template <typename T>
-int launch_shared(const SharedArgs& a, void* out, int64_t o_sb, int64_t o_sh, float* lse,
-                  hipStream_t st) {
+int launch_shared(const SharedArgs& a, int wr, bool mfma, void* out, int64_t o_sb, int64_t o_sh,
+                  float* lse, hipStream_t st) {
   const int splits = a.p_splits + a.s_splits;
-  if (splits > 0) {
+  if (splits > 0 && mfma) {
+    if constexpr (sizeof(T) == 2) {
+      const int rc = a.D <= 64 ? launch_mfma<T, 64>(a, wr, st) : launch_mfma<T, 128>(a, wr, st);
+      if (rc != LC_OK) return rc;
+    }
+  } else if (splits > 0) {
     shared_generic_kernel<T><<<dim3(splits, a.Hq, a.B), 64, 0, st>>>(a);
     const int rc = lc_check_launch("lc_shared_prefix_decode_fwd (generic)");
     if (rc != LC_OK) return rc;
@@ -341,14 +692,18 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
   a.p_splits = plan.p_splits;
   a.s_splits = plan.s_splits;
   a.scale_log2 = scale * kLog2e;
+  const bool mfma = dtype != LC_DTYPE_F32 && D % 8 == 0 && D <= 128 && q_sb % 8 == 0 &&
+                    q_sh % 8 == 0 && kv_s_page % 8 == 0 && kv_s_head % 8 == 0 &&
+                    kv_s_tok % 8 == 0 && a.p_shift >= 0 && lc_aligned(q, 16) && lc_aligned(key_pages, 16) &&
+                    lc_aligned(value_pages, 16);
   hipStream_t st = lc_stream(stream);
   switch (dtype) {
     case LC_DTYPE_F32:
-      return launch_shared<float>(a, out, o_sb, o_sh, lse, st);
+      return launch_shared<float>(a, plan.wr, false, out, o_sb, o_sh, lse, st);
     case LC_DTYPE_BF16:
-      return launch_shared<bf16_t>(a, out, o_sb, o_sh, lse, st);
+      return launch_shared<bf16_t>(a, plan.wr, mfma, out, o_sb, o_sh, lse, st);
     default:
-      return launch_shared<f16_t>(a, out, o_sb, o_sh, lse, st);
+      return launch_shared<f16_t>(a, plan.wr, mfma, out, o_sb, o_sh, lse, st);
   }
 }
 
