@@ -2,6 +2,8 @@
 // over beams and vocabulary, and the reordering of the caches that follows it.
 #include <math.h>
 
+#include <type_traits>
+
 #include "lc_common.h"
 
 namespace {
@@ -16,11 +18,10 @@ namespace {
 // into registers) gives each chunk's K best and its part of the softmax sum; a
 // second, small launch joins the chunks: one workgroup per group.
 //
-// A chunk's K best without a sort: the K-th largest of a wave's 64 lane maxima
-// (found bit by bit on ballots) bounds the chunk's K-th largest from below, so
-// only elements that reach the best such bound of the four waves are gathered
-// (about K to 2K of them); each one's rank is the number of gathered keys above
-// it. Keys are (order-preserving bits of the logit, inverted index): all are
+// A chunk's K best without a sort: the k-th largest of a wave's 64 lane maxima
+// (found on ballots, two bits at a time) bounds the chunk's K-th largest from
+// below, so only elements that reach the bound are gathered (little more than K);
+// each one's rank is the number of gathered keys above it. Keys are (order-preserving bits of the logit, inverted index): all are
 // different, and ties rank by index.
 //
 // The order of candidates of different beams hangs on their lse: the terms of
@@ -32,7 +33,8 @@ constexpr int kBeamThreads = 256;
 constexpr int kBeamWaves = kBeamThreads / 64;
 constexpr int kMaxCount = 64;      // candidates per group: lanes of a wave
 constexpr int kMaxWidth = 256;     // beams per group: threads of a workgroup
-constexpr int kChunkCap = 1024;    // gathered keys of a chunk
+constexpr int kWaveCap = 256;      // gathered keys of a chunk's wave
+constexpr int kTieSlack = 32;      // lanes past the K-th at its value before ties are cut by index
 constexpr int kMergeCap = 2048;    // gathered candidates of a group
 
 // Order-preserving bits of a float (not NaN); -0 counts as +0.
@@ -54,14 +56,49 @@ __device__ __forceinline__ double from_ordered64(uint64_t k) {
   return __builtin_bit_cast(double, k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull));
 }
 
-// The largest t that at least `count` of the wave's keys reach, bits `top` .. 0.
-__device__ __forceinline__ uint32_t wave_kth_largest(uint32_t key, int count, int top) {
+// The largest t with the bits below LOW clear that at least `count` of the wave's
+// keys reach, two bits at a time (the three compares of a step are independent).
+template <int TOP, int LOW>
+__device__ __forceinline__ uint32_t wave_kth_largest(uint32_t key, int count) {
+  static_assert((TOP - LOW) % 2 == 1, "whole pairs of bits");
   uint32_t t = 0;
-  for (int bit = top; bit >= 0; --bit) {
-    const uint32_t c = t | (1u << bit);
-    if (__popcll(__ballot(key >= c)) >= count) t = c;
+#pragma unroll
+  for (int bit = TOP - 1; bit >= LOW; bit -= 2) {
+    const uint32_t c1 = t | (1u << bit), c2 = t | (2u << bit), c3 = t | (3u << bit);
+    const int n1 = __popcll(__ballot(key >= c1)), n2 = __popcll(__ballot(key >= c2)),
+              n3 = __popcll(__ballot(key >= c3));
+    t = n3 >= count ? c3 : n2 >= count ? c2 : n1 >= count ? c1 : t;
   }
   return t;
+}
+
+// The lowest bit of ordered(x) that tells values of T apart; those below it are
+// all clear (x >= 0) or all set.
+template <typename T>
+constexpr int ordered_low() { return 0; }
+template <>
+constexpr int ordered_low<bf16_t>() { return 16; }
+template <>
+constexpr int ordered_low<f16_t>() { return 12; }
+
+// Wave reductions on DPP moves (shifts inside rows of 16 lanes, then the row totals
+// broadcast to the rows after them); the result is in lane 63.
+template <typename F>
+__device__ __forceinline__ float wave_reduce(float x, float none, F op) {
+  auto step = [&](auto ctrl, auto rows) {
+    const int moved = __builtin_amdgcn_update_dpp(
+        __float_as_int(none), __float_as_int(x), decltype(ctrl)::value, decltype(rows)::value, 0xf,
+        false);
+    x = op(x, __int_as_float(moved));
+  };
+  typedef std::integral_constant<int, 0xf> All;
+  step(std::integral_constant<int, 0x111>(), All());  // row_shr:1
+  step(std::integral_constant<int, 0x112>(), All());
+  step(std::integral_constant<int, 0x114>(), All());
+  step(std::integral_constant<int, 0x118>(), All());
+  step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());  // row_bcast:15
+  step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());  // row_bcast:31
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
 struct SelectArgs {
@@ -92,107 +129,178 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
   constexpr int VEC = 16 / sizeof(T);
   constexpr int CHUNK = kBeamThreads * ITEMS;
   static_assert(ITEMS % VEC == 0, "whole vectors per thread");
-  __shared__ uint64_t list[kChunkCap];
-  __shared__ uint64_t bound[kBeamWaves];
+  static_assert(CHUNK < (1 << 14), "inverted indices inside a chunk are 14 bits");
+  __shared__ uint64_t list[kBeamWaves][kWaveCap];
+  __shared__ uint64_t bound_k[kBeamWaves], bound_q[kBeamWaves];
   __shared__ float w_top[kBeamWaves], w_sum[kBeamWaves];
-  __shared__ int count;
+  __shared__ int found[kBeamWaves];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / a.chunks;
   const int chunk = blockIdx.x - static_cast<int>(row) * a.chunks;
-  if (a.finished != nullptr && a.finished[row]) return;
+  // (few rows: the flag arrives with the logits instead of before them)
+  const bool done = a.finished != nullptr && a.finished[row] != 0;
+  if (ITEMS > 8 && done) return;
   const int64_t n = row / a.W;
   const T* x = static_cast<const T*>(a.logits) + n * a.s_group + (row - n * a.W) * a.s_beam;
   const int c0 = chunk * CHUNK;
 
-  // Element i of this thread: index c0 + (i / VEC) * 256 VEC + tid VEC + i % VEC,
-  // whatever the row's alignment, so equal rows give equal sums.
+  // Element i of this thread, in the chunk; whatever the row's alignment, so equal
+  // rows give equal sums.
+  auto index_of = [&](int i) -> uint32_t {
+    return ((i / VEC) * kBeamThreads + tid) * VEC + i % VEC;
+  };
   float v[ITEMS];
+  if (a.V >= VEC) {
+    // Every load is issued before the first is used; a vector across the row's end
+    // is read again element by element, one past it reads the row's last ones.
+    Vec16<T> raw[ITEMS / VEC];
 #pragma unroll
-  for (int j = 0; j < ITEMS / VEC; ++j) {
-    const int at = c0 + (j * kBeamThreads + tid) * VEC;
-    if (at + VEC <= a.V) {
-      const Vec16<T> raw = load16_any(x + at);
+    for (int j = 0; j < ITEMS / VEC; ++j)
+      raw[j] = load16_any(x + min(c0 + static_cast<int>(index_of(j * VEC)), a.V - VEC));
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[j * VEC + e] = lc_to_f32(raw.v[e]);
-    } else {
+    for (int i = 0; i < ITEMS; ++i) v[i] = lc_to_f32(raw[i / VEC].v[i % VEC]);
+    if (ITEMS <= 8 && done) return;
+    if (c0 + CHUNK > a.V) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[j * VEC + e] = at + e < a.V ? lc_to_f32(x[at + e]) : -INFINITY;
+      for (int j = 0; j < ITEMS / VEC; ++j) {
+        const int at = c0 + static_cast<int>(index_of(j * VEC));
+        if (at + VEC > a.V) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e)
+            v[j * VEC + e] = at + e < a.V ? lc_to_f32(x[at + e]) : -INFINITY;
+        }
+      }
+    }
+  } else {
+    if (done) return;
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int at = c0 + static_cast<int>(index_of(i));
+      v[i] = at < a.V ? lc_to_f32(x[at]) : -INFINITY;
     }
   }
-  if (tid == 0) count = 0;
 
-  // This wave's part of the softmax sum. NaN and +inf make it NaN.
-  float top = -INFINITY;
+  // This wave's part of the softmax sum, relative to its largest logit. NaN and
+  // +inf make it NaN. 2^(v L - r) with r = ref L rounded: one rounding of the
+  // argument per term, and the factor 2^(ref L - r), common to all, taken off.
+  float top = v[0];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) top = fmaxf(top, v[i]);
-  const float w_max = lc_wave_max(top);
+  for (int i = 1; i < ITEMS; ++i) top = fmaxf(top, v[i]);
+  if (!(top >= -INFINITY)) top = -INFINITY;  // (all NaN)
+  const float w_max = wave_reduce(top, -INFINITY, [](float p, float q) { return fmaxf(p, q); });
   const float ref = w_max == -INFINITY ? 0.f : w_max;
-  float sum = 0.f;
+  float part[4] = {0.f, 0.f, 0.f, 0.f}, scale = 1.f;
+  if (fabsf(ref) < 1e30f) {
+    const float shift = ref * kLog2e;
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) sum += lc_exp2((v[i] - ref) * kLog2e);
-  sum = lc_wave_sum(sum);
+    for (int i = 0; i < ITEMS; ++i) part[i % 4] += lc_exp2(fmaf(v[i], kLog2e, -shift));
+    scale = lc_exp2(-fmaf(ref, kLog2e, -shift));
+  } else {  // (ref L may not be finite)
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) part[i % 4] += lc_exp2((v[i] - ref) * kLog2e);
+  }
+  const float sum = wave_reduce((part[0] + part[1]) + (part[2] + part[3]), 0.f,
+                                [](float p, float q) { return p + q; }) * scale;
 
-  // The wave's bound: the K-th largest (value, lowest index) of its lanes.
+  // Two lower bounds of the chunk's K-th largest from the lanes' largest values:
+  // the K-th largest of one wave, and the least of the waves' q-th largest, q = K /
+  // 4 rounded up. The first always holds enough; the second, where all waves are
+  // alike, little more. Elements equal to a bound count up to an index.
   const uint32_t key = ordered(top);
-  const uint32_t t = wave_kth_largest(key, a.K, 31);
-  uint32_t t_index = 0xffffffffu;  // of elements equal to t: those of at most this index
-  if (__popcll(__ballot(key >= t)) > a.K) {
-    // More lanes than needed at t: the lowest indices among them are enough.
-    uint32_t low = 0;  // inverted lowest index of this lane's elements equal to t
-    if (key == t) {
-      const float tv = from_ordered(t);
+  constexpr int LOW = ordered_low<T>();
+  auto whole = [](uint32_t t) {  // (a negative value's bits below LOW are set)
+    return t < 0x80000000u ? t | ((1u << LOW) - 1) : t;
+  };
+  const uint32_t t = whole(wave_kth_largest<31, LOW>(key, a.K));
+  const int q = (a.K + kBeamWaves - 1) / kBeamWaves;
+  const uint32_t tq = q == 1 ? ordered(w_max) : whole(wave_kth_largest<31, LOW>(key, q));
+  uint32_t t_index = CHUNK - 1;
+  if (__popcll(__ballot(key >= t)) > a.K + kTieSlack) {
+    // Far more lanes than needed reach t: the lowest indices among those at t do.
+    const float tv = from_ordered(t);
+    uint32_t low = 0;  // one more than the inverted lowest index of this lane's at t
 #pragma unroll
-      for (int i = ITEMS - 1; i >= 0; --i)
-        if (v[i] == tv) low = ~static_cast<uint32_t>(((i / VEC) * kBeamThreads + tid) * VEC + i % VEC) & 0x1fffu;
-    }
+    for (int i = ITEMS - 1; i >= 0; --i)
+      if (v[i] == tv) low = CHUNK - index_of(i);
     const int more = a.K - __popcll(__ballot(key > t));
-    static_assert(CHUNK <= 0x2000, "indices inside a chunk are 13 bits");
-    const uint32_t kth = wave_kth_largest(key == t ? low + 1 : 0, more, 13);
-    t_index = 0x1fffu - (kth - 1);
+    t_index = CHUNK - wave_kth_largest<13, 0>(key == t ? low : 0, more);
   }
   if (lane == 0) {
     w_top[wave] = w_max;
     w_sum[wave] = sum;
-    bound[wave] = (static_cast<uint64_t>(t) << 32) | static_cast<uint32_t>(~t_index);
+    bound_k[wave] = (static_cast<uint64_t>(t) << 32) | (CHUNK - t_index);
+    bound_q[wave] = (static_cast<uint64_t>(tq) << 32) | 1;
   }
   __syncthreads();
-  uint64_t limit = bound[0];
+  uint64_t limit = bound_k[0], least = bound_q[0];
 #pragma unroll
-  for (int w = 1; w < kBeamWaves; ++w) limit = max(limit, bound[w]);
+  for (int w = 1; w < kBeamWaves; ++w) {
+    limit = max(limit, bound_k[w]);
+    least = min(least, bound_q[w]);
+  }
+  limit = max(limit, least);
+  const float lim = from_ordered(static_cast<uint32_t>(limit >> 32));
+  const uint32_t lim_index = CHUNK - static_cast<uint32_t>(limit);
 
-  auto key_of = [&](int i) -> uint64_t {
-    const uint32_t at = ((i / VEC) * kBeamThreads + tid) * VEC + i % VEC;
+  auto key_of = [&](int i) -> uint64_t {  // (NaN: below every number; its beam's list is not used)
     const float f = v[i] == v[i] ? v[i] : -INFINITY;
-    return (static_cast<uint64_t>(ordered(f)) << 32) | static_cast<uint32_t>(~at);
+    return (static_cast<uint64_t>(ordered(f)) << 32) | ~static_cast<uint32_t>(index_of(i));
   };
-  if (key >= static_cast<uint32_t>(limit >> 32)) {
+  // Gather what reaches the bound, each wave into its own part of the list.
+  int n_found = 0;
+  if (__ballot(top >= lim)) {
+    auto gather = [&](int i, bool hit) {
+      const unsigned long long hits = __ballot(hit);
+      if (hits == 0) return;
+      const int pos = n_found + __builtin_amdgcn_mbcnt_hi(
+                                    static_cast<uint32_t>(hits >> 32),
+                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hits), 0));
+      if (hit && pos < kWaveCap) list[wave][pos] = key_of(i);
+      n_found += __popcll(hits);
+    };
+    if (lim_index == CHUNK - 1) {
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      const uint64_t k = key_of(i);
-      if (k >= limit) {
-        const int pos = atomicAdd(&count, 1);
-        if (pos < kChunkCap) list[pos] = k;
-      }
+      for (int i = 0; i < ITEMS; ++i) gather(i, v[i] >= lim);
+    } else {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i)
+        gather(i, v[i] > lim || (v[i] == lim && index_of(i) <= lim_index));
     }
   }
+  if (lane == 0) found[wave] = n_found;
   __syncthreads();
-  const int m = count;
+  int m = 0, most = 0, before[kBeamWaves];
+#pragma unroll
+  for (int w = 0; w < kBeamWaves; ++w) {
+    before[w] = m;
+    m += found[w];
+    most = max(most, found[w]);
+  }
   uint64_t* out = a.keys + (row * a.chunks + chunk) * a.K;
   // (stored with the index in the row, not in the chunk)
   auto store = [&](int rank, uint64_t k) {
     out[rank] = (k & 0xffffffff00000000ull) |
                 static_cast<uint32_t>(~(~static_cast<uint32_t>(k) + static_cast<uint32_t>(c0)));
   };
-  if (m <= kChunkCap) {
-    for (int i = tid; i < m; i += kBeamThreads) {
-      const uint64_t k = list[i];
+  if (most <= kWaveCap) {
+    // Four threads count the keys above each one, a wave's part of the list each.
+    static_assert(kBeamWaves == 4, "a thread per part");
+    const int seg = tid & 3, n_seg = found[seg];
+    for (int i = tid >> 2; i < (m + 15) / 16 * 16; i += kBeamThreads / 4) {
+      int at = 0;
+#pragma unroll
+      for (int w = 1; w < kBeamWaves; ++w) at = i >= before[w] ? w : at;
+      const uint64_t k = i < m ? list[at][i - before[at]] : ~0ull;
       int rank = 0;
-      for (int j = 0; j < m; ++j) rank += list[j] > k;
-      if (rank < a.K) store(rank, k);
+#pragma unroll 4
+      for (int j = 0; j < n_seg; ++j) rank += list[seg][j] > k;
+      rank += __shfl_xor(rank, 1, 64);
+      rank += __shfl_xor(rank, 2, 64);
+      if (seg == 0 && i < m && rank < a.K) store(rank, k);
     }
   } else {
-    // Values laid out against the bound (few lanes hold most of the best): the
+    // Values laid out against the bounds (few lanes hold most of the best): the
     // largest key below the last one, K times.
     uint64_t last = ~0ull;
     for (int r = 0; r < a.K; ++r) {
@@ -208,10 +316,10 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
         best = max(best, other);
       }
       __syncthreads();
-      if (lane == 0) bound[wave] = best;
+      if (lane == 0) bound_k[wave] = best;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kBeamWaves; ++w) best = max(best, bound[w]);
+      for (int w = 0; w < kBeamWaves; ++w) best = max(best, bound_k[w]);
       if (tid == 0) store(r, best);
       last = best;
     }
@@ -237,24 +345,49 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
 // everywhere) and undefined (NaN or +inf in the logits or the score: NaN).
 enum : int { kBeamOrdinary = 0, kBeamFinished, kBeamEmpty, kBeamUndefined };
 
-__global__ __launch_bounds__(kBeamThreads) void beam_merge_kernel(SelectArgs a) {
+constexpr int kMergeThreads = 1024;
+constexpr int kMergeWaves = kMergeThreads / 64;
+
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
   __shared__ double base[kMaxWidth];  // score - ln of the sum relative to `peak`
   __shared__ float peak[kMaxWidth];   // the beam's largest logit
   __shared__ int kind[kMaxWidth];
   __shared__ uint64_t value[kMergeCap];
   __shared__ uint32_t flat[kMergeCap];  // inverted w V + v
-  __shared__ uint32_t bound[kBeamWaves];
-  __shared__ uint64_t best_v[kBeamWaves];
-  __shared__ uint32_t best_f[kBeamWaves];
-  __shared__ int count;
+  __shared__ int reach[kMergeCap];      // lists whose best candidate reaches the bound
+  __shared__ uint32_t bound[kMergeWaves];
+  __shared__ uint64_t best_v[kMergeWaves];
+  __shared__ uint32_t best_f[kMergeWaves];
+  __shared__ int count, reached;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t n = blockIdx.x;
-  const int K = a.K;
-  if (tid == 0) count = 0;
-  for (int w = wave; w < a.W; w += kBeamWaves) {
+  const int K = a.K, lists = a.W * a.chunks;
+  if (tid == 0) count = reached = 0;
+  // Few candidates: every thread's kHeld of them, the lists' first ones first, are
+  // loaded before the sums are joined; else only the lists that turn out to matter.
+  constexpr int kHeld = 2;
+  const bool few = lists * K <= kHeld * kMergeThreads;
+  uint64_t held[kHeld];
+  int held_l[kHeld], held_k[kHeld];
+  if (few) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+      const uint32_t i = tid + r * kMergeThreads;
+      held_k[r] = static_cast<int>(i / static_cast<uint32_t>(lists));
+      held_l[r] = static_cast<int>(i) - held_k[r] * lists;
+      held[r] = a.keys[(n * lists + held_l[r]) * K + min(held_k[r], K - 1)];
+    }
+  }
+  for (int w = wave; w < a.W; w += kMergeWaves) {
     const int64_t row = n * a.W + w;
     const float score = a.scores[row];
+    float t0 = -INFINITY;
+    double s0 = 0;
+    if (lane < a.chunks) {  // (with the score: one round trip for up to 64 chunks)
+      t0 = a.tops[row * a.chunks + lane];
+      s0 = a.sums[row * a.chunks + lane];
+    }
     if (a.finished != nullptr && a.finished[row]) {
       if (lane == 0) {
         kind[w] = kBeamFinished;
@@ -262,15 +395,15 @@ __global__ __launch_bounds__(kBeamThreads) void beam_merge_kernel(SelectArgs a) 
       }
       continue;
     }
-    float top = -INFINITY;
-    for (int c = lane; c < a.chunks; c += 64) top = fmaxf(top, a.tops[row * a.chunks + c]);
+    float top = t0;
+    for (int c = lane + 64; c < a.chunks; c += 64) top = fmaxf(top, a.tops[row * a.chunks + c]);
     top = lc_wave_max(top);
-    double sum = 0;
-    for (int c = lane; c < a.chunks; c += 64) {
-      const float t = a.tops[row * a.chunks + c];
-      const double s = a.sums[row * a.chunks + c];
-      sum += t == -INFINITY ? s : s * exp(static_cast<double>(t) - top);
-    }
+    auto weighed = [&](float t, double s) {
+      return t == -INFINITY ? s : s * exp(static_cast<double>(t) - top);
+    };
+    double sum = weighed(t0, s0);
+    for (int c = lane + 64; c < a.chunks; c += 64)
+      sum += weighed(a.tops[row * a.chunks + c], a.sums[row * a.chunks + c]);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if (lane == 0) {
@@ -286,22 +419,21 @@ __global__ __launch_bounds__(kBeamThreads) void beam_merge_kernel(SelectArgs a) 
   }
   __syncthreads();
 
-  // Candidate k of list (w, c): its value and inverted flat index; a value of 0
-  // (below every number): none.
-  const int lists = a.W * a.chunks;
-  auto candidate = [&](int w, int c, int k, uint64_t& v, uint32_t& f) {
+  // Candidate k of list l = w * chunks + c, whose key is e: its value and inverted
+  // flat index; a value of 0 (below every number): none.
+  auto candidate_of = [&](int l, int k, uint64_t e, uint64_t& v, uint32_t& f) {
+    const int w = static_cast<int>(static_cast<uint32_t>(l) / static_cast<uint32_t>(a.chunks));
     v = 0;
     f = 0;
     const int kd = kind[w];
     uint32_t token = static_cast<uint32_t>(k);
     if (kd == kBeamOrdinary) {
-      const uint64_t e = a.keys[((n * a.W + w) * a.chunks + c) * K + k];
       token = ~static_cast<uint32_t>(e);
       if (token >= static_cast<uint32_t>(a.V)) return;
       const float x = from_ordered(static_cast<uint32_t>(e >> 32));
       v = ordered64(base[w] + (static_cast<double>(x) - peak[w]));
     } else {
-      if (c != 0) return;
+      if (l != w * a.chunks) return;
       if (kd == kBeamFinished) {
         // eos first, then the lowest tokens
         if (k == 0)
@@ -317,34 +449,68 @@ __global__ __launch_bounds__(kBeamThreads) void beam_merge_kernel(SelectArgs a) 
     f = ~(static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V) + token);
   };
 
+  auto candidate = [&](int l, int k, uint64_t& v, uint32_t& f) {
+    candidate_of(l, k, a.keys[(n * lists + l) * K + k], v, f);
+  };
+
   // A lower bound of the K-th largest value (its upper 32 bits) from the lists'
-  // first candidates, as in the chunks.
-  uint64_t head = 0;
-  for (int l = tid; l < lists; l += kBeamThreads) {
-    uint64_t v;
-    uint32_t f;
-    candidate(l / a.chunks, l % a.chunks, 0, v, f);
-    head = max(head, v);
+  // first candidates, as in the chunks; then the lists that reach it, and their
+  // candidates that do.
+  uint64_t head = 0, held_v[kHeld];
+  uint32_t held_f[kHeld];
+  if (few) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+      held_v[r] = 0;
+      if (held_k[r] < K) candidate_of(held_l[r], held_k[r], held[r], held_v[r], held_f[r]);
+      if (held_k[r] == 0) head = max(head, held_v[r]);
+    }
+  } else {
+    for (int l = tid; l < lists; l += kMergeThreads) {
+      uint64_t v;
+      uint32_t f;
+      candidate(l, 0, v, f);
+      head = max(head, v);
+    }
   }
-  const uint32_t t = wave_kth_largest(static_cast<uint32_t>(head >> 32), K, 31);
+  const uint32_t t = wave_kth_largest<31, 0>(static_cast<uint32_t>(head >> 32), K);
   if (lane == 0) bound[wave] = t;
   __syncthreads();
   uint32_t limit = bound[0];
 #pragma unroll
-  for (int w = 1; w < kBeamWaves; ++w) limit = max(limit, bound[w]);
-
-  const int total = lists * K;
-  for (int i = tid; i < total; i += kBeamThreads) {
-    uint64_t v;
-    uint32_t f;
-    const int l = i / K;
-    candidate(l / a.chunks, l % a.chunks, i - l * K, v, f);
-    if (v != 0 && static_cast<uint32_t>(v >> 32) >= limit) {
-      const int pos = atomicAdd(&count, 1);
-      if (pos < kMergeCap) {
-        value[pos] = v;
-        flat[pos] = f;
+  for (int w = 1; w < kMergeWaves; ++w) limit = max(limit, bound[w]);
+  auto take_if = [&](uint64_t v, uint32_t f) {  // (whole waves)
+    const bool hit = v != 0 && static_cast<uint32_t>(v >> 32) >= limit;
+    const unsigned long long hits = __ballot(hit);
+    if (hits == 0) return;
+    int first = 0;
+    if (lane == 0) first = atomicAdd(&count, __popcll(hits));
+    const int pos = __builtin_amdgcn_readfirstlane(first) + __popcll(hits & ((1ull << lane) - 1));
+    if (hit && pos < kMergeCap) {
+      value[pos] = v;
+      flat[pos] = f;
+    }
+  };
+  if (few) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) take_if(held_v[r], held_f[r]);
+  } else {
+    for (int l = tid; l < lists; l += kMergeThreads) {
+      uint64_t v = head;
+      uint32_t f;
+      if (lists > kMergeThreads) candidate(l, 0, v, f);
+      if (v != 0 && static_cast<uint32_t>(v >> 32) >= limit) {
+        const int pos = atomicAdd(&reached, 1);
+        if (pos < kMergeCap) reach[pos] = l;
       }
+    }
+    __syncthreads();
+    const int nr = min(reached, kMergeCap);
+    for (int i = wave; i < nr; i += kMergeWaves) {
+      uint64_t v = 0;
+      uint32_t f = 0;
+      if (lane < K) candidate(reach[i], lane, v, f);
+      take_if(v, f);
     }
   }
   __syncthreads();
@@ -360,13 +526,19 @@ __global__ __launch_bounds__(kBeamThreads) void beam_merge_kernel(SelectArgs a) 
     if (a.out_finished != nullptr)
       a.out_finished[o] = token == a.eos || (a.finished != nullptr && a.finished[n * a.W + w]);
   };
-  if (m <= kMergeCap) {
-    for (int i = tid; i < m; i += kBeamThreads) {
-      const uint64_t v = value[i];
-      const uint32_t f = flat[i];
+  if (m <= kMergeCap && reached <= kMergeCap) {
+    // Eight threads count the candidates above each one.
+    const int part = tid & 7;
+    for (int i = tid >> 3; i < (m + 7) / 8 * 8; i += kMergeThreads / 8) {
+      const uint64_t v = i < m ? value[i] : 0;
+      const uint32_t f = i < m ? flat[i] : 0;
       int rank = 0;
-      for (int j = 0; j < m; ++j) rank += value[j] > v || (value[j] == v && flat[j] > f);
-      if (rank < K) store(rank, v, f);
+#pragma unroll 4
+      for (int j = part; j < m; j += 8) rank += value[j] > v || (value[j] == v && flat[j] > f);
+      rank += __shfl_xor(rank, 1, 64);
+      rank += __shfl_xor(rank, 2, 64);
+      rank += __shfl_xor(rank, 4, 64);
+      if (part == 0 && i < m && rank < K) store(rank, v, f);
     }
   } else {
     uint64_t last_v = ~0ull;
@@ -380,11 +552,11 @@ __global__ __launch_bounds__(kBeamThreads) void beam_merge_kernel(SelectArgs a) 
           bf = f;
         }
       };
-      for (int i = tid; i < total; i += kBeamThreads) {
+      for (int i = tid; i < lists * K; i += kMergeThreads) {
         uint64_t v;
         uint32_t f;
         const int l = i / K;
-        candidate(l / a.chunks, l % a.chunks, i - l * K, v, f);
+        candidate(l, i - l * K, v, f);
         if (r == 0 || v < last_v || (v == last_v && f < last_f)) take(v, f);
       }
 #pragma unroll
@@ -400,7 +572,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_merge_kernel(SelectArgs a) 
       }
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kBeamWaves; ++w) take(best_v[w], best_f[w]);
+      for (int w = 0; w < kMergeWaves; ++w) take(best_v[w], best_f[w]);
       if (tid == 0) store(r, bv, bf);
       last_v = bv;
       last_f = bf;
@@ -408,20 +580,26 @@ __global__ __launch_bounds__(kBeamThreads) void beam_merge_kernel(SelectArgs a) 
   }
 }
 
-// Elements of a row per chunk (workgroup).
-int64_t beam_chunk(int64_t rows, int64_t V) {
-  (void)rows;
-  (void)V;
-  return kBeamThreads * 32;
+// Logits of a row per workgroup: 8192 where that gives a round of workgroups (two
+// to a CU), else 2048, so that a few rows' latency is short.
+int beam_items(int64_t rows, int64_t V) {
+  return rows * lc_cdiv(V, kBeamThreads * 32) >= 2 * lc_cu_count() ? 32 : 8;
+}
+int64_t beam_chunks(int64_t rows, int64_t V) {
+  return lc_cdiv(V, kBeamThreads * beam_items(rows, V));
 }
 
 template <typename T>
 int launch_select(SelectArgs a, int64_t groups, hipStream_t st) {
   const int64_t rows = groups * a.W;
-  beam_chunk_kernel<T, 32><<<static_cast<unsigned>(rows * a.chunks), kBeamThreads, 0, st>>>(a);
+  const unsigned blocks = static_cast<unsigned>(rows * a.chunks);
+  if (beam_items(rows, a.V) == 32)
+    beam_chunk_kernel<T, 32><<<blocks, kBeamThreads, 0, st>>>(a);
+  else
+    beam_chunk_kernel<T, 8><<<blocks, kBeamThreads, 0, st>>>(a);
   const int rc = lc_check_launch("lc_beam_select (chunks)");
   if (rc != LC_OK) return rc;
-  beam_merge_kernel<<<static_cast<unsigned>(groups), kBeamThreads, 0, st>>>(a);
+  beam_merge_kernel<<<static_cast<unsigned>(groups), kMergeThreads, 0, st>>>(a);
   return lc_check_launch("lc_beam_select (merge)");
 }
 
@@ -551,7 +729,7 @@ extern "C" {
 int64_t lc_beam_select_workspace_bytes(int64_t groups, int64_t width, int64_t vocab,
                                        int64_t count) {
   if (groups < 0 || width <= 0 || vocab <= 0 || count <= 0) return -1;
-  const int64_t rows = groups * width, lists = rows * lc_cdiv(vocab, beam_chunk(rows, vocab));
+  const int64_t rows = groups * width, lists = rows * beam_chunks(rows, vocab);
   return align256(lists * count * 8) + align256(lists * 8) + lists * 4;
 }
 
@@ -577,7 +755,7 @@ int lc_beam_select(const void* logits, int64_t group_stride, int64_t beam_stride
   LC_REQUIRE(logits && scores && out_scores && out_tokens && out_parents && workspace,
              "%s: null pointer", who);
   LC_REQUIRE(group_stride >= 0 && beam_stride >= 0, "%s: negative stride", who);
-  const int64_t rows = groups * width, chunks = lc_cdiv(vocab, beam_chunk(rows, vocab));
+  const int64_t rows = groups * width, chunks = beam_chunks(rows, vocab);
   LC_REQUIRE(rows * chunks < (1LL << 24), "%s: too many rows (%lld)", who, (long long)rows);
   const int64_t need = lc_beam_select_workspace_bytes(groups, width, vocab, count);
   if (workspace_bytes < need)
