@@ -132,15 +132,16 @@ __global__ __launch_bounds__(64) void shared_generic_kernel(SharedArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// MFMA kernel (bf16/f16, head_dim a multiple of 8 up to 128, pages of a power of two): one workgroup of 4
-// waves per (token range, 32 WR rows). A prefix's rows are the W G query heads of
-// its sequences that share a kv head, row r = w G + g; a sequence's own rows are
-// its G heads. Tiles of 64 tokens go through LDS (double-buffered, by DMA), so a
-// byte of K and V is read once for all rows of the workgroup:
-//   S^T[64 tok x 32 rows] = K Q^T, O^T[d x 32 rows] += V^T P^T   (32x32x16 MFMA)
-// The waves share the tile as WR row tiles x WK token halves: with 128 rows each
-// wave has 32 rows and all 64 tokens, with fewer rows the tokens are halved and
-// the halves' softmax states joined through LDS at the end.
+// MFMA kernel (bf16/f16, head_dim a multiple of 8 up to 128, pages of a power of
+// two from 8 up): one workgroup of 4 waves per (token range, 32 WR rows). A prefix's
+// rows are the W G query heads of its sequences that share a kv head, row r = w G +
+// g; a sequence's own rows are its G heads.
+//   S^T[tok x 32 rows] = K Q^T, O^T[d x 32 rows] += V^T P^T   (32x32x16 MFMA)
+// so a byte of K and V is read once for all rows of the workgroup. Up to 32 rows
+// the waves take token steps of their own (shared_stream below). With more, tiles
+// of 64 tokens go through LDS (double-buffered, by DMA), which the waves share: with
+// 128 rows each has 32 rows and all tokens, with 64 rows 32 tokens, and the token
+// halves' softmax states are joined through LDS at the end.
 // Tokens are named by a table, so every lane finds the address of its own 16-byte
 // chunk of a DMA; lanes whose token is past the range, whose page entry is invalid
 // or whose chunk is past head_dim read zeros instead, and their scores are masked.
@@ -173,9 +174,9 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wave_s = __builtin_amdgcn_readfirstlane(wave);
   const int l32 = lane & 31, hh = lane >> 5;
-  const int wr = WR == 4 ? wave : WR == 2 ? (wave & 1) : 0;
-  const int wk = WR == 4 ? 0 : WR == 2 ? (wave >> 1) : wave;
-  const bool active = wk < 2 && it.row0 + wr * 32 < it.rows;  // (wave-uniform)
+  const int wr = WR == 4 ? wave : (wave & 1);
+  const int wk = WR == 4 ? 0 : (wave >> 1);
+  const bool active = it.row0 + wr * 32 < it.rows;  // (wave-uniform)
 
   // This lane's query row.
   const int r_abs = it.row0 + wr * 32 + l32;
@@ -234,7 +235,7 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
   int kaddr[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
-    kaddr[s] = (wk < 2 ? wk * 32 : 0) * ROW_B + l32 * ROW_B +
+    kaddr[s] = wk * 32 * ROW_B + l32 * ROW_B +
                (((hh * (CPR / 2) + s) ^ pf_swz<CPR>(l32)) << 4);
   int vaddr[2][DTL];
   {
@@ -245,7 +246,7 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
       for (int dt = 0; dt < DTL; ++dt) {
         const int kr = jj * 8 + hh * 4 + te;
         const int d = dt * 32 + (gq & 1) * 16 + 4 * tc;
-        vaddr[jj][dt] = ((wk < 2 ? wk * 32 : 0) + kr) * ROW_B +
+        vaddr[jj][dt] = (wk * 32 + kr) * ROW_B +
                         ((((d >> 3) ^ pf_swz<CPR>(kr)) << 4) | ((d & 7) * (int)sizeof(T)));
       }
   }
@@ -399,6 +400,238 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
   if (hh == 0) a.part_lse[pidx] = l_tot == 0.f ? -INFINITY : m_ref + lc_log2(l_tot);
 }
 
+// Up to 32 rows: bound by reading K and V, so the waves stream on their own, each
+// every fourth 32-token step of the range, without barriers. A step's K and V rows
+// are loaded into registers (16 KB in flight per wave, 8 waves on a CU) while the
+// previous step computes from the wave's LDS. An instruction loads RPI token rows,
+// which share a page (pages of a power of two from RPI up): a scalar base and one
+// lane offset address it.
+template <typename T, int DPAD>
+__device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeItem& it,
+                                              LC_LDS char* b0, LC_LDS char* b1, LC_LDS char* b2,
+                                              LC_LDS char* b3, LC_LDS float* ml) {
+  typedef Mfma32<T> Ops;
+  typedef typename Ops::v8 v8;
+  constexpr int KS = DPAD / 16, DTL = DPAD / 32, CPR = DPAD / 8;
+  constexpr int RPI = 64 / CPR, NI = 32 / RPI;
+  constexpr int ROW_B = DPAD * (int)sizeof(T);
+  constexpr int kStep = 32;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  auto buffer = [&](int w) { return w == 0 ? b0 : w == 1 ? b1 : w == 2 ? b2 : b3; };
+  LC_LDS char* lds_k = buffer(wave);
+  LC_LDS char* lds_v = lds_k + kStep * ROW_B;
+
+  const int r_abs = it.row0 + l32;
+  const bool row_ok = r_abs < it.rows;
+  const int r_safe = row_ok ? r_abs : it.row0;
+  const int b = it.b0 + r_safe / a.G;
+  const int h = it.kvh * a.G + r_safe % a.G;
+  v8 qop[KS];
+  {
+    const T* qh = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int d0 = (hh * (CPR / 2) + s) * 8;
+      const bool ok = row_ok && d0 < a.D;
+      const v8 x = *reinterpret_cast<const v8*>(qh + (ok ? d0 : 0));
+      qop[s] = ok ? x : v8{};
+    }
+  }
+
+  const T* kp = static_cast<const T*>(a.kp) + (int64_t)it.kvh * a.s_head;
+  const T* vp = static_cast<const T*>(a.vp) + (int64_t)it.kvh * a.s_head;
+  const int last_page = (it.t_end - 1) >> a.p_shift;
+  const int srow = lane / CPR, chunk = lane % CPR;
+  const int lane_off =
+      chunk * 8 < a.D ? static_cast<int>((srow * a.s_tok + chunk * 8) * sizeof(T)) : -16;
+  // Page entry of token t + l32 (past the range: an entry that is not used).
+  auto fetch = [&](int t) { return it.table[min((t + l32) >> a.p_shift, last_page)]; };
+  auto live_of = [&](int t, int page) -> uint32_t {
+    return static_cast<uint32_t>(
+        __ballot(static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages) &&
+                 t + l32 < it.t_end));
+  };
+  // Rows past the range, of invalid pages or past head_dim lie outside the
+  // instruction's buffer and read zeros (which also keeps 0 x NaN out of the second
+  // product); no branch separates the loads.
+  const int row_b = static_cast<int>(a.s_tok * sizeof(T)), d_b = a.D * (int)sizeof(T);
+  u32x4_t sk[NI], sv[NI];
+  auto issue = [&](int t, int pages) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int pg = __builtin_amdgcn_readlane(pages, i * RPI);
+      const int tok = t + i * RPI;
+      const bool ok = static_cast<unsigned>(pg) < static_cast<unsigned>(a.num_pages);
+      const int64_t at = ok ? (int64_t)pg * a.s_page + (int64_t)(tok & (a.P - 1)) * a.s_tok : 0;
+      const int rows = min(RPI, it.t_end - tok);
+      const int nbytes = ok && rows > 0 ? (rows - 1) * row_b + d_b : 0;
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<T*>(kp + at), 0, nbytes, 0x00020000);
+      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<T*>(vp + at), 0, nbytes, 0x00020000);
+      sk[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_off, 0, 2);  // non-temporal
+      sv[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_off, 0, 2);
+    }
+  };
+
+  int kaddr[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    kaddr[s] = l32 * ROW_B + (((hh * (CPR / 2) + s) ^ pf_swz<CPR>(l32)) << 4);
+  int vaddr[2][DTL];
+  {
+    const int gq = lane >> 4, te = (lane & 15) >> 2, tc = lane & 3;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+      for (int dt = 0; dt < DTL; ++dt) {
+        const int kr = jj * 8 + hh * 4 + te;
+        const int d = dt * 32 + (gq & 1) * 16 + 4 * tc;
+        vaddr[jj][dt] =
+            kr * ROW_B + ((((d >> 3) ^ pf_swz<CPR>(kr)) << 4) | ((d & 7) * (int)sizeof(T)));
+      }
+  }
+
+  f32x16_t o[DTL];
+#pragma unroll
+  for (int i = 0; i < DTL; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+  float m_ref = -INFINITY, l_lane = 0.f;
+
+  const int t0 = it.t_begin + wave * kStep;
+  constexpr int kNext = 4 * kStep;
+  int page_next = 0;
+  uint32_t live_next = 0;
+  if (t0 < it.t_end) {
+    const int page = fetch(t0);
+    issue(t0, page);
+    live_next = live_of(t0, page);
+    page_next = fetch(t0 + kNext);
+  }
+  for (int t = t0; t < it.t_end; t += kNext) {
+    const uint32_t live = live_next;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int row = i * RPI + srow;
+      const int at = row * ROW_B + ((chunk ^ pf_swz<CPR>(row)) << 4);
+      *reinterpret_cast<LC_LDS u32x4_t*>(lds_k + at) = sk[i];
+      *reinterpret_cast<LC_LDS u32x4_t*>(lds_v + at) = sv[i];
+    }
+    if (t + kNext < it.t_end) {
+      issue(t + kNext, page_next);
+      live_next = live_of(t + kNext, page_next);
+      page_next = fetch(t + 2 * kNext);
+    }
+    lc_compiler_fence();
+    if (live == 0) continue;
+
+    f32x16_t x;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      x = Ops::mma(*reinterpret_cast<LC_LDS const v8*>(lds_k + kaddr[s]), qop[s], x);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= a.scale_log2;
+    if (live != 0xffffffffu) {
+      const uint32_t mine = live >> (hh * 4);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (!((mine >> ((r >> 2) * 8 + (r & 3))) & 1)) x[r] = -INFINITY;
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
+    mx = pf_half_max(mx);
+    if (__ballot(mx > m_ref + kSharedRescaleLog2)) {
+      const float m_new = fmaxf(m_ref, mx);
+      const float alpha = m_new == -INFINITY ? 1.f : lc_exp2(m_ref - m_new);
+      l_lane *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+      m_ref = m_new;
+    }
+    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+    v8 pop[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = lc_exp2(x[r] - m_use);
+      l_lane += p;
+      pop[r >> 3][r & 7] = static_cast<T>(p);
+    }
+#pragma unroll
+    for (int jp = 0; jp < 2; ++jp)
+#pragma unroll
+      for (int dt = 0; dt < DTL; ++dt) {
+        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (LC_LDS i16x4_t*)(lds_v + vaddr[0][dt] + jp * 16 * ROW_B));
+        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (LC_LDS i16x4_t*)(lds_v + vaddr[1][dt] + jp * 16 * ROW_B));
+        const i16x8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        o[dt] = Ops::mma(__builtin_bit_cast(v8, both), pop[jp], o[dt]);
+      }
+    lc_compiler_fence();
+  }
+
+  // Join the waves: each leaves O in its own buffer, [register][lane]; wave w then
+  // sums the 32 columns dt = w of every wave.
+  float l_tot;
+  {
+    const unsigned u = __float_as_uint(l_lane);
+    const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    l_tot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+  }
+  LC_LDS float* rec = (LC_LDS float*)lds_k;
+#pragma unroll
+  for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) rec[(dt * 16 + r) * 64 + lane] = o[dt][r];
+  ml[wave * 128 + lane] = m_ref;
+  ml[wave * 128 + 64 + lane] = l_tot;
+  __syncthreads();
+  if (wave >= DTL) return;
+  float mw[4], lw[4], m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    mw[w] = ml[w * 128 + lane];
+    lw[w] = ml[w * 128 + 64 + lane];
+    m = fmaxf(m, mw[w]);
+  }
+  float l = 0.f;
+  f32x16_t sum;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) sum[r] = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    // (a wave without tokens has m = -inf, l = 0 and O = 0; NaN passes)
+    const float f = lw[w] == 0.f ? 0.f : mw[w] == -INFINITY ? 1.f : lc_exp2(mw[w] - m);
+    l += lw[w] * f;
+    LC_LDS const float* from = (LC_LDS const float*)buffer(w) + wave * 16 * 64 + lane;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[r] += from[r * 64] * f;
+  }
+  if (!row_ok) return;
+  const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
+  const float inv_l = l == 0.f ? 0.f : 1.0f / l;
+  float* po = a.part_o + pidx * a.D;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int d0 = wave * 32 + j * 8 + hh * 4;
+    if (d0 < a.D) {
+      f32x4_t w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = sum[j * 4 + e] * inv_l;
+      *reinterpret_cast<f32x4_t*>(po + d0) = w;
+    }
+  }
+  if (wave == 0 && hh == 0) a.part_lse[pidx] = l == 0.f ? -INFINITY : m + lc_log2(l);
+}
+
 // Workgroups below p_blocks take the prefixes' ranges, the others the sequences'
 // own. A prefix range's row tiles read the same K and V: they get block ids 8
 // apart, which run on one XCD, and find it in its L2.
@@ -411,6 +644,7 @@ shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
   __shared__ __align__(16) char lds_k1[TILE_B];
   __shared__ __align__(16) char lds_v0[TILE_B];
   __shared__ __align__(16) char lds_v1[TILE_B];
+  __shared__ float lds_ml[4 * 128];
   RangeItem it;
   const int id = blockIdx.x;
   if (id < p_blocks) {
@@ -431,8 +665,12 @@ shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
     it.rows = a.W * a.G;
     it.row0 = tile * 32 * WR;
     it.slot = split;
-    shared_range<T, DPAD, WR>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
-                              (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1);
+    if constexpr (WR > 1)
+      shared_range<T, DPAD, WR>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
+                                (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1);
+    else
+      shared_stream<T, DPAD>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
+                             (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1, (LC_LDS float*)lds_ml);
   } else {
     const int units = a.B * a.Hkv * head_groups;
     const int split = (id - p_blocks) / units, u = id - p_blocks - split * units;
@@ -449,8 +687,8 @@ shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
     it.rows = a.G;
     it.row0 = hg * 32;
     it.slot = a.p_splits + split;
-    shared_range<T, DPAD, 1>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
-                              (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1);
+    shared_stream<T, DPAD>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
+                           (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1, (LC_LDS float*)lds_ml);
   }
 }
 
@@ -694,7 +932,7 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
   a.scale_log2 = scale * kLog2e;
   const bool mfma = dtype != LC_DTYPE_F32 && D % 8 == 0 && D <= 128 && q_sb % 8 == 0 &&
                     q_sh % 8 == 0 && kv_s_page % 8 == 0 && kv_s_head % 8 == 0 &&
-                    kv_s_tok % 8 == 0 && a.p_shift >= 0 && lc_aligned(q, 16) && lc_aligned(key_pages, 16) &&
+                    kv_s_tok % 8 == 0 && a.p_shift >= 3 && kv_s_tok < (1LL << 24) && lc_aligned(q, 16) && lc_aligned(key_pages, 16) &&
                     lc_aligned(value_pages, 16);
   hipStream_t st = lc_stream(stream);
   switch (dtype) {
