@@ -160,6 +160,94 @@ struct RangeItem {
   int kvh, t_begin, t_end, slot;
 };
 
+// Where the token of each lane lies: its byte offset in the pools, and the bytes of
+// the RPI rows from it on that hold tokens of the range (0: none, or an invalid
+// page). One lane's answer serves a whole DMA instruction, by v_readlane: computed
+// by all lanes at once, it costs a few instructions per tile instead of a 64-bit
+// scalar product and its branches per DMA instruction.
+struct RowPlace {
+  uint32_t lo, hi;
+  int bytes;
+};
+template <int RPI>
+__device__ __forceinline__ RowPlace row_place(const SharedArgs& a, int page, int tok, int t_end,
+                                              int esz) {
+  const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages) && tok < t_end;
+  const uint32_t slot = static_cast<uint32_t>(tok & (a.P - 1)) * static_cast<uint32_t>(a.s_tok);
+  const uint64_t at =
+      (static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(a.s_page) + slot) *
+      static_cast<uint32_t>(esz);
+  RowPlace p;
+  p.lo = ok ? static_cast<uint32_t>(at) : 0;
+  p.hi = ok ? static_cast<uint32_t>(at >> 32) : 0;
+  p.bytes = ok ? ((min(RPI, t_end - tok) - 1) * static_cast<int>(a.s_tok) + a.D) * esz : 0;
+  return p;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* base, const RowPlace& p,
+                                                             int lane) {
+  const uint64_t at =
+      (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(p.hi), lane))) << 32) |
+      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(p.lo), lane));
+  return __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(static_cast<const char*>(base) + at), 0,
+      __builtin_amdgcn_readlane(p.bytes, lane), 0x00020000);
+}
+
+// Operands of a lane's query row: step s takes the 8 elements of chunk hh CPR / 2 + s
+// (zeros for a row that is none, or past head_dim).
+template <typename T, int DPAD>
+__device__ __forceinline__ void load_rows(const SharedArgs& a, int b, int h, bool row_ok, int hh,
+                                          typename Mfma32<T>::v8 (&qop)[DPAD / 16]) {
+  typedef typename Mfma32<T>::v8 v8;
+  constexpr int CPR = DPAD / 8;
+  const T* qh = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
+#pragma unroll
+  for (int s = 0; s < DPAD / 16; ++s) {
+    const int d0 = (hh * (CPR / 2) + s) * 8;
+    const bool ok = row_ok && d0 < a.D;
+    const v8 x = *reinterpret_cast<const v8*>(qh + (ok ? d0 : 0));
+    qop[s] = ok ? x : v8{};
+  }
+}
+
+// LDS addresses of a tile's operands from token row0 on (rows of DPAD, chunks
+// swizzled by pf_swz): K rows for S^T, V columns for O^T by transposed reads.
+template <typename T, int DPAD>
+__device__ __forceinline__ void operand_addresses(int lane, int row0, int (&kaddr)[DPAD / 16],
+                                                  int (&vaddr)[2][DPAD / 32]) {
+  constexpr int CPR = DPAD / 8, ROW_B = DPAD * (int)sizeof(T);
+  const int l32 = lane & 31, hh = lane >> 5;
+#pragma unroll
+  for (int s = 0; s < DPAD / 16; ++s)
+    kaddr[s] = (row0 + l32) * ROW_B + (((hh * (CPR / 2) + s) ^ pf_swz<CPR>(l32)) << 4);
+  const int gq = lane >> 4, te = (lane & 15) >> 2, tc = lane & 3;
+#pragma unroll
+  for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+    for (int dt = 0; dt < DPAD / 32; ++dt) {
+      const int kr = jj * 8 + hh * 4 + te;
+      const int d = dt * 32 + (gq & 1) * 16 + 4 * tc;
+      vaddr[jj][dt] = (row0 + kr) * ROW_B +
+                      ((((d >> 3) ^ pf_swz<CPR>(kr)) << 4) | ((d & 7) * (int)sizeof(T)));
+    }
+}
+
+// Writes columns dt * 32 .. of a row's partial output.
+__device__ __forceinline__ void store_columns(const SharedArgs& a, int64_t pidx, int dt, int hh,
+                                              const f32x16_t& o, float inv_l) {
+  float* po = a.part_o + pidx * a.D;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int d0 = dt * 32 + j * 8 + hh * 4;
+    if (d0 < a.D) {  // (D % 8 == 0: whole groups of 4)
+      f32x4_t w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = o[j * 4 + e] * inv_l;
+      *reinterpret_cast<f32x4_t*>(po + d0) = w;
+    }
+  }
+}
+
 template <typename T, int DPAD, int WR>
 __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeItem& it,
                                              LC_LDS char* lds_k0, LC_LDS char* lds_k1,
@@ -176,90 +264,58 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
   const int l32 = lane & 31, hh = lane >> 5;
   const int wr = WR == 4 ? wave : (wave & 1);
   const int wk = WR == 4 ? 0 : (wave >> 1);
-  const bool active = it.row0 + wr * 32 < it.rows;  // (wave-uniform)
 
-  // This lane's query row.
+  // This lane's query row (a wave whose rows are none computes on zeros: it shares
+  // the others' steps anyway).
   const int r_abs = it.row0 + wr * 32 + l32;
   const bool row_ok = r_abs < it.rows;
   const int r_safe = row_ok ? r_abs : it.row0;
   const int b = it.b0 + r_safe / a.G;
   const int h = it.kvh * a.G + r_safe % a.G;
   v8 qop[KS];
-  {
-    const T* qh = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d0 = (hh * (CPR / 2) + s) * 8;
-      const bool ok = row_ok && d0 < a.D;
-      const v8 x = *reinterpret_cast<const v8*>(qh + (ok ? d0 : 0));
-      qop[s] = ok ? x : v8{};
-    }
-  }
+  load_rows<T, DPAD>(a, b, h, row_ok, hh, qop);
 
   const T* kp = static_cast<const T*>(a.kp) + (int64_t)it.kvh * a.s_head;
   const T* vp = static_cast<const T*>(a.vp) + (int64_t)it.kvh * a.s_head;
-  const T* zeros = reinterpret_cast<const T*>(shared_zeros);
-  // Pages of this lane's DMA rows of the tile at t0, and of the token it masks
-  // (past the range: an entry that is not used).
   const int last_page = (it.t_end - 1) >> a.p_shift;
-  auto fetch = [&](int t0, int (&pg)[NIW], int& own) {
+  // Page entry of the tile's token t0 + lane (past the range: one that is not used).
+  auto fetch = [&](int t0) { return it.table[min((t0 + lane) >> a.p_shift, last_page)]; };
+  // DMA of one tensor's tile: this lane's 16-byte chunk of its row.
+  PfLoadOffsets<NIW> off;
 #pragma unroll
-    for (int u = 0; u < NIW; ++u) {
-      const int tok = t0 + (wave * NIW + u) * RPI + lane / CPR;
-      pg[u] = it.table[min(tok >> a.p_shift, last_page)];
-    }
-    const int tok = t0 + (NKT == 2 ? lane : wk * 32 + l32);
-    own = it.table[min(tok >> a.p_shift, last_page)];
+  for (int u = 0; u < NIW; ++u) {
+    const int row = (wave * NIW + u) * RPI + lane / CPR;
+    const int ch = (lane % CPR) ^ pf_swz<CPR>(row);
+    off.o[u] = ch * 8 < a.D ? static_cast<int>(((lane / CPR) * a.s_tok + ch * 8) * sizeof(T)) : -16;
+  }
+  auto place = [&](int t0, int pages) {
+    return row_place<RPI>(a, pages, t0 + lane, it.t_end, sizeof(T));
   };
-  auto issue = [&](int t0, const int (&pg)[NIW], LC_LDS char* kd, LC_LDS char* vd) {
+  auto issue = [&](const T* base, const RowPlace& at, LC_LDS char* dst) {
 #pragma unroll
     for (int u = 0; u < NIW; ++u) {
-      const int row = (wave * NIW + u) * RPI + lane / CPR;
-      const int ch = (lane % CPR) ^ pf_swz<CPR>(row);
-      const int tok = t0 + row;
-      const bool ok = static_cast<unsigned>(pg[u]) < static_cast<unsigned>(a.num_pages) &&
-                      tok < it.t_end && ch * 8 < a.D;
-      const int slot = tok & (a.P - 1);
-      const int64_t off = (int64_t)pg[u] * a.s_page + (int64_t)slot * a.s_tok + ch * 8;
-      const T* ks = ok ? kp + off : zeros;
-      const T* vs = ok ? vp + off : zeros;
-      const int dst = (wave_s * NIW + u) * RPI * ROW_B;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)ks,
-                                       (LC_LDS void*)(kd + dst), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)vs,
-                                       (LC_LDS void*)(vd + dst), 16, 0, 0);
+      const int row0 = (wave_s * NIW + u) * RPI;
+      const int vo = off.o[u];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(row_buffer(base, at, row0),
+                                               (LC_LDS void*)(dst + row0 * ROW_B), 16, vo, 0, 0, 0);
     }
   };
 
   // LDS addresses of the operands (see the prefill kernel's).
-  int kaddr[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s)
-    kaddr[s] = wk * 32 * ROW_B + l32 * ROW_B +
-               (((hh * (CPR / 2) + s) ^ pf_swz<CPR>(l32)) << 4);
-  int vaddr[2][DTL];
-  {
-    const int gq = lane >> 4, te = (lane & 15) >> 2, tc = lane & 3;
-#pragma unroll
-    for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-      for (int dt = 0; dt < DTL; ++dt) {
-        const int kr = jj * 8 + hh * 4 + te;
-        const int d = dt * 32 + (gq & 1) * 16 + 4 * tc;
-        vaddr[jj][dt] = (wk * 32 + kr) * ROW_B +
-                        ((((d >> 3) ^ pf_swz<CPR>(kr)) << 4) | ((d & 7) * (int)sizeof(T)));
-      }
-  }
+  int kaddr[KS], vaddr[2][DTL];
+  operand_addresses<T, DPAD>(lane, wk * 32, kaddr, vaddr);
 
   f32x16_t o[DTL];
 #pragma unroll
   for (int i = 0; i < DTL; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-  float m_ref = -INFINITY, l_lane = 0.f;
+  float m_ref = -INFINITY, l_lane = 0.f, l_tile = 0.f;
+  f32x16_t x[NKT];  // raw scores of the next tile
+  f32x16_t y[NKT];  // exponents of the current tile, relative to m_ref
+  v8 pop[NKT][2];
 
-  auto compute = [&](LC_LDS const char* kt_lds, LC_LDS const char* vt_lds, uint64_t live) {
-    f32x16_t x[NKT];
+  auto qk = [&](LC_LDS const char* kt_lds) __attribute__((always_inline)) {
 #pragma unroll
     for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
@@ -270,47 +326,8 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
       for (int kt = 0; kt < NKT; ++kt)
         x[kt] = Ops::mma(*reinterpret_cast<LC_LDS const v8*>(kt_lds + kaddr[s] + kt * 32 * ROW_B),
                          qop[s], x[kt]);
-#pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[kt][r] *= a.scale_log2;
-    constexpr uint64_t kAll = NKT == 2 ? ~0ull : 0xffffffffull;
-    if ((live & kAll) != kAll) {
-      const uint64_t mine = live >> (hh * 4);
-#pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((mine >> (kt * 32 + (r >> 2) * 8 + (r & 3))) & 1)) x[kt][r] = -INFINITY;
-    }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[kt][r]);
-    mx = pf_half_max(mx);
-    // The reference max only moves when some row's max grew by more than 2^8
-    // (exact: O and l share it).
-    if (__ballot(mx > m_ref + kSharedRescaleLog2)) {
-      const float m_new = fmaxf(m_ref, mx);
-      const float alpha = m_new == -INFINITY ? 1.f : lc_exp2(m_ref - m_new);
-      l_lane *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DTL; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-      m_ref = m_new;
-    }
-    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-    v8 pop[NKT][2];
-#pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = lc_exp2(x[kt][r] - m_use);
-        l_lane += p;
-        pop[kt][r >> 3][r & 7] = static_cast<T>(p);
-      }
+  };
+  auto pv = [&](LC_LDS const char* vt_lds) __attribute__((always_inline)) {
 #pragma unroll
     for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
@@ -326,27 +343,144 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
           o[dt] = Ops::mma(__builtin_bit_cast(v8, both), pop[kt][jp], o[dt]);
         }
   };
-
-  // Tile t computes from one buffer while tile t + 1 arrives in the other and the
-  // page entries of tile t + 2 are on their way.
-  int pg[NIW], own, own_next;
-  fetch(it.t_begin, pg, own);
-  issue(it.t_begin, pg, lds_k0, lds_v0);
-  fetch(it.t_begin + kTile, pg, own_next);
-  auto step = [&](int t, LC_LDS char* kc, LC_LDS char* vc, LC_LDS char* kn, LC_LDS char* vn) {
-    pf_barrier<true>();  // tile t is in LDS; the other buffer's reads are done
-    if (t + kTile < it.t_end) issue(t + kTile, pg, kn, vn);
-    const uint64_t live =
-        __ballot(static_cast<unsigned>(own) < static_cast<unsigned>(a.num_pages) &&
-                 t + (NKT == 2 ? lane : wk * 32 + l32) < it.t_end);
-    own = own_next;
-    fetch(t + 2 * kTile, pg, own_next);
-    if (active && live != 0) compute(kc, vc, live);
+  // Scores of tokens that are none are masked; rows without a reference max (only
+  // before the first live tile) take the tile's.
+  constexpr uint64_t kAll = NKT == 2 ? ~0ull : 0xffffffffull;
+  auto prepare = [&](uint64_t live) __attribute__((always_inline)) {
+    const uint64_t mine = (live >> (wk * 32)) & kAll;
+    if (mine != kAll) {
+      const uint64_t bits = mine >> (hh * 4);
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((bits >> (kt * 32 + (r >> 2) * 8 + (r & 3))) & 1)) x[kt][r] = -INFINITY;
+    }
+    if (__ballot(m_ref == -INFINITY)) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[kt][r]);
+      mx = pf_half_max(mx) * a.scale_log2;
+      if (m_ref == -INFINITY) m_ref = mx;
+    }
   };
-  for (int t = it.t_begin; t < it.t_end; t += 2 * kTile) {
-    step(t, lds_k0, lds_v0, lds_k1, lds_v1);
-    if (t + kTile < it.t_end) step(t + kTile, lds_k1, lds_v1, lds_k0, lds_v0);
+  auto shift = [&]() __attribute__((always_inline)) {
+    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) y[kt][r] = fmaf(x[kt][r], a.scale_log2, -m_use);
+  };
+  auto weigh = [&]() __attribute__((always_inline)) {
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = lc_exp2(y[kt][r]);
+        if (r & 1) s1 += p; else s0 += p;
+        pop[kt][r >> 3][r & 7] = static_cast<T>(p);
+      }
+    l_tile = s0 + s1;
+  };
+  // A weight past 2^8 (then its lane's sum is too): the rows whose max grew move
+  // their reference there, with O and l, and the tile is weighed again.
+  auto settle = [&]() __attribute__((always_inline)) {
+    if (__builtin_expect(__ballot(l_tile > 256.f) != 0, 0)) {
+      float up = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) up = fmaxf(up, y[kt][r]);
+      up = pf_half_max(up);
+      const float alpha = lc_exp2(-up);
+      l_lane *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+      m_ref = m_ref == -INFINITY ? up : m_ref + up;
+#pragma unroll
+      for (int kt = 0; kt < NKT; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[kt][r] -= up;
+      weigh();
+    }
+    l_lane += l_tile;
+  };
+
+  // Step t computes S of tile t + 1 beside the softmax and PV of tile t: K runs a
+  // tile ahead of V. Its DMA (K of tile t + 2, V of t + 1) goes into the buffers that
+  // step t - 1 read; the page entries of tile t + 3 are on their way.
+  const int tb = it.t_begin;
+  const int n_tiles = (it.t_end - tb + kTile - 1) / kTile;
+  int pg3;             // page entries
+  RowPlace at1, at2;   // of tiles t + 1 and t + 2
+  uint64_t live1;
+  {
+    const int pg0 = fetch(tb), pg1 = fetch(tb + kTile), pg2 = fetch(tb + 2 * kTile);
+    pg3 = fetch(tb + 3 * kTile);
+    const RowPlace at0 = place(tb, pg0);
+    at1 = place(tb + kTile, pg1);
+    at2 = place(tb + 2 * kTile, pg2);
+    issue(kp, at0, lds_k0);
+    issue(vp, at0, lds_v0);
+    if (n_tiles > 1) issue(kp, at1, lds_k1);
+    const uint64_t live0 = __ballot(at0.bytes != 0);
+    live1 = __ballot(at1.bytes != 0);
+    pf_barrier<true>();
+    qk(lds_k0);
+    prepare(live0);
+    shift();
   }
+  auto step = [&](int t, LC_LDS char* kc, LC_LDS char* vc, LC_LDS char* kn, LC_LDS char* vn)
+      __attribute__((always_inline)) {
+    // Tiles K t + 1 and V t are in LDS; the other buffers' reads are done.
+    pf_barrier<true>();
+    const int t0 = tb + t * kTile;
+    if (t + 2 < n_tiles) issue(kp, at2, kc);
+    issue(vp, at1, vn);
+    const uint64_t live = live1;
+    at1 = at2;
+    live1 = __ballot(at1.bytes != 0);
+    at2 = place(t0 + 3 * kTile, pg3);
+    pg3 = fetch(t0 + 4 * kTile);
+    // One matrix instruction, its operands' reads LA ahead, and vector work.
+    constexpr int NQ = NKT * KS, NP = NKT * 2 * DTL, LA = 4;
+    qk(kn);
+    weigh();
+    __builtin_amdgcn_sched_group_barrier(0x100, LA, 0);
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (j + LA < NQ) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+    }
+    settle();
+    prepare(live);
+    pv(vc);
+    shift();
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * LA, 0);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (j + LA < NP) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+    }
+  };
+  int t = 0;
+  for (; t + 2 < n_tiles; t += 2) {
+    step(t, lds_k0, lds_v0, lds_k1, lds_v1);
+    step(t + 1, lds_k1, lds_v1, lds_k0, lds_v0);
+  }
+  if (t + 1 < n_tiles) step(t, lds_k0, lds_v0, lds_k1, lds_v1);
+  // The last tile.
+  weigh();
+  settle();
+  pf_barrier<true>();
+  pv(n_tiles & 1 ? lds_v0 : lds_v1);
 
   float l_tot = l_lane;
   {
@@ -384,30 +518,20 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
   if (!row_ok) return;
   const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
   const float inv_l = l_tot == 0.f ? 0.f : 1.0f / l_tot;
-  float* po = a.part_o + pidx * a.D;
 #pragma unroll
-  for (int dt = 0; dt < DTL; ++dt)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d0 = dt * 32 + j * 8 + hh * 4;
-      if (d0 < a.D) {
-        f32x4_t w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = o[dt][j * 4 + e] * inv_l;
-        *reinterpret_cast<f32x4_t*>(po + d0) = w;
-      }
-    }
+  for (int dt = 0; dt < DTL; ++dt) store_columns(a, pidx, dt, hh, o[dt], inv_l);
   if (hh == 0) a.part_lse[pidx] = l_tot == 0.f ? -INFINITY : m_ref + lc_log2(l_tot);
 }
 
-// Up to 32 rows: bound by reading K and V, so the waves stream on their own, each
-// every fourth 32-token step of the range, without barriers. A step's K and V rows
+// Up to 32 rows: bound by reading K and V, so the waves stream on their own, without
+// barriers: groups of gw waves (1, 2 or 4) share a range, wave i of a group taking
+// every gw-th 32-token step. `it` may be empty. A step's K and V rows
 // are loaded into registers (16 KB in flight per wave, 8 waves on a CU) while the
 // previous step computes from the wave's LDS. An instruction loads RPI token rows,
 // which share a page (pages of a power of two from RPI up): a scalar base and one
 // lane offset address it.
 template <typename T, int DPAD>
-__device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeItem& it,
+__device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeItem& it, int gw,
                                               LC_LDS char* b0, LC_LDS char* b1, LC_LDS char* b2,
                                               LC_LDS char* b3, LC_LDS float* ml) {
   typedef Mfma32<T> Ops;
@@ -418,6 +542,7 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
   constexpr int kStep = 32;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wg = wave & (gw - 1);  // this wave in its group
   const int l32 = lane & 31, hh = lane >> 5;
   auto buffer = [&](int w) { return w == 0 ? b0 : w == 1 ? b1 : w == 2 ? b2 : b3; };
   LC_LDS char* lds_k = buffer(wave);
@@ -429,16 +554,7 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
   const int b = it.b0 + r_safe / a.G;
   const int h = it.kvh * a.G + r_safe % a.G;
   v8 qop[KS];
-  {
-    const T* qh = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int d0 = (hh * (CPR / 2) + s) * 8;
-      const bool ok = row_ok && d0 < a.D;
-      const v8 x = *reinterpret_cast<const v8*>(qh + (ok ? d0 : 0));
-      qop[s] = ok ? x : v8{};
-    }
-  }
+  load_rows<T, DPAD>(a, b, h, row_ok, hh, qop);
 
   const T* kp = static_cast<const T*>(a.kp) + (int64_t)it.kvh * a.s_head;
   const T* vp = static_cast<const T*>(a.vp) + (int64_t)it.kvh * a.s_head;
@@ -448,51 +564,23 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
       chunk * 8 < a.D ? static_cast<int>((srow * a.s_tok + chunk * 8) * sizeof(T)) : -16;
   // Page entry of token t + l32 (past the range: an entry that is not used).
   auto fetch = [&](int t) { return it.table[min((t + l32) >> a.p_shift, last_page)]; };
-  auto live_of = [&](int t, int page) -> uint32_t {
-    return static_cast<uint32_t>(
-        __ballot(static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages) &&
-                 t + l32 < it.t_end));
+  auto place = [&](int t, int page) {
+    return row_place<RPI>(a, page, t + l32, it.t_end, sizeof(T));
   };
   // Rows past the range, of invalid pages or past head_dim lie outside the
   // instruction's buffer and read zeros (which also keeps 0 x NaN out of the second
   // product); no branch separates the loads.
-  const int row_b = static_cast<int>(a.s_tok * sizeof(T)), d_b = a.D * (int)sizeof(T);
   u32x4_t sk[NI], sv[NI];
-  auto issue = [&](int t, int pages) {
+  auto issue = [&](const RowPlace& at) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int pg = __builtin_amdgcn_readlane(pages, i * RPI);
-      const int tok = t + i * RPI;
-      const bool ok = static_cast<unsigned>(pg) < static_cast<unsigned>(a.num_pages);
-      const int64_t at = ok ? (int64_t)pg * a.s_page + (int64_t)(tok & (a.P - 1)) * a.s_tok : 0;
-      const int rows = min(RPI, it.t_end - tok);
-      const int nbytes = ok && rows > 0 ? (rows - 1) * row_b + d_b : 0;
-      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<T*>(kp + at), 0, nbytes, 0x00020000);
-      const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<T*>(vp + at), 0, nbytes, 0x00020000);
-      sk[i] = __builtin_amdgcn_raw_buffer_load_b128(rk, lane_off, 0, 2);  // non-temporal
-      sv[i] = __builtin_amdgcn_raw_buffer_load_b128(rv, lane_off, 0, 2);
+      sk[i] = __builtin_amdgcn_raw_buffer_load_b128(row_buffer(kp, at, i * RPI), lane_off, 0, 2);
+      sv[i] = __builtin_amdgcn_raw_buffer_load_b128(row_buffer(vp, at, i * RPI), lane_off, 0, 2);
     }
-  };
+  };  // (2: non-temporal)
 
-  int kaddr[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s)
-    kaddr[s] = l32 * ROW_B + (((hh * (CPR / 2) + s) ^ pf_swz<CPR>(l32)) << 4);
-  int vaddr[2][DTL];
-  {
-    const int gq = lane >> 4, te = (lane & 15) >> 2, tc = lane & 3;
-#pragma unroll
-    for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-      for (int dt = 0; dt < DTL; ++dt) {
-        const int kr = jj * 8 + hh * 4 + te;
-        const int d = dt * 32 + (gq & 1) * 16 + 4 * tc;
-        vaddr[jj][dt] =
-            kr * ROW_B + ((((d >> 3) ^ pf_swz<CPR>(kr)) << 4) | ((d & 7) * (int)sizeof(T)));
-      }
-  }
+  int kaddr[KS], vaddr[2][DTL];
+  operand_addresses<T, DPAD>(lane, 0, kaddr, vaddr);
 
   f32x16_t o[DTL];
 #pragma unroll
@@ -501,17 +589,22 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
   float m_ref = -INFINITY, l_lane = 0.f;
 
-  const int t0 = it.t_begin + wave * kStep;
-  constexpr int kNext = 4 * kStep;
+  const int t0 = it.t_begin + wg * kStep;
+  const int next = gw * kStep;
+  // (the places of a step's rows are found a step ahead of its loads, and its page
+  // entries a step before that)
+  RowPlace at_next{};
   int page_next = 0;
   uint32_t live_next = 0;
   if (t0 < it.t_end) {
-    const int page = fetch(t0);
-    issue(t0, page);
-    live_next = live_of(t0, page);
-    page_next = fetch(t0 + kNext);
+    const int page = fetch(t0), page1 = fetch(t0 + next);
+    page_next = fetch(t0 + 2 * next);
+    const RowPlace at = place(t0, page);
+    issue(at);
+    live_next = static_cast<uint32_t>(__ballot(at.bytes != 0));
+    at_next = place(t0 + next, page1);
   }
-  for (int t = t0; t < it.t_end; t += kNext) {
+  for (int t = t0; t < it.t_end; t += next) {
     const uint32_t live = live_next;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -520,10 +613,11 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
       *reinterpret_cast<LC_LDS u32x4_t*>(lds_k + at) = sk[i];
       *reinterpret_cast<LC_LDS u32x4_t*>(lds_v + at) = sv[i];
     }
-    if (t + kNext < it.t_end) {
-      issue(t + kNext, page_next);
-      live_next = live_of(t + kNext, page_next);
-      page_next = fetch(t + 2 * kNext);
+    if (t + next < it.t_end) {
+      issue(at_next);
+      live_next = static_cast<uint32_t>(__ballot(at_next.bytes != 0));
+      at_next = place(t + 2 * next, page_next);
+      page_next = fetch(t + 3 * next);
     }
     lc_compiler_fence();
     if (live == 0) continue;
@@ -578,58 +672,56 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
     lc_compiler_fence();
   }
 
-  // Join the waves: each leaves O in its own buffer, [register][lane]; wave w then
-  // sums the 32 columns dt = w of every wave.
-  float l_tot;
+  float l;
   {
     const unsigned u = __float_as_uint(l_lane);
     const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    l_tot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
   }
+  const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
+  if (gw == 1) {
+    if (!row_ok || it.t_begin >= it.t_end) return;
+    const float inv_l = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int dt = 0; dt < DTL; ++dt) store_columns(a, pidx, dt, hh, o[dt], inv_l);
+    if (hh == 0) a.part_lse[pidx] = l == 0.f ? -INFINITY : m_ref + lc_log2(l);
+    return;
+  }
+  // Join the group's waves: each leaves O in its own buffer, [register][lane], and
+  // takes every gw-th block of 32 columns of all of them.
   LC_LDS float* rec = (LC_LDS float*)lds_k;
 #pragma unroll
   for (int dt = 0; dt < DTL; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) rec[(dt * 16 + r) * 64 + lane] = o[dt][r];
   ml[wave * 128 + lane] = m_ref;
-  ml[wave * 128 + 64 + lane] = l_tot;
+  ml[wave * 128 + 64 + lane] = l;
   __syncthreads();
-  if (wave >= DTL) return;
-  float mw[4], lw[4], m = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    mw[w] = ml[w * 128 + lane];
-    lw[w] = ml[w * 128 + 64 + lane];
-    m = fmaxf(m, mw[w]);
-  }
-  float l = 0.f;
-  f32x16_t sum;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) sum[r] = 0.f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    // (a wave without tokens has m = -inf, l = 0 and O = 0; NaN passes)
-    const float f = lw[w] == 0.f ? 0.f : mw[w] == -INFINITY ? 1.f : lc_exp2(mw[w] - m);
-    l += lw[w] * f;
-    LC_LDS const float* from = (LC_LDS const float*)buffer(w) + wave * 16 * 64 + lane;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sum[r] += from[r * 64] * f;
-  }
-  if (!row_ok) return;
-  const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
+  if (it.t_begin >= it.t_end) return;
+  const int w0 = wave - wg;
+  float m = -INFINITY;
+  for (int w = w0; w < w0 + gw; ++w) m = fmaxf(m, ml[w * 128 + lane]);
+  // (a wave without tokens has m = -inf, l = 0 and O = 0; NaN passes)
+  auto weight = [&](int w) {
+    const float mw = ml[w * 128 + lane], lw = ml[w * 128 + 64 + lane];
+    return lw == 0.f ? 0.f : mw == -INFINITY ? 1.f : lc_exp2(mw - m);
+  };
+  l = 0.f;
+  for (int w = w0; w < w0 + gw; ++w) l += ml[w * 128 + 64 + lane] * weight(w);
   const float inv_l = l == 0.f ? 0.f : 1.0f / l;
-  float* po = a.part_o + pidx * a.D;
+  for (int dt = wg; dt < DTL; dt += gw) {
+    f32x16_t sum;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d0 = wave * 32 + j * 8 + hh * 4;
-    if (d0 < a.D) {
-      f32x4_t w;
+    for (int r = 0; r < 16; ++r) sum[r] = 0.f;
+    for (int w = w0; w < w0 + gw; ++w) {
+      const float f = weight(w);
+      LC_LDS const float* from = (LC_LDS const float*)buffer(w) + dt * 16 * 64 + lane;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = sum[j * 4 + e] * inv_l;
-      *reinterpret_cast<f32x4_t*>(po + d0) = w;
+      for (int r = 0; r < 16; ++r) sum[r] += from[r * 64] * f;
     }
+    if (row_ok) store_columns(a, pidx, dt, hh, sum, inv_l);
   }
-  if (wave == 0 && hh == 0) a.part_lse[pidx] = l == 0.f ? -INFINITY : m + lc_log2(l);
+  if (row_ok && wg == 0 && hh == 0) a.part_lse[pidx] = l == 0.f ? -INFINITY : m + lc_log2(l);
 }
 
 // Workgroups below p_blocks take the prefixes' ranges, the others the sequences'
@@ -637,7 +729,7 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
 // apart, which run on one XCD, and find it in its L2.
 template <typename T, int DPAD, int WR>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
+shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups, int own_waves) {
   constexpr int TILE_B = kTile * DPAD * (int)sizeof(T);
   // (separate arrays: the compiler tracks a DMA by the array that it writes)
   __shared__ __align__(16) char lds_k0[TILE_B];
@@ -669,25 +761,30 @@ shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
       shared_range<T, DPAD, WR>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
                                 (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1);
     else
-      shared_stream<T, DPAD>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
+      shared_stream<T, DPAD>(a, it, 4, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
                              (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1, (LC_LDS float*)lds_ml);
   } else {
+    // Item i: all kv heads of a sequence follow one another (one table row, and
+    // neighbours in a page).
     const int units = a.B * a.Hkv * head_groups;
-    const int split = (id - p_blocks) / units, u = id - p_blocks - split * units;
+    const int i = (id - p_blocks) * (4 / own_waves) +
+                  __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / own_waves;
+    const int split = i / units, u = i - split * units;
     const int hg = u % head_groups, bk = u / head_groups;
     const int b = bk / a.Hkv;
-    const int len = clamp_len(a.slens[b], a.s_pages, a.P);
+    const bool item = split < a.s_splits;
+    const int len = item ? clamp_len(a.slens[b], a.s_pages, a.P) : 0;
     const int each = range_tokens(len, a.s_splits);
     it.t_begin = split * each;
-    if (it.t_begin >= len) return;
     it.t_end = min(len, it.t_begin + each);
-    it.table = a.btab + (int64_t)b * a.btab_stride;
-    it.kvh = bk - b * a.Hkv;
-    it.b0 = b;
+    if (own_waves == 4 && it.t_begin >= it.t_end) return;
+    it.table = a.btab + (int64_t)(item ? b : 0) * a.btab_stride;
+    it.kvh = item ? bk - b * a.Hkv : 0;
+    it.b0 = item ? b : 0;
     it.rows = a.G;
     it.row0 = hg * 32;
     it.slot = a.p_splits + split;
-    shared_stream<T, DPAD>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
+    shared_stream<T, DPAD>(a, it, own_waves, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
                            (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1, (LC_LDS float*)lds_ml);
   }
 }
@@ -760,27 +857,44 @@ __global__ __launch_bounds__(64) void shared_merge_kernel(SharedArgs a, T* __res
 }
 
 struct SharedPlan {
-  int wr;  // a prefix workgroup's row tiles of 32
+  int wr;         // row tiles of 32 of a prefix's workgroups
+  int own_waves;  // waves that share a range of a sequence's own tokens
   int p_splits, s_splits;
 };
 
-// Ranges per prefix and per sequence: about one round of the workgroups that the
-// CUs hold at once (two each) over all tokens, no range shorter than two tiles.
+// Ranges per prefix and per sequence, such that a range is what one CU would do if
+// all tokens were dealt out evenly: every further range costs its partial outputs
+// (512 bytes a row, written and read back) and a start. A prefix token of a 128-row
+// tile counts as four of a stream's, of a 64-row tile as two (GPU time of a call,
+// us, by ranges per prefix; 8B heads):
+//   256 x (8192 + 200) tokens  2: 109  3: 88  4: 78  5: 78  6: 83  8: 91
+//   64 x (8192 + 625)          8: 52  12: 52  16: 54  20: 69  32: 69
+//   4 groups x 8 x (4096 + 128)  4: 23.8  6: 23.2  8: 27  13: 27  16: 33
+// No range is shorter than two tiles.
+// A range of a sequence's own tokens is shared by 4, 2 or 1 waves: one wave has no
+// join at the end and a longer run of steps, which pays with many short ranges
+// (256 x 200 tokens: 88 / 79 / 78 us with 4 / 2 / 1 waves; 64 x 625: 53 / 52 / 59);
+// where the ranges are few, four finish sooner.
 SharedPlan shared_plan(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_cap,
                        int64_t s_cap) {
-  if (B == 0) return SharedPlan{1, 0, 0};
-  const int64_t G = Hq / Hkv, W = B / N;
+  if (B == 0) return SharedPlan{1, 4, 0, 0};
+  const int64_t G = Hq / Hkv, W = B / N, cus = lc_cu_count();
   const int wr = W * G <= 32 ? 1 : W * G <= 64 ? 2 : 4;
   const int64_t up = N * Hkv * lc_cdiv(W * G, 32 * wr), us = B * Hkv * lc_cdiv(G, 32);
-  const int64_t total = up * p_cap + us * s_cap;
-  int64_t each = lc_cdiv(total, 2 * lc_cu_count());
-  if (each < 2 * kSharedStep) each = 2 * kSharedStep;
-  auto splits = [&](int64_t cap) -> int {
+  const int64_t each = lc_cdiv(up * p_cap * wr + us * s_cap, cus);
+  auto splits = [&](int64_t cap, int64_t tokens) -> int {
     if (cap == 0) return 0;
-    const int64_t s = lc_cdiv(cap, each);
+    const int64_t s = lc_cdiv(cap, tokens < 2 * kSharedStep ? 2 * kSharedStep : tokens);
     return static_cast<int>(s < 64 ? s : 64);
   };
-  return SharedPlan{wr, splits(p_cap), splits(s_cap)};
+  SharedPlan p;
+  p.wr = wr;
+  p.p_splits = splits(p_cap, lc_cdiv(each, wr));
+  p.s_splits = splits(s_cap, each);
+  const int64_t ranges = us * p.s_splits;
+  const int64_t steps = p.s_splits > 0 ? lc_cdiv(lc_cdiv(s_cap, p.s_splits), 32) : 0;
+  p.own_waves = ranges < 2 * cus || steps > 40 ? 4 : steps > 12 ? 2 : 1;
+  return p;
 }
 
 int64_t shared_bytes(int64_t rows, int64_t D, const SharedPlan& p) {
@@ -803,32 +917,34 @@ int launch_merge(const SharedArgs& a, void* out, int64_t o_sb, int64_t o_sh, flo
 }
 
 template <typename T, int DPAD>
-int launch_mfma(const SharedArgs& a, int wr, hipStream_t st) {
+int launch_mfma(const SharedArgs& a, int wr, int own_waves, hipStream_t st) {
   const int64_t row_tiles = lc_cdiv((int64_t)a.W * a.G, 32 * wr), head_groups = lc_cdiv(a.G, 32);
   const int64_t pairs = (int64_t)(a.B / a.W) * a.Hkv * a.p_splits;
   const int64_t p_blocks = lc_cdiv(pairs, 8) * 8 * row_tiles;
-  const int64_t blocks = p_blocks + (int64_t)a.B * a.Hkv * head_groups * a.s_splits;
+  const int64_t items = (int64_t)a.B * a.Hkv * head_groups * a.s_splits;
+  const int64_t blocks = p_blocks + lc_cdiv(items, 4 / own_waves);
   LC_REQUIRE(blocks < (1LL << 24), "lc_shared_prefix_decode_fwd: %lld workgroups",
              (long long)blocks);
   const dim3 grid(static_cast<unsigned>(blocks));
   const int pb = static_cast<int>(p_blocks), rt = static_cast<int>(row_tiles),
             hg = static_cast<int>(head_groups);
   if (wr == 1)
-    shared_mfma_kernel<T, DPAD, 1><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+    shared_mfma_kernel<T, DPAD, 1><<<grid, 256, 0, st>>>(a, pb, rt, hg, own_waves);
   else if (wr == 2)
-    shared_mfma_kernel<T, DPAD, 2><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+    shared_mfma_kernel<T, DPAD, 2><<<grid, 256, 0, st>>>(a, pb, rt, hg, own_waves);
   else
-    shared_mfma_kernel<T, DPAD, 4><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+    shared_mfma_kernel<T, DPAD, 4><<<grid, 256, 0, st>>>(a, pb, rt, hg, own_waves);
   return lc_check_launch("lc_shared_prefix_decode_fwd (mfma)");
 }
 
 template <typename T>
-int launch_shared(const SharedArgs& a, int wr, bool mfma, void* out, int64_t o_sb, int64_t o_sh,
+int launch_shared(const SharedArgs& a, int wr, int own_waves, bool mfma, void* out, int64_t o_sb, int64_t o_sh,
                   float* lse, hipStream_t st) {
   const int splits = a.p_splits + a.s_splits;
   if (splits > 0 && mfma) {
     if constexpr (sizeof(T) == 2) {
-      const int rc = a.D <= 64 ? launch_mfma<T, 64>(a, wr, st) : launch_mfma<T, 128>(a, wr, st);
+      const int rc = a.D <= 64 ? launch_mfma<T, 64>(a, wr, own_waves, st)
+                                 : launch_mfma<T, 128>(a, wr, own_waves, st);
       if (rc != LC_OK) return rc;
     }
   } else if (splits > 0) {
@@ -932,16 +1048,16 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
   a.scale_log2 = scale * kLog2e;
   const bool mfma = dtype != LC_DTYPE_F32 && D % 8 == 0 && D <= 128 && q_sb % 8 == 0 &&
                     q_sh % 8 == 0 && kv_s_page % 8 == 0 && kv_s_head % 8 == 0 &&
-                    kv_s_tok % 8 == 0 && a.p_shift >= 3 && kv_s_tok < (1LL << 24) && lc_aligned(q, 16) && lc_aligned(key_pages, 16) &&
+                    kv_s_tok % 8 == 0 && a.p_shift >= 3 && kv_s_tok < (1LL << 31) / (2 * page_size) && kv_s_page < (1LL << 32) && scale > 0 && lc_aligned(q, 16) && lc_aligned(key_pages, 16) &&
                     lc_aligned(value_pages, 16);
   hipStream_t st = lc_stream(stream);
   switch (dtype) {
     case LC_DTYPE_F32:
-      return launch_shared<float>(a, plan.wr, false, out, o_sb, o_sh, lse, st);
+      return launch_shared<float>(a, plan.wr, plan.own_waves, false, out, o_sb, o_sh, lse, st);
     case LC_DTYPE_BF16:
-      return launch_shared<bf16_t>(a, plan.wr, mfma, out, o_sb, o_sh, lse, st);
+      return launch_shared<bf16_t>(a, plan.wr, plan.own_waves, mfma, out, o_sb, o_sh, lse, st);
     default:
-      return launch_shared<f16_t>(a, plan.wr, mfma, out, o_sb, o_sh, lse, st);
+      return launch_shared<f16_t>(a, plan.wr, plan.own_waves, mfma, out, o_sb, o_sh, lse, st);
   }
 }
 
