@@ -490,7 +490,7 @@ LC_API int lc_paged_kv_gather(const void* key_pages, const void* value_pages, in
 LC_API int64_t lc_shared_prefix_decode_workspace_bytes(int64_t B, int64_t groups, int64_t Hq,
                                                        int64_t Hkv, int64_t D,
                                                        int64_t prefix_capacity,
-                                                       int64_t own_capacity);
+                                                       int64_t own_capacity, int dtype);
 
 /* Paged GQA decode of a batch whose groups of sequences share a prefix: one
  * query token per sequence. The B sequences are `groups` groups of W = B /

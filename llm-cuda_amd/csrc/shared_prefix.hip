@@ -12,6 +12,7 @@
 // the workspace, and a merge launch joins them.
 #include <math.h>
 
+#include "attn_f32.h"
 #include "attn_tiles.h"
 #include "lc_common.h"
 
@@ -724,9 +725,53 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
   if (row_ok && wg == 0 && hh == 0) a.part_lse[pidx] = l == 0.f ? -INFINITY : m + lc_log2(l);
 }
 
+// Work of block `id` below p_blocks: a range of a prefix and `tile_rows` of its
+// group's rows. A range's row tiles read the same K and V: they get block ids 8
+// apart, which run on one XCD, and find it in its L2. False: no work.
+__device__ __forceinline__ bool prefix_item(const SharedArgs& a, int id, int row_tiles,
+                                            int tile_rows, RangeItem& it) {
+  const int run = id / (8 * row_tiles), rest = id - run * 8 * row_tiles;
+  const int pair = run * 8 + (rest & 7), tile = rest >> 3;
+  const int units = (a.B / a.W) * a.Hkv;
+  const int split = pair / units, u = pair - split * units;
+  if (split >= a.p_splits) return false;
+  const int n = u / a.Hkv;
+  const int len = clamp_len(a.plens[n], a.p_pages, a.P);
+  const int each = range_tokens(len, a.p_splits);
+  it.t_begin = split * each;
+  it.t_end = min(len, it.t_begin + each);
+  it.table = a.ptab + (int64_t)n * a.ptab_stride;
+  it.kvh = u - n * a.Hkv;
+  it.b0 = n * a.W;
+  it.rows = a.W * a.G;
+  it.row0 = tile * tile_rows;
+  it.slot = split;
+  return it.t_begin < it.t_end;
+}
+
+// Item i of the sequences' own ranges: all kv heads of a sequence follow one another
+// (one table row, and neighbours in a page). An item without tokens is left empty.
+__device__ __forceinline__ void own_item(const SharedArgs& a, int i, int head_groups,
+                                         RangeItem& it) {
+  const int units = a.B * a.Hkv * head_groups;
+  const int split = i / units, u = i - split * units;
+  const int hg = u % head_groups, bk = u / head_groups;
+  const int b = bk / a.Hkv;
+  const bool item = split < a.s_splits;
+  const int len = item ? clamp_len(a.slens[b], a.s_pages, a.P) : 0;
+  const int each = range_tokens(len, a.s_splits);
+  it.t_begin = split * each;
+  it.t_end = min(len, it.t_begin + each);
+  it.table = a.btab + (int64_t)(item ? b : 0) * a.btab_stride;
+  it.kvh = item ? bk - b * a.Hkv : 0;
+  it.b0 = item ? b : 0;
+  it.rows = a.G;
+  it.row0 = hg * 32;
+  it.slot = a.p_splits + split;
+}
+
 // Workgroups below p_blocks take the prefixes' ranges, the others the sequences'
-// own. A prefix range's row tiles read the same K and V: they get block ids 8
-// apart, which run on one XCD, and find it in its L2.
+// own, 4 / own_waves of them each.
 template <typename T, int DPAD, int WR>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
 shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups, int own_waves) {
@@ -737,55 +782,180 @@ shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups, i
   __shared__ __align__(16) char lds_v0[TILE_B];
   __shared__ __align__(16) char lds_v1[TILE_B];
   __shared__ float lds_ml[4 * 128];
+  LC_LDS char *k0 = (LC_LDS char*)lds_k0, *k1 = (LC_LDS char*)lds_k1;
+  LC_LDS char *v0 = (LC_LDS char*)lds_v0, *v1 = (LC_LDS char*)lds_v1;
   RangeItem it;
   const int id = blockIdx.x;
   if (id < p_blocks) {
-    const int run = id / (8 * row_tiles), rest = id - run * 8 * row_tiles;
-    const int pair = run * 8 + (rest & 7), tile = rest >> 3;
-    const int units = (a.B / a.W) * a.Hkv;
-    const int split = pair / units, u = pair - split * units;
-    if (split >= a.p_splits) return;
-    const int n = u / a.Hkv;
-    const int len = clamp_len(a.plens[n], a.p_pages, a.P);
-    const int each = range_tokens(len, a.p_splits);
-    it.t_begin = split * each;
-    if (it.t_begin >= len) return;
-    it.t_end = min(len, it.t_begin + each);
-    it.table = a.ptab + (int64_t)n * a.ptab_stride;
-    it.kvh = u - n * a.Hkv;
-    it.b0 = n * a.W;
-    it.rows = a.W * a.G;
-    it.row0 = tile * 32 * WR;
-    it.slot = split;
+    if (!prefix_item(a, id, row_tiles, 32 * WR, it)) return;
     if constexpr (WR > 1)
-      shared_range<T, DPAD, WR>(a, it, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
-                                (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1);
+      shared_range<T, DPAD, WR>(a, it, k0, k1, v0, v1);
     else
-      shared_stream<T, DPAD>(a, it, 4, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
-                             (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1, (LC_LDS float*)lds_ml);
+      shared_stream<T, DPAD>(a, it, 4, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
   } else {
-    // Item i: all kv heads of a sequence follow one another (one table row, and
-    // neighbours in a page).
-    const int units = a.B * a.Hkv * head_groups;
-    const int i = (id - p_blocks) * (4 / own_waves) +
-                  __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / own_waves;
-    const int split = i / units, u = i - split * units;
-    const int hg = u % head_groups, bk = u / head_groups;
-    const int b = bk / a.Hkv;
-    const bool item = split < a.s_splits;
-    const int len = item ? clamp_len(a.slens[b], a.s_pages, a.P) : 0;
-    const int each = range_tokens(len, a.s_splits);
-    it.t_begin = split * each;
-    it.t_end = min(len, it.t_begin + each);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    own_item(a, (id - p_blocks) * (4 / own_waves) + wave / own_waves, head_groups, it);
     if (own_waves == 4 && it.t_begin >= it.t_end) return;
-    it.table = a.btab + (int64_t)(item ? b : 0) * a.btab_stride;
-    it.kvh = item ? bk - b * a.Hkv : 0;
-    it.b0 = item ? b : 0;
-    it.rows = a.G;
-    it.row0 = hg * 32;
-    it.slot = a.p_splits + split;
-    shared_stream<T, DPAD>(a, it, own_waves, (LC_LDS char*)lds_k0, (LC_LDS char*)lds_k1,
-                           (LC_LDS char*)lds_v0, (LC_LDS char*)lds_v1, (LC_LDS float*)lds_ml);
+    shared_stream<T, DPAD>(a, it, own_waves, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// fp32 on v_mfma_f32_32x32x2_f32 (head_dim a multiple of 4 up to 128, pages of a
+// power of two from 8 up): 32 rows per workgroup, whose 4 waves take every fourth
+// 32-token step of the range and are joined through LDS. Operands come straight
+// from global memory into registers, in the forms of attn_f32.h: a K row per lane,
+// at the lane's own address; V rows in groups of 8 tokens, which share a page.
+// Bound by the fp32 matrix rate where rows fill the tile, else by the start and the
+// latency of few steps.
+// ---------------------------------------------------------------------------
+template <int DPAD>
+__global__ __launch_bounds__(256) __attribute__((
+    amdgpu_waves_per_eu(DPAD <= 64 ? 2 : 1, DPAD <= 64 ? 2 : 1))) void
+shared_f32_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
+  constexpr int DTL = DPAD / 32, LD = DPAD + 4, NC = DPAD / 8;
+  __shared__ __align__(16) float slab[4][32 * LD];
+  __shared__ float ms[4][32], ls[4][32];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hh = lane >> 5;
+  RangeItem it;
+  const int id = blockIdx.x;
+  if (id < p_blocks) {
+    if (!prefix_item(a, id, row_tiles, 32, it)) return;
+  } else {
+    own_item(a, id - p_blocks, head_groups, it);
+    if (it.t_begin >= it.t_end) return;
+  }
+
+  const int r_abs = it.row0 + l32;
+  const bool row_ok = r_abs < it.rows;
+  F32Row<DPAD> q, k;
+  {
+    const int r = row_ok ? r_abs : it.row0;
+    const float* qh = static_cast<const float*>(a.q) + (int64_t)(it.b0 + r / a.G) * a.q_sb +
+                      (int64_t)(it.kvh * a.G + r % a.G) * a.q_sh;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int d = i * 8 + hh * 4;
+      const bool ok = row_ok && d < a.D;
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(qh + (ok ? d : 0));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q.c[i][e] = ok ? x[e] : 0.f;
+    }
+  }
+  const float* kp = static_cast<const float*>(a.kp) + (int64_t)it.kvh * a.s_head;
+  const float* vp = static_cast<const float*>(a.vp) + (int64_t)it.kvh * a.s_head;
+  const int last_page = (it.t_end - 1) >> a.p_shift;
+  auto fetch = [&](int t) { return it.table[min((t + l32) >> a.p_shift, last_page)]; };
+  auto place = [&](int t, int page) { return row_place<8>(a, page, t + l32, it.t_end, 4); };
+  auto load_k = [&](const RowPlace& at) {
+    const char* row = reinterpret_cast<const char*>(kp) +
+                      ((static_cast<uint64_t>(at.hi) << 32) | at.lo) + hh * 16;
+    const char* none = reinterpret_cast<const char*>(shared_zeros);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const bool ok = at.bytes != 0 && i * 8 + hh * 4 < a.D;
+      k.c[i] = *reinterpret_cast<const f32x4_t*>(ok ? row + i * 32 : none);
+    }
+  };
+  const int row_b = static_cast<int>(a.s_tok * 4);
+  const int v_off = l32 * DTL < a.D ? 4 * hh * row_b + l32 * DTL * 4 : kF32Oob;
+
+  f32x16_t o[DTL];
+#pragma unroll
+  for (int dt = 0; dt < DTL; ++dt) f32_zero(o[dt]);
+  float m = -INFINITY, l = 0.f;
+  constexpr int kNext = 4 * 32;
+  const int t0 = it.t_begin + wave * 32;
+  RowPlace at{};
+  int page_next = 0;
+  if (t0 < it.t_end) {
+    const int page = fetch(t0);
+    page_next = fetch(t0 + kNext);
+    at = place(t0, page);
+    load_k(at);
+  }
+  for (int t = t0; t < it.t_end; t += kNext) {
+    const uint32_t live = static_cast<uint32_t>(__ballot(at.bytes != 0));
+    F32Cols<DTL> v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __amdgpu_buffer_rsrc_t rs = row_buffer(vp, at, j * 8);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v.n[j * 4 + i] = f32_load_dims<DTL>(
+            rs, static_cast<int>(static_cast<unsigned>(v_off) + static_cast<unsigned>(i * row_b)));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16_t s;
+    f32_zero(s);
+    f32_dot<DPAD>(s, k, q);
+    at = place(t + kNext, page_next);
+    page_next = fetch(t + 2 * kNext);
+    load_k(at);
+    __builtin_amdgcn_sched_barrier(0);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] *= a.scale_log2;
+      if (live != 0xffffffffu && !((live >> (8 * (r >> 2) + 4 * hh + (r & 3))) & 1))
+        s[r] = -INFINITY;
+      mx = fmaxf(mx, s[r]);
+    }
+    const float m_new = fmaxf(m, pf_half_max(mx));
+    if (__ballot(m_new > m) != 0) {
+      const float alpha = m_new == -INFINITY ? 1.f : lc_exp2(m - m_new);
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DTL; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+      m = m_new;
+    }
+    const float m_use = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = lc_exp2(s[r] - m_use);
+      l += s[r];
+    }
+    f32_outer<DTL>(o, v, s);
+  }
+
+  l += __shfl_xor(l, 32, 64);
+  f32_put<DPAD>(slab[wave], o, l32, hh);
+  if (hh == 0) {
+    ms[wave][l32] = m;
+    ls[wave][l32] = l;
+  }
+  __syncthreads();
+  constexpr int CPR = DPAD / 4;
+#pragma unroll
+  for (int e = tid; e < 32 * CPR; e += 256) {
+    const int row = e / CPR, d = (e - row * CPR) * 4, r = it.row0 + row;
+    if (r >= it.rows || d >= a.D) continue;
+    float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ms[w][row]);
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      // (a wave without tokens has m = -inf, l = 0 and O = 0; NaN passes)
+      const float mw = ms[w][row], lw = ls[w][row];
+      const float f = lw == 0.f ? 0.f : mw == -INFINITY ? 1.f : lc_exp2(mw - mt);
+      lt = fmaf(lw, f, lt);
+      const f32x4_t ow = *reinterpret_cast<const f32x4_t*>(&slab[w][row * LD + d]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(ow[i], f, acc[i]);
+    }
+    const float inv = lt == 0.f ? 0.f : 1.0f / lt;
+    const int b = it.b0 + r / a.G, h = it.kvh * a.G + r % a.G;
+    const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
+    f32x4_t out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = acc[i] * inv;
+    *reinterpret_cast<f32x4_t*>(a.part_o + pidx * a.D + d) = out;
+    if (d == 0) a.part_lse[pidx] = lt == 0.f ? -INFINITY : mt + lc_log2(lt);
   }
 }
 
@@ -876,10 +1046,10 @@ struct SharedPlan {
 // (256 x 200 tokens: 88 / 79 / 78 us with 4 / 2 / 1 waves; 64 x 625: 53 / 52 / 59);
 // where the ranges are few, four finish sooner.
 SharedPlan shared_plan(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_cap,
-                       int64_t s_cap) {
+                       int64_t s_cap, int dtype) {
   if (B == 0) return SharedPlan{1, 4, 0, 0};
   const int64_t G = Hq / Hkv, W = B / N, cus = lc_cu_count();
-  const int wr = W * G <= 32 ? 1 : W * G <= 64 ? 2 : 4;
+  const int wr = dtype == LC_DTYPE_F32 || W * G <= 32 ? 1 : W * G <= 64 ? 2 : 4;
   const int64_t up = N * Hkv * lc_cdiv(W * G, 32 * wr), us = B * Hkv * lc_cdiv(G, 32);
   const int64_t each = lc_cdiv(up * p_cap * wr + us * s_cap, cus);
   auto splits = [&](int64_t cap, int64_t tokens) -> int {
@@ -937,6 +1107,25 @@ int launch_mfma(const SharedArgs& a, int wr, int own_waves, hipStream_t st) {
   return lc_check_launch("lc_shared_prefix_decode_fwd (mfma)");
 }
 
+int launch_f32(const SharedArgs& a, hipStream_t st) {
+  const int64_t row_tiles = lc_cdiv((int64_t)a.W * a.G, 32), head_groups = lc_cdiv(a.G, 32);
+  const int64_t pairs = (int64_t)(a.B / a.W) * a.Hkv * a.p_splits;
+  const int64_t p_blocks = lc_cdiv(pairs, 8) * 8 * row_tiles;
+  const int64_t blocks = p_blocks + (int64_t)a.B * a.Hkv * head_groups * a.s_splits;
+  LC_REQUIRE(blocks < (1LL << 24), "lc_shared_prefix_decode_fwd: %lld workgroups",
+             (long long)blocks);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  const int pb = static_cast<int>(p_blocks), rt = static_cast<int>(row_tiles),
+            hg = static_cast<int>(head_groups);
+  if (a.D <= 32)
+    shared_f32_kernel<32><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+  else if (a.D <= 64)
+    shared_f32_kernel<64><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+  else
+    shared_f32_kernel<128><<<grid, 256, 0, st>>>(a, pb, rt, hg);
+  return lc_check_launch("lc_shared_prefix_decode_fwd (fp32 mfma)");
+}
+
 template <typename T>
 int launch_shared(const SharedArgs& a, int wr, int own_waves, bool mfma, void* out, int64_t o_sb, int64_t o_sh,
                   float* lse, hipStream_t st) {
@@ -945,6 +1134,9 @@ int launch_shared(const SharedArgs& a, int wr, int own_waves, bool mfma, void* o
     if constexpr (sizeof(T) == 2) {
       const int rc = a.D <= 64 ? launch_mfma<T, 64>(a, wr, own_waves, st)
                                  : launch_mfma<T, 128>(a, wr, own_waves, st);
+      if (rc != LC_OK) return rc;
+    } else {
+      const int rc = launch_f32(a, st);
       if (rc != LC_OK) return rc;
     }
   } else if (splits > 0) {
@@ -961,11 +1153,12 @@ extern "C" {
 
 int64_t lc_shared_prefix_decode_workspace_bytes(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv,
                                                 int64_t D, int64_t prefix_capacity,
-                                                int64_t own_capacity) {
+                                                int64_t own_capacity, int dtype) {
   if (B < 0 || groups <= 0 || B % groups != 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || D <= 0 ||
       prefix_capacity < 0 || own_capacity < 0)
     return -1;
-  return shared_bytes(B * Hq, D, shared_plan(B, groups, Hq, Hkv, prefix_capacity, own_capacity));
+  return shared_bytes(B * Hq, D,
+                      shared_plan(B, groups, Hq, Hkv, prefix_capacity, own_capacity, dtype));
 }
 
 int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const void* key_pages,
@@ -1006,7 +1199,7 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
                  kv_s_head >= 0 && kv_s_tok >= 0,
              "%s: negative stride", who);
   const SharedPlan plan = shared_plan(B, groups, Hq, Hkv, max_prefix_pages * page_size,
-                                      max_pages_per_seq * page_size);
+                                      max_pages_per_seq * page_size, dtype);
   const int64_t need = shared_bytes(B * Hq, D, plan);
   if (workspace_bytes < need)
     return lc_fail(LC_EWORKSPACE, "%s: workspace %lld < %lld bytes", who,
@@ -1046,14 +1239,18 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
   a.p_splits = plan.p_splits;
   a.s_splits = plan.s_splits;
   a.scale_log2 = scale * kLog2e;
-  const bool mfma = dtype != LC_DTYPE_F32 && D % 8 == 0 && D <= 128 && q_sb % 8 == 0 &&
-                    q_sh % 8 == 0 && kv_s_page % 8 == 0 && kv_s_head % 8 == 0 &&
-                    kv_s_tok % 8 == 0 && a.p_shift >= 3 && kv_s_tok < (1LL << 31) / (2 * page_size) && kv_s_page < (1LL << 32) && scale > 0 && lc_aligned(q, 16) && lc_aligned(key_pages, 16) &&
-                    lc_aligned(value_pages, 16);
+  // The matrix kernels take whole 16-byte vectors of rows, pages of a power of two
+  // from 8 tokens up, and 32-bit strides (a page's rows within 2 GiB).
+  const int64_t vec = 16 / lc_dtype_size(dtype);
+  const bool mfma = D % vec == 0 && D <= 128 && q_sb % vec == 0 && q_sh % vec == 0 &&
+                    kv_s_page % vec == 0 && kv_s_head % vec == 0 && kv_s_tok % vec == 0 &&
+                    a.p_shift >= 3 && kv_s_tok < (1LL << 29) / page_size &&
+                    kv_s_page < (1LL << 32) && scale > 0 && lc_aligned(q, 16) &&
+                    lc_aligned(key_pages, 16) && lc_aligned(value_pages, 16);
   hipStream_t st = lc_stream(stream);
   switch (dtype) {
     case LC_DTYPE_F32:
-      return launch_shared<float>(a, plan.wr, plan.own_waves, false, out, o_sb, o_sh, lse, st);
+      return launch_shared<float>(a, plan.wr, plan.own_waves, mfma, out, o_sb, o_sh, lse, st);
     case LC_DTYPE_BF16:
       return launch_shared<bf16_t>(a, plan.wr, plan.own_waves, mfma, out, o_sb, o_sh, lse, st);
     default:

@@ -149,7 +149,7 @@ _SIGNATURES = {
         [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p],
     ),
-    "lc_shared_prefix_decode_workspace_bytes": (_c_i64, [_c_i64] * 7),
+    "lc_shared_prefix_decode_workspace_bytes": (_c_i64, [_c_i64] * 7 + [ctypes.c_int]),
     "lc_shared_prefix_decode_fwd": (
         ctypes.c_int,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,

@@ -1403,7 +1403,7 @@ def _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, 
     if B > 0:
         lib = nat.load()
         need = nat.size("lc_shared_prefix_decode_workspace_bytes", B, N, Hq, Hkv, D,
-                        prefix_table.shape[1] * P, block_table.shape[1] * P)
+                        prefix_table.shape[1] * P, block_table.shape[1] * P, dtype)
         ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
         with _guard(dev):
             rc = lib.lc_shared_prefix_decode_fwd(

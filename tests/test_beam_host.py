@@ -146,11 +146,11 @@ def test_workspace_sizes():
     from llm_cuda import _native
 
     lib = _native.load()
-    assert lib.lc_shared_prefix_decode_workspace_bytes(4, 3, 4, 2, 16, 8, 8) == -1
-    assert lib.lc_shared_prefix_decode_workspace_bytes(4, 2, 4, 3, 16, 8, 8) == -1
-    assert lib.lc_shared_prefix_decode_workspace_bytes(0, 2, 4, 2, 16, 8, 8) == 0
+    assert lib.lc_shared_prefix_decode_workspace_bytes(4, 3, 4, 2, 16, 8, 8, 0) == -1
+    assert lib.lc_shared_prefix_decode_workspace_bytes(4, 2, 4, 3, 16, 8, 8, 0) == -1
+    assert lib.lc_shared_prefix_decode_workspace_bytes(0, 2, 4, 2, 16, 8, 8, 0) == 0
     # both parts present: at least one range each of fp32 output and logsumexp per row
-    assert lib.lc_shared_prefix_decode_workspace_bytes(4, 2, 4, 2, 16, 8, 8) >= 4 * 4 * 2 * (16 + 1) * 4
+    assert lib.lc_shared_prefix_decode_workspace_bytes(4, 2, 4, 2, 16, 8, 8, 0) >= 4 * 4 * 2 * (16 + 1) * 4
     assert lib.lc_beam_select_workspace_bytes(1, 4, 0, 4) == -1
     assert lib.lc_beam_select_workspace_bytes(0, 4, 10, 4) == 0
 
