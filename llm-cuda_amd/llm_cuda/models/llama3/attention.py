@@ -43,7 +43,7 @@ from llm_cuda.kernels.triton.decode_attention import (
 
 from .config import Llama3Config
 from .fused import FusedLinearWeights
-from .kv_cache import PagedKVLayerCache
+from .kv_cache import BeamKVLayerCache, PagedKVLayerCache
 from .rotary import apply_rotary, build_inv_freq, build_rope_cache
 
 
@@ -107,6 +107,38 @@ class Llama3Attention(nn.Module):
         bsz, seq_len, _ = x.shape
         return x.view(bsz, seq_len, heads, self.head_dim).transpose(1, 2)
 
+    def _project_out(self, out: torch.Tensor, partial_out: bool):
+        """o_proj of a decode step's attention output [B, H, 1, D]."""
+        bsz, _, seq_len, _ = out.shape
+        out = out.transpose(1, 2).reshape(bsz, seq_len, self.num_heads * self.head_dim)
+        wo = self.o_proj.weight
+        if partial_out and _ops.decode_linear_partials_applies(out, wo):
+            return _ops.decode_linear_partials(out, wo)
+        if _ops.decode_linear_applies(out, wo):
+            return _ops.decode_linear(out, wo)
+        return _ops.project(out, self.o_proj)
+
+    def _beam_forward(self, q, k, v, attention_mask, cache: BeamKVLayerCache, use_cache: bool,
+                      partial_out: bool):
+        """A step of a beam search: the prompts, [groups, seq], which fill the shared
+        prefix, then one token of every beam, [groups * width, 1]."""
+        if attention_mask is not None:
+            raise NotImplementedError("attention_mask with a beam cache")
+        if not use_cache:
+            raise ValueError("a beam cache needs use_cache=True")
+        bsz, _, seq_len, _ = q.shape
+        if cache.prefix_length == 0:
+            cos, sin = self._rope_tables(0, seq_len, q.device, q.dtype)
+            q, k = apply_rotary(q, k, cos, sin)
+            cache.append_prompt(k, v)
+            out = triton_fused_causal_attention(q, k, v)
+            out = out.transpose(1, 2).reshape(bsz, seq_len, self.num_heads * self.head_dim)
+            return _ops.project(out, self.o_proj), cache
+        own_rows = cache.cache.block_table.shape[1] * cache.cache.page_size
+        self._rope_tables(0, cache.prefix_length + own_rows, q.device, q.dtype)
+        q = cache.append_rotated(q, k, v, self._rope_cache[2], self._rope_cache[3])
+        return self._project_out(cache.attend(q), partial_out), cache
+
     def forward(
         self,
         x: torch.Tensor,
@@ -132,6 +164,10 @@ class Llama3Attention(nn.Module):
             q = self._shape(self.q_proj(x), self.num_heads)
             k = self._shape(self.k_proj(x), self.num_kv_heads)
             v = self._shape(self.v_proj(x), self.num_kv_heads)
+
+        if isinstance(past_key_value, BeamKVLayerCache):
+            return self._beam_forward(q, k, v, attention_mask, past_key_value, use_cache,
+                                      partial_out)
 
         paged = isinstance(past_key_value, PagedKVLayerCache)
         if paged:
@@ -159,13 +195,7 @@ class Llama3Attention(nn.Module):
                 out = paged_decode_attention(
                     q, cache.key_pages, cache.value_pages, cache.block_table, cache.seq_lens,
                     attention_mask=attention_mask, uniform_length=cache.uniform_length)
-            out = out.transpose(1, 2).reshape(bsz, seq_len, self.num_heads * self.head_dim)
-            wo = self.o_proj.weight
-            if partial_out and _ops.decode_linear_partials_applies(out, wo):
-                return _ops.decode_linear_partials(out, wo), cache
-            if _ops.decode_linear_applies(out, wo):
-                return _ops.decode_linear(out, wo), cache
-            return _ops.project(out, self.o_proj), cache
+            return self._project_out(out, partial_out), cache
 
         cos, sin = self._rope_tables(past_len, seq_len, x.device, x.dtype)
         q, k = apply_rotary(q, k, cos, sin)

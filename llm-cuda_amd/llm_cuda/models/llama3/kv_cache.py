@@ -14,6 +14,8 @@ t % page_size of that sequence's pages. What changes:
     loop of 2*seq slice copies; `get_kv` is one HIP gather (lc_paged_kv_gather)
     instead of a torch.cat of pages. The decode path does not call get_kv at
     all: it reads the pools in place (paged_decode_attention).
+
+`BeamKVCache` is the cache of a beam search (no counterpart in the reference).
 """
 from __future__ import annotations
 
@@ -244,3 +246,98 @@ class PagedKVCache:
     def clear(self) -> None:
         for layer in self.layer_caches:
             layer.clear()
+
+
+class BeamKVLayerCache:
+    """One layer of a BeamKVCache: views of its pools, tables and lengths."""
+
+    def __init__(self, cache: "BeamKVCache", layer: int):
+        self.cache = cache
+        self.key_pages = cache.key_pages[layer]
+        self.value_pages = cache.value_pages[layer]
+        self.prefix_lens = cache.prefix_lens_all[layer]
+        self.seq_lens = cache.seq_lens_all[layer]
+        self.prefix_length = 0  # host mirrors of the (equal) lengths
+        self.length = 0
+
+    def append_prompt(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The prompts' (rotated) keys and values, [groups, kv_heads, seq, head_dim]."""
+        c = self.cache
+        if k.shape != v.shape or k.dim() != 4 or k.shape[0] != c.groups:
+            raise ValueError(f"expected k and v of {c.groups} prompts, [groups, kv_heads, seq, "
+                             f"head_dim]; got {tuple(k.shape)} and {tuple(v.shape)}")
+        if self.prefix_length:
+            raise ValueError("the cache already holds its prompts")
+        if k.shape[2] > c.max_prefix_len:
+            raise ValueError("the prompts exceed max_prefix_len")
+        _ops.kv_append(k, v, self.key_pages, self.value_pages, c.prefix_table, self.prefix_lens)
+        self.prefix_lens.add_(k.shape[2])
+        self.prefix_length = k.shape[2]
+
+    def append_rotated(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        """Rotates every beam's q and k of one token, appends k and v to the beam's own
+        tokens and returns the rotated q. cos/sin: tables by position."""
+        c = self.cache
+        if k.shape != v.shape or k.dim() != 4 or k.shape[0] != c.batch_size or k.shape[2] != 1:
+            raise ValueError(f"expected one token of {c.batch_size} beams, [beams, kv_heads, 1, "
+                             f"head_dim]; got {tuple(k.shape)} and {tuple(v.shape)}")
+        if self.length + 1 > c.max_new_len:
+            raise ValueError("Appending would exceed max_new_len")
+        # The kernel places a token by its beam's own length; its position follows the
+        # prompt's, so the tables start there.
+        rows = c.block_table.shape[1] * c.page_size
+        at = slice(self.prefix_length, self.prefix_length + rows)
+        q = _ops.rope_kv_append(q, k, v, cos[at], sin[at], self.key_pages, self.value_pages,
+                                c.block_table, self.seq_lens)
+        self.length += 1
+        return q
+
+    def attend(self, q: torch.Tensor) -> torch.Tensor:
+        """Attention of q [beams, heads, 1, head_dim] over prompt and own tokens."""
+        c = self.cache
+        return _ops.shared_prefix_decode(q, self.key_pages, self.value_pages, c.prefix_table,
+                                         self.prefix_lens, c.block_table, self.seq_lens)
+
+
+class BeamKVCache:
+    """The paged cache of a beam search: `groups` prompts of equal length, `width` beams
+    each. A prompt's pages are stored once for all of its beams (prefix_table); a beam's
+    own tokens are in pages named by block_table, whole pages of which beams share after
+    a `reorder`. The layers' pools are one tensor [layers, pages, kv_heads, page_size,
+    head_dim], which share both tables."""
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, groups: int, width: int,
+                 max_prefix_len: int, max_new_len: int, page_size: int, device: torch.device,
+                 dtype: torch.dtype):
+        if min(num_layers, groups, width, max_prefix_len, max_new_len, page_size) <= 0:
+            raise ValueError("layers, groups, width, lengths and page_size must be > 0")
+        device = torch.device(device)
+        self.groups, self.width, self.batch_size = groups, width, groups * width
+        self.max_prefix_len, self.max_new_len, self.page_size = (max_prefix_len, max_new_len,
+                                                                 page_size)
+        prefix_pages = math.ceil(max_prefix_len / page_size)
+        own_pages = math.ceil(max_new_len / page_size)
+        shared = groups * prefix_pages
+        pool = shared + self.batch_size * own_pages
+        pages = torch.arange(pool, dtype=torch.int32, device=device)
+        self.prefix_table = pages[:shared].view(groups, prefix_pages)
+        self.block_table = pages[shared:].view(self.batch_size, own_pages)
+        self.key_pages = torch.empty(num_layers, pool, num_kv_heads, page_size, head_dim,
+                                     device=device, dtype=dtype)
+        self.value_pages = torch.empty_like(self.key_pages)
+        self.prefix_lens_all = torch.zeros(num_layers, groups, dtype=torch.int32, device=device)
+        self.seq_lens_all = torch.zeros(num_layers, self.batch_size, dtype=torch.int32,
+                                        device=device)
+        self.layer_caches = [BeamKVLayerCache(self, i) for i in range(num_layers)]
+
+    def get_layer(self, layer_idx: int) -> BeamKVLayerCache:
+        return self.layer_caches[layer_idx]
+
+    def reorder(self, parents: torch.Tensor) -> None:
+        """Beam w of prompt n continues what its beam parents[n, w] (int64) holds."""
+        if tuple(parents.shape) != (self.groups, self.width):
+            raise ValueError(f"parents must be {(self.groups, self.width)}, got "
+                             f"{tuple(parents.shape)}")
+        self.block_table.copy_(_ops.paged_kv_reorder(
+            self.key_pages, self.value_pages, self.block_table, self.seq_lens_all[0], parents))

@@ -14,11 +14,12 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from llm_cuda.kernels import _ops
 from llm_cuda.kernels._ops import add_rms_norm, lm_head_argmax
 
 from .attention import Llama3Attention
 from .config import Llama3Config
-from .kv_cache import PagedKVCache, PagedKVLayerCache
+from .kv_cache import BeamKVCache, PagedKVCache, PagedKVLayerCache
 from .mlp import Llama3MLP
 from .norm import RMSNorm
 
@@ -93,7 +94,7 @@ class Llama3Model(nn.Module):
         use_cache: bool = False,
     ) -> dict:
         x = self.embed_tokens(input_ids)
-        paged = isinstance(past_key_values, PagedKVCache)
+        paged = isinstance(past_key_values, (PagedKVCache, BeamKVCache))
         presents: list[tuple[torch.Tensor, torch.Tensor]] = []
         # Each layer's closing residual add is fused with the next norm (the
         # next layer's input norm, or the final norm): `pending` carries the
@@ -242,3 +243,110 @@ class Llama3ForCausalLM(nn.Module):
         if return_logit:
             return ids.unsqueeze(-1), out["past_key_values"], best
         return ids.unsqueeze(-1), out["past_key_values"]
+
+    @torch.no_grad()
+    def beam_search(
+        self,
+        input_ids: torch.Tensor,
+        num_beams: int,
+        max_new_tokens: int = 16,
+        page_size: int = 64,
+        eos_token_id: int | None = None,
+        use_graph: bool = False,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """Beam search over prompts [N, S]: (ids [N, num_beams, S + max_new_tokens],
+        scores fp32 [N, num_beams]), the best beam of each prompt first. An extension
+        (the reference decodes greedily, model.py:200-218).
+
+        A score is the sum of the log-probabilities of the beam's new tokens; every
+        step keeps the num_beams best continuations over all beams and tokens (ties:
+        the lower beam, then the lower token). With eos_token_id a beam that produced
+        it is finished: it keeps its score and is continued with that token only. The
+        prompts are computed and stored once; per token the attention computes a
+        prompt's part once for all of its beams, and the cache follows the selected
+        beams without copying whole pages.
+
+        use_graph: the prompts and the first step over the beams run eagerly, the next
+        step is captured in a HIP graph and replayed for every later token, with the
+        eager steps' results.
+        """
+        if input_ids.dim() != 2 or input_ids.shape[1] == 0:
+            raise ValueError(f"input_ids must be [prompts, tokens], got {tuple(input_ids.shape)}")
+        N, S = input_ids.shape
+        W, V, T = int(num_beams), self.config.vocab_size, int(max_new_tokens)
+        if not 1 <= W <= min(64, V):
+            raise ValueError(f"num_beams {W} not in [1, min(64, vocab_size)]")
+        if T < 1:
+            raise ValueError("max_new_tokens must be >= 1")
+        if eos_token_id is not None and not 0 <= int(eos_token_id) < V:
+            raise ValueError(f"eos_token_id {eos_token_id} outside a vocabulary of {V}")
+        self.eval()
+        dev = input_ids.device
+        if N == 0:
+            return (input_ids.new_empty((0, W, S + T)),
+                    torch.empty((0, W), dtype=torch.float32, device=dev))
+        cache = BeamKVCache(
+            num_layers=self.config.num_hidden_layers,
+            num_kv_heads=self.config.num_key_value_heads,
+            head_dim=self.config.head_dim,
+            groups=N,
+            width=W,
+            max_prefix_len=S,
+            max_new_len=max(1, T - 1),  # the last token is not appended
+            page_size=page_size,
+            device=dev,
+            dtype=self.model.embed_tokens.weight.dtype,
+        )
+
+        def select(ids, scores, finished):
+            hidden = self.model(ids, past_key_values=cache, use_cache=True)["hidden_states"]
+            hidden, weight = hidden[:, -1, :], self.lm_head.weight
+            if _ops.decode_linear_applies(hidden, weight):
+                logits = _ops.decode_linear(hidden, weight)
+            else:
+                logits = self.lm_head(hidden)
+            got = _ops.beam_select(logits.view(N, -1, V), scores, num_candidates=W,
+                                   finished=finished, eos_token_id=eos_token_id)
+            return got if finished is not None else (*got, None)
+
+        def beam_step(ids, scores, finished):
+            scores, tokens, parents, finished = select(ids, scores, finished)
+            cache.reorder(parents)
+            return scores, tokens, parents, finished
+
+        done = None
+        if eos_token_id is not None:
+            done = torch.zeros(N, 1, dtype=torch.bool, device=dev)
+        scores, tokens, parents, done = select(
+            input_ids, torch.zeros(N, 1, dtype=torch.float32, device=dev), done)
+        history = [(tokens, parents)]
+        eager = min(T, 2) if use_graph else T
+        for _ in range(1, eager):
+            scores, tokens, parents, done = beam_step(tokens.view(N * W, 1), scores, done)
+            history.append((tokens, parents))
+        if eager < T:
+            # As in generate: the eager step allocated what a step needs; the captured
+            # kernels take lengths, tables and the beams' state from device memory.
+            ids, state, ended = tokens.clone(), scores.clone(), None if done is None else done.clone()
+            lengths = [layer.length for layer in cache.layer_caches]
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = beam_step(ids.view(N * W, 1), state, ended)
+                state.copy_(out[0])
+                ids.copy_(out[1])
+                if ended is not None:
+                    ended.copy_(out[3])
+            for step in range(eager, T):
+                graph.replay()
+                history.append((out[1].clone(), out[2].clone()))
+            for layer, length in zip(cache.layer_caches, lengths):
+                layer.length = length + T - eager
+            scores = state
+        # Follow the parents back from the last step.
+        at = torch.arange(W, device=dev).expand(N, W)
+        line = []
+        for tokens, parents in reversed(history):
+            line.append(torch.gather(tokens, 1, at))
+            at = torch.gather(parents, 1, at)
+        new = torch.stack(line[::-1], dim=2)
+        return torch.cat([input_ids.unsqueeze(1).expand(N, W, S), new], dim=2), scores

@@ -93,3 +93,27 @@ def kv_reorder(key_pages, value_pages, block_table, seq_lens, parents):
                         new_pool[..., dst, :, :fill, :] = pool[..., src, :, :fill, :]
             seen.add(p)
     return kp, vp, new
+
+
+def beam_search(state, cfg, input_ids, width, max_new_tokens, eos=None):
+    """(ids [N, width, S + n], scores [N, width] float64, smallest gap between a kept and a
+    dropped candidate) by full recomputation of every beam at every step."""
+    from .model import forward
+
+    N, S = input_ids.shape
+    ids = input_ids.cpu().unsqueeze(1)
+    scores = torch.zeros(N, 1, dtype=torch.float64)
+    done = None if eos is None else torch.zeros(N, 1, dtype=torch.bool)
+    gap = math.inf
+    for _ in range(max_new_tokens):
+        n, w, length = ids.shape
+        logits = forward(state, cfg, ids.reshape(n * w, length))[:, -1].view(n, w, -1)
+        count = min(width + 1, w * logits.shape[-1])
+        best, tokens, parents, fin = beam_select(logits, scores, count, done, eos)
+        if count > width:
+            gap = min(gap, (best[:, :-1] - best[:, 1:]).min().item())
+        scores, tokens, parents = best[:, :width], tokens[:, :width], parents[:, :width]
+        done = None if fin is None else fin[:, :width]
+        ids = torch.cat([torch.gather(ids, 1, parents.unsqueeze(-1).expand(-1, -1, length)),
+                         tokens.unsqueeze(-1)], dim=2)
+    return ids, scores, gap
