@@ -1354,72 +1354,95 @@ def shared_prefix_decode(q: torch.Tensor, key_pages: torch.Tensor, value_pages: 
     seq_lens int32 [B]: each sequence's own tokens. Returns out with q's shape
     (and lse [B, Hq] fp32 if return_lse).
     """
-    args = (prefix_table, prefix_lens, block_table, seq_lens, scale, return_lse)
     if _records_grad(q, key_pages, value_pages):
-        return _ForwardOnly.apply("shared_prefix_decode",
-                                  lambda a, k, v: _shared_prefix_decode(a, k, v, *args),
-                                  q, key_pages, value_pages)
-    return _shared_prefix_decode(q, key_pages, value_pages, *args)
+        return _ForwardOnly.apply(
+            "shared_prefix_decode",
+            lambda a, k, v: _shared_prefix_decode(a, k, v, prefix_table, prefix_lens, block_table,
+                                                  seq_lens, scale, return_lse),
+            q, key_pages, value_pages)
+    return _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, block_table,
+                                 seq_lens, scale, return_lse)
 
 
-def _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, block_table,
-                          seq_lens, scale, return_lse):
-    squeeze = q.dim() == 3
-    q4 = q.unsqueeze(2) if squeeze else q
-    if q4.dim() != 4 or q4.shape[2] != 1:
-        raise ValueError(f"q must be [batch, heads, 1, head_dim], got {tuple(q.shape)}")
-    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape:
+@functools.lru_cache(maxsize=1024)
+def _shared_prefix_sizes(q, k, v, prefix_table, prefix_lens, block_table, seq_lens, ks, vs, lc_dtype):
+    """Checks the shapes of a shared_prefix_decode call; (batch, groups, heads, kv heads,
+    head_dim, page size, pages, prefix pages, own pages, workspace bytes, whether the pools'
+    strides ks and vs do). A function of its arguments alone, run once for each."""
+    if len(q) not in (3, 4) or (len(q) == 4 and q[2] != 1):
+        raise ValueError(f"q must be [batch, heads, 1, head_dim], got {tuple(q)}")
+    if len(k) != 4 or k != v:
         raise ValueError("key_pages and value_pages must both be [num_pages, kv_heads, page, dim]")
-    B, Hq, _, D = q4.shape
-    num_pages, Hkv, P, Dk = key_pages.shape
+    B, Hq, D = q[0], q[1], q[-1]
+    num_pages, Hkv, P, Dk = k
     if Dk != D:
         raise ValueError(f"head_dim mismatch: q {D}, pages {Dk}")
     if Hkv == 0 or Hq % Hkv != 0:
         raise ValueError(f"n_heads ({Hq}) must be a multiple of n_kv_heads ({Hkv})")
-    for t in (prefix_table, prefix_lens, block_table, seq_lens):
-        if t.dtype != torch.int32:
-            raise TypeError("prefix_table, prefix_lens, block_table and seq_lens must be int32")
-    if prefix_table.dim() != 2 or prefix_lens.shape != (prefix_table.shape[0],):
+    if len(prefix_table) != 2 or tuple(prefix_lens) != (prefix_table[0],):
         raise ValueError("prefix_table must be [groups, pages] and prefix_lens [groups]")
-    if block_table.dim() != 2 or block_table.shape[0] != B or seq_lens.shape != (B,):
+    if len(block_table) != 2 or block_table[0] != B or tuple(seq_lens) != (B,):
         raise ValueError("block_table must be [batch, max_pages] and seq_lens [batch]")
-    N = prefix_table.shape[0]
+    N = prefix_table[0]
     if (B % N != 0) if N else B != 0:
         raise ValueError(f"a batch of {B} sequences is not a multiple of {N} prefix groups")
-    if q4.dtype != key_pages.dtype or q4.dtype != value_pages.dtype:
-        raise TypeError("q and the page pools must share a dtype")
-    dtype = nat.lc_dtype(q4)
-    dev = nat.require_device(q4, key_pages, value_pages, prefix_table, prefix_lens, block_table,
-                             seq_lens)
-    if key_pages.stride() != value_pages.stride() or key_pages.stride(-1) != 1:
-        key_pages, value_pages = key_pages.contiguous(), value_pages.contiguous()
-    if q4.stride(-1) != 1:
-        q4 = q4.contiguous()
-    prefix_table, block_table = (t if t.shape[1] < 2 or t.stride(1) == 1 else t.contiguous()
-                                 for t in (prefix_table, block_table))
-    prefix_lens, seq_lens = prefix_lens.contiguous(), seq_lens.contiguous()
-    out = torch.empty((B, Hq, 1, D), dtype=q4.dtype, device=dev)
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
-    if B > 0:
-        lib = nat.load()
+    need = 0
+    if B:
         need = nat.size("lc_shared_prefix_decode_workspace_bytes", B, N, Hq, Hkv, D,
-                        prefix_table.shape[1] * P, block_table.shape[1] * P, dtype)
-        ws = torch.empty(max(need, 256), dtype=torch.uint8, device=dev)
+                        prefix_table[1] * P, block_table[1] * P, lc_dtype)
+    return (B, N, Hq, Hkv, D, P, num_pages, prefix_table[1], block_table[1], max(need, 256),
+            ks == vs and ks[-1] == 1)
+
+
+def _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, block_table,
+                          seq_lens, scale, return_lse):
+    i32 = torch.int32
+    if not (prefix_table.dtype is i32 and prefix_lens.dtype is i32 and block_table.dtype is i32
+            and seq_lens.dtype is i32):
+        raise TypeError("prefix_table, prefix_lens, block_table and seq_lens must be int32")
+    if not q.dtype is key_pages.dtype is value_pages.dtype:
+        raise TypeError("q and the page pools must share a dtype")
+    dtype = nat.lc_dtype(q)
+    ks = key_pages.stride()
+    B, N, Hq, Hkv, D, P, num_pages, p_pages, s_pages, ws_bytes, strides_ok = _shared_prefix_sizes(
+        q.shape, key_pages.shape, value_pages.shape, prefix_table.shape, prefix_lens.shape,
+        block_table.shape, seq_lens.shape, ks, value_pages.stride(), dtype)
+    dev = nat.require_device(q, key_pages, value_pages, prefix_table, prefix_lens, block_table,
+                             seq_lens)
+    if not strides_ok:
+        key_pages, value_pages = key_pages.contiguous(), value_pages.contiguous()
+        ks = key_pages.stride()
+    qs = q.stride()
+    if qs[-1] != 1:
+        q = q.contiguous()
+        qs = q.stride()
+    pt_s, bt_s = prefix_table.stride(), block_table.stride()
+    if p_pages > 1 and pt_s[1] != 1:
+        prefix_table = prefix_table.contiguous()
+        pt_s = prefix_table.stride()
+    if s_pages > 1 and bt_s[1] != 1:
+        block_table = block_table.contiguous()
+        bt_s = block_table.stride()
+    prefix_lens, seq_lens = prefix_lens.contiguous(), seq_lens.contiguous()
+    # (in q's order of dimensions: the token's heads side by side for a projection's view)
+    out = torch.empty_like(q)
+    os = out.stride()
+    if os[-1] != 1:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        os = out.stride()
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
+    if B:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         with _guard(dev):
-            rc = lib.lc_shared_prefix_decode_fwd(
-                q4.data_ptr(), q4.stride(0), q4.stride(1), key_pages.data_ptr(),
-                value_pages.data_ptr(), key_pages.stride(0), key_pages.stride(1),
-                key_pages.stride(2), num_pages, prefix_table.data_ptr(),
-                max(prefix_table.stride(0), prefix_table.shape[1]), prefix_table.shape[1],
-                prefix_lens.data_ptr(), block_table.data_ptr(),
-                max(block_table.stride(0), block_table.shape[1]), block_table.shape[1],
-                seq_lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
-                None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), B, N, Hq,
-                Hkv, D, P, float(1.0 / math.sqrt(D) if scale is None else scale), dtype,
-                _stream(dev))
-        nat.check(rc, "lc_shared_prefix_decode_fwd")
-    if squeeze:
-        out = out.squeeze(2)
+            rc = nat.load().lc_shared_prefix_decode_fwd(
+                q.data_ptr(), qs[0], qs[1], key_pages.data_ptr(), value_pages.data_ptr(), ks[0],
+                ks[1], ks[2], num_pages, prefix_table.data_ptr(), max(pt_s[0], p_pages), p_pages,
+                prefix_lens.data_ptr(), block_table.data_ptr(), max(bt_s[0], s_pages), s_pages,
+                seq_lens.data_ptr(), out.data_ptr(), os[0], os[1],
+                None if lse is None else lse.data_ptr(), ws.data_ptr(), ws_bytes, B, N, Hq, Hkv,
+                D, P, 1.0 / math.sqrt(D) if scale is None else float(scale), dtype, _stream(dev))
+        if rc:
+            nat.check(rc, "lc_shared_prefix_decode_fwd")
     return (out, lse) if return_lse else out
 
 
@@ -1444,49 +1467,68 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_candidates: int 
     return _beam_select(logits, scores, num_candidates, finished, eos_token_id)
 
 
-def _beam_select(logits, scores, num_candidates, finished, eos_token_id):
-    if logits.dim() != 3:
-        raise ValueError(f"logits must be [groups, beams, vocab], got {tuple(logits.shape)}")
-    N, W, V = logits.shape
-    if scores.shape != (N, W):
-        raise ValueError(f"scores must be {(N, W)}, got {tuple(scores.shape)}")
-    if scores.dtype != torch.float32:
-        raise TypeError(f"scores must be float32, got {scores.dtype}")
-    K = W if num_candidates is None else int(num_candidates)
+@functools.lru_cache(maxsize=1024)
+def _beam_sizes(logits, scores, num_candidates, finished, eos_token_id):
+    """Checks the sizes of a beam_select call; (groups, beams, vocab, candidates, workspace
+    bytes). A function of its arguments alone, run once for each."""
+    if len(logits) != 3:
+        raise ValueError(f"logits must be [groups, beams, vocab], got {tuple(logits)}")
+    N, W, V = logits
+    if tuple(scores) != (N, W):
+        raise ValueError(f"scores must be {(N, W)}, got {tuple(scores)}")
+    K = W if num_candidates is None else num_candidates
     if not (1 <= W <= 256 and V >= 1 and 1 <= K <= min(64, W * V)):
         raise ValueError(f"{K} candidates of {W} beams x {V} tokens: beams are 1 to 256, "
                          "candidates 1 to min(64, beams * vocab)")
     if W * V >= 2 ** 31:
         raise ValueError(f"{W} beams x {V} tokens: 2^31 or more")
     if finished is not None:
-        if finished.dtype != torch.bool or finished.shape != (N, W):
+        if tuple(finished) != (N, W):
             raise TypeError(f"finished must be bool {(N, W)}")
         if eos_token_id is None:
             raise ValueError("finished needs eos_token_id")
-        if not 0 <= int(eos_token_id) < V:
+        if not 0 <= eos_token_id < V:
             raise ValueError(f"eos_token_id {eos_token_id} outside a vocabulary of {V}")
+    return N, W, V, K, nat.size("lc_beam_select_workspace_bytes", N, W, V, K)
+
+
+def _beam_select(logits, scores, num_candidates, finished, eos_token_id):
+    if scores.dtype is not torch.float32:
+        raise TypeError(f"scores must be float32, got {scores.dtype}")
+    if finished is not None and finished.dtype is not torch.bool:
+        raise TypeError(f"finished must be bool, got {finished.dtype}")
+    N, W, V, K, ws_bytes = _beam_sizes(
+        logits.shape, scores.shape, None if num_candidates is None else int(num_candidates),
+        None if finished is None else finished.shape,
+        None if eos_token_id is None else int(eos_token_id))
     dtype = nat.lc_dtype(logits)
     dev = nat.require_device(logits, scores, finished)
-    if V > 1 and logits.stride(2) != 1:
+    ls = logits.stride()
+    if V > 1 and ls[2] != 1:
         logits = logits.contiguous()
+        ls = logits.stride()
     scores = scores.contiguous()
-    finished = None if finished is None else finished.contiguous()
-    out_s = torch.empty((N, K), dtype=torch.float32, device=dev)
-    out_t = torch.empty((N, K), dtype=torch.int64, device=dev)
-    out_p = torch.empty((N, K), dtype=torch.int64, device=dev)
-    out_f = None if finished is None else torch.empty((N, K), dtype=torch.bool, device=dev)
-    if N > 0:
-        lib = nat.load()
-        ws = torch.empty(nat.size("lc_beam_select_workspace_bytes", N, W, V, K),
-                         dtype=torch.uint8, device=dev)
+    # (tokens and parents in one allocation, as its two rows)
+    tokens, parents = torch.empty((2, N, K), dtype=torch.int64, device=dev).unbind()
+    out = torch.empty_like(scores) if K == W else torch.empty((N, K), dtype=torch.float32,
+                                                              device=dev)
+    done = None
+    if finished is not None:
+        finished = finished.contiguous()
+        done = torch.empty_like(finished) if K == W else torch.empty((N, K), dtype=torch.bool,
+                                                                     device=dev)
+    if N:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         with _guard(dev):
-            rc = lib.lc_beam_select(
-                logits.data_ptr(), logits.stride(0), logits.stride(1), scores.data_ptr(),
-                nat.ptr(finished), 0 if finished is None else int(eos_token_id), N, W, V, K,
-                out_s.data_ptr(), out_t.data_ptr(), out_p.data_ptr(), nat.ptr(out_f),
-                ws.data_ptr(), ws.numel(), dtype, _stream(dev))
-        nat.check(rc, "lc_beam_select")
-    return (out_s, out_t, out_p) if finished is None else (out_s, out_t, out_p, out_f)
+            rc = nat.load().lc_beam_select(
+                logits.data_ptr(), ls[0], ls[1], scores.data_ptr(),
+                None if finished is None else finished.data_ptr(),
+                0 if finished is None else int(eos_token_id), N, W, V, K, out.data_ptr(),
+                tokens.data_ptr(), parents.data_ptr(), None if done is None else done.data_ptr(),
+                ws.data_ptr(), ws_bytes, dtype, _stream(dev))
+        if rc:
+            nat.check(rc, "lc_beam_select")
+    return (out, tokens, parents) if done is None else (out, tokens, parents, done)
 
 
 def paged_kv_reorder(key_pages: torch.Tensor, value_pages: torch.Tensor,
@@ -1505,45 +1547,62 @@ def paged_kv_reorder(key_pages: torch.Tensor, value_pages: torch.Tensor,
     in the pools). out: an int32 [B, pages] buffer for the new table that does not
     overlap block_table.
     """
-    one = key_pages.dim() == 4
-    if key_pages.dim() not in (4, 5) or key_pages.shape != value_pages.shape:
-        raise ValueError("key_pages and value_pages must both be [layers, num_pages, kv_heads, "
-                         "page, dim]")
-    if key_pages.dtype != value_pages.dtype:
+    ks = key_pages.stride()
+    L, num_pages, Hkv, P, D, N, W, M, s_layer = _reorder_sizes(
+        key_pages.shape, value_pages.shape, ks, value_pages.stride(), block_table.shape,
+        seq_lens.shape, parents.shape)
+    if key_pages.dtype is not value_pages.dtype:
         raise TypeError("key_pages and value_pages must share a dtype")
     if key_pages.requires_grad or value_pages.requires_grad:
         raise NotImplementedError("paged_kv_reorder writes the pools in place: they cannot "
                                   "require grad")
-    if key_pages.stride() != value_pages.stride() or key_pages.stride(-1) != 1:
-        raise ValueError("key_pages and value_pages must share a layout with unit dim stride")
-    kp, vp = (key_pages.unsqueeze(0), value_pages.unsqueeze(0)) if one else (key_pages, value_pages)
-    L, num_pages, Hkv, P, D = kp.shape
-    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+    if block_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32:
         raise TypeError("block_table and seq_lens must be int32")
-    if parents.dtype != torch.int64 or parents.dim() != 2:
+    if parents.dtype is not torch.int64:
         raise TypeError("parents must be int64 [groups, beams]")
-    N, W = parents.shape
-    if block_table.dim() != 2 or block_table.shape[0] != N * W or seq_lens.shape != (N * W,):
+    dtype = nat.lc_dtype(key_pages)
+    dev = nat.require_device(key_pages, value_pages, block_table, seq_lens, parents, out)
+    ts = block_table.stride()
+    if M > 1 and ts[1] != 1:
+        block_table = block_table.contiguous()
+        ts = block_table.stride()
+    seq_lens, parents = seq_lens.contiguous(), parents.contiguous()
+    if out is None:
+        out = torch.empty((N * W, M), dtype=torch.int32, device=dev)
+        o_stride = M
+    else:
+        if out.dtype is not torch.int32 or out.shape != (N * W, M) or (M > 1 and out.stride(1) != 1):
+            raise ValueError(f"out must be int32 {(N * W, M)} with contiguous rows")
+        o_stride = max(out.stride(0), M)
+    if N * W and M:
+        with _guard(dev):
+            rc = nat.load().lc_paged_kv_reorder(
+                key_pages.data_ptr(), value_pages.data_ptr(), s_layer, ks[-4], ks[-3], ks[-2], L,
+                num_pages, block_table.data_ptr(), max(ts[0], M), out.data_ptr(), o_stride, M,
+                seq_lens.data_ptr(), parents.data_ptr(), N, W, Hkv, D, P, dtype, _stream(dev))
+        if rc:
+            nat.check(rc, "lc_paged_kv_reorder")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _reorder_sizes(k, v, ks, vs, block_table, seq_lens, parents):
+    """Checks the shapes of a paged_kv_reorder call; (layers, pages, kv heads, page size,
+    head_dim, groups, beams, table width, layer stride). A function of its arguments alone,
+    run once for each."""
+    if len(k) not in (4, 5) or k != v:
+        raise ValueError("key_pages and value_pages must both be [layers, num_pages, kv_heads, "
+                         "page, dim]")
+    if ks != vs or ks[-1] != 1:
+        raise ValueError("key_pages and value_pages must share a layout with unit dim stride")
+    L, s_layer = (k[0], ks[0]) if len(k) == 5 else (1, 0)
+    num_pages, Hkv, P, D = k[-4:]
+    if len(parents) != 2:
+        raise TypeError("parents must be int64 [groups, beams]")
+    N, W = parents
+    if len(block_table) != 2 or block_table[0] != N * W or tuple(seq_lens) != (N * W,):
         raise ValueError(f"block_table must be [{N * W}, pages] and seq_lens [{N * W}] for "
                          f"parents {(N, W)}")
     if N and not 1 <= W <= 256:
         raise ValueError(f"{W} beams: 1 to 256")
-    M = block_table.shape[1]
-    dtype = nat.lc_dtype(kp)
-    dev = nat.require_device(kp, vp, block_table, seq_lens, parents, out)
-    block_table = block_table if M < 2 or block_table.stride(1) == 1 else block_table.contiguous()
-    seq_lens, parents = seq_lens.contiguous(), parents.contiguous()
-    if out is None:
-        out = torch.empty((N * W, M), dtype=torch.int32, device=dev)
-    elif out.dtype != torch.int32 or out.shape != (N * W, M) or (M > 1 and out.stride(1) != 1):
-        raise ValueError(f"out must be int32 {(N * W, M)} with contiguous rows")
-    if N * W and M:
-        lib = nat.load()
-        with _guard(dev):
-            rc = lib.lc_paged_kv_reorder(
-                kp.data_ptr(), vp.data_ptr(), kp.stride(0), kp.stride(1), kp.stride(2),
-                kp.stride(3), L, num_pages, block_table.data_ptr(),
-                max(block_table.stride(0), M), out.data_ptr(), max(out.stride(0), M), M,
-                seq_lens.data_ptr(), parents.data_ptr(), N, W, Hkv, D, P, dtype, _stream(dev))
-        nat.check(rc, "lc_paged_kv_reorder")
-    return out
+    return L, num_pages, Hkv, P, D, N, W, block_table[1], s_layer
