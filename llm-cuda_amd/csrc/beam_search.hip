@@ -34,8 +34,9 @@ constexpr int kBeamWaves = kBeamThreads / 64;
 constexpr int kMaxCount = 64;      // candidates per group: lanes of a wave
 constexpr int kMaxWidth = 256;     // beams per group: threads of a workgroup
 constexpr int kWaveCap = 256;      // gathered keys of a chunk's wave
-constexpr int kTieSlack = 32;      // lanes past the K-th at its value before ties are cut by index
-constexpr int kMergeCap = 2048;    // gathered candidates of a group
+constexpr int kTieSlack = 8;       // lanes at the K-th value before ties are cut by index
+constexpr int kMergeCap = 4096;    // gathered candidates of a group
+constexpr int kReachCap = 1024;    // lists of a group whose candidates are looked through
 
 // Order-preserving bits of a float (not NaN); -0 counts as +0.
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -99,6 +100,17 @@ __device__ __forceinline__ float wave_reduce(float x, float none, F op) {
   step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());  // row_bcast:15
   step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());  // row_bcast:31
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ int wave_incl_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31
+  return x;
 }
 
 struct SelectArgs {
@@ -181,27 +193,19 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
     }
   }
 
-  // This wave's part of the softmax sum, relative to its largest logit. NaN and
-  // +inf make it NaN. 2^(v L - r) with r = ref L rounded: one rounding of the
-  // argument per term, and the factor 2^(ref L - r), common to all, taken off.
+  // This wave's part of the softmax sum, relative to its largest logit, whose term is
+  // exactly 1 (a beam with one logit left keeps its score). NaN and +inf make it NaN.
   float top = v[0];
 #pragma unroll
   for (int i = 1; i < ITEMS; ++i) top = fmaxf(top, v[i]);
   if (!(top >= -INFINITY)) top = -INFINITY;  // (all NaN)
   const float w_max = wave_reduce(top, -INFINITY, [](float p, float q) { return fmaxf(p, q); });
   const float ref = w_max == -INFINITY ? 0.f : w_max;
-  float part[4] = {0.f, 0.f, 0.f, 0.f}, scale = 1.f;
-  if (fabsf(ref) < 1e30f) {
-    const float shift = ref * kLog2e;
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) part[i % 4] += lc_exp2(fmaf(v[i], kLog2e, -shift));
-    scale = lc_exp2(-fmaf(ref, kLog2e, -shift));
-  } else {  // (ref L may not be finite)
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) part[i % 4] += lc_exp2((v[i] - ref) * kLog2e);
-  }
+  for (int i = 0; i < ITEMS; ++i) part[i % 4] += lc_exp2((v[i] - ref) * kLog2e);
   const float sum = wave_reduce((part[0] + part[1]) + (part[2] + part[3]), 0.f,
-                                [](float p, float q) { return p + q; }) * scale;
+                                [](float p, float q) { return p + q; });
 
   // Two lower bounds of the chunk's K-th largest from the lanes' largest values:
   // the K-th largest of one wave, and the least of the waves' q-th largest, q = K /
@@ -216,15 +220,24 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
   const int q = (a.K + kBeamWaves - 1) / kBeamWaves;
   const uint32_t tq = q == 1 ? ordered(w_max) : whole(wave_kth_largest<31, LOW>(key, q));
   uint32_t t_index = CHUNK - 1;
-  if (__popcll(__ballot(key >= t)) > a.K + kTieSlack) {
-    // Far more lanes than needed reach t: the lowest indices among those at t do.
+  if (__builtin_expect(t == ordered(-INFINITY) || __popcll(__ballot(key == t)) > kTieSlack, 0)) {
+    // Many elements at t (all masked ones, say): the lowest indices among them do. A
+    // lane's first vector, the wave's first VEC x 64 indices in order, mostly holds them.
     const float tv = from_ordered(t);
-    uint32_t low = 0;  // one more than the inverted lowest index of this lane's at t
-#pragma unroll
-    for (int i = ITEMS - 1; i >= 0; --i)
-      if (v[i] == tv) low = CHUNK - index_of(i);
     const int more = a.K - __popcll(__ballot(key > t));
-    t_index = CHUNK - wave_kth_largest<13, 0>(key == t ? low : 0, more);
+    int at_t = 0;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) at_t += v[i] == tv;
+    const unsigned long long full = __ballot(wave_incl_scan(at_t) >= more);
+    if (full != 0) {
+      t_index = (wave * 64 + __builtin_ctzll(full)) * VEC + VEC - 1;
+    } else {
+      uint32_t low = 0;  // one more than the inverted lowest index of this lane's at t
+#pragma unroll
+      for (int i = ITEMS - 1; i >= 0; --i)
+        if (v[i] == tv) low = CHUNK - index_of(i);
+      t_index = CHUNK - wave_kth_largest<13, 0>(key == t ? low : 0, more);
+    }
   }
   if (lane == 0) {
     w_top[wave] = w_max;
@@ -259,7 +272,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
       if (hit && pos < kWaveCap) list[wave][pos] = key_of(i);
       n_found += __popcll(hits);
     };
-    if (lim_index == CHUNK - 1) {
+    if (__builtin_expect(lim_index == CHUNK - 1, 1)) {
 #pragma unroll
       for (int i = 0; i < ITEMS; ++i) gather(i, v[i] >= lim);
     } else {
@@ -283,7 +296,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
     out[rank] = (k & 0xffffffff00000000ull) |
                 static_cast<uint32_t>(~(~static_cast<uint32_t>(k) + static_cast<uint32_t>(c0)));
   };
-  if (most <= kWaveCap) {
+  if (__builtin_expect(most <= kWaveCap, 1)) {
     // Four threads count the keys above each one, a wave's part of the list each.
     static_assert(kBeamWaves == 4, "a thread per part");
     const int seg = tid & 3, n_seg = found[seg];
@@ -354,8 +367,8 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a)
   __shared__ int kind[kMaxWidth];
   __shared__ uint64_t value[kMergeCap];
   __shared__ uint32_t flat[kMergeCap];  // inverted w V + v
-  __shared__ int reach[kMergeCap];      // lists whose best candidate reaches the bound
-  __shared__ uint32_t bound[kMergeWaves];
+  __shared__ int reach[kReachCap];      // lists whose best candidate reaches the bound
+  __shared__ uint64_t bound[kMergeWaves];
   __shared__ uint64_t best_v[kMergeWaves];
   __shared__ uint32_t best_f[kMergeWaves];
   __shared__ int count, reached;
@@ -453,15 +466,68 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a)
     candidate_of(l, k, a.keys[(n * lists + l) * K + k], v, f);
   };
 
-  // A lower bound of the K-th largest value (its upper 32 bits) from the lists'
-  // first candidates, as in the chunks; then the lists that reach it, and their
-  // candidates that do.
+  // Candidates below `limit` are out. A candidate's key is the upper half of its value
+  // and, for -inf alone (where equal halves are equal values), its inverted index.
+  const uint32_t none_hi = static_cast<uint32_t>(ordered64(-static_cast<double>(INFINITY)) >> 32);
+  auto key_of = [&](uint64_t v, uint32_t f) -> uint64_t {
+    const uint32_t hi = static_cast<uint32_t>(v >> 32);
+    return (static_cast<uint64_t>(hi) << 32) | (hi == none_hi ? f : 0);
+  };
+  uint64_t limit = 1;
+  auto add = [&](uint64_t v, uint32_t f) {  // (whole waves)
+    const bool hit = v != 0 && key_of(v, f) >= limit;
+    const unsigned long long hits = __ballot(hit);
+    if (hits == 0) return;
+    int first = 0;
+    if (lane == 0) first = atomicAdd(&count, __popcll(hits));
+    const int pos = __builtin_amdgcn_readfirstlane(first) + __popcll(hits & ((1ull << lane) - 1));
+    if (hit && pos < kMergeCap) {
+      value[pos] = v;
+      flat[pos] = f;
+    }
+  };
+  // Raises the limit to the least of the waves' q-th best gathered candidates, q = K /
+  // 16 rounded up (so K reach it), and drops what is below.
+  constexpr int kEach = kMergeCap / kMergeThreads;
+  auto prune = [&](int m) {
+    uint64_t v[kEach];
+    uint32_t f[kEach];
+    uint64_t best = 0;
+#pragma unroll
+    for (int r = 0; r < kEach; ++r) {
+      const int i = r * kMergeThreads + lane * kMergeWaves + wave;
+      v[r] = i < m ? value[i] : 0;
+      f[r] = i < m ? flat[i] : 0;
+      if (i < m) best = max(best, key_of(v[r], f[r]));
+    }
+    const int q = (K + kMergeWaves - 1) / kMergeWaves;
+    const uint32_t hi = static_cast<uint32_t>(best >> 32), lo = static_cast<uint32_t>(best);
+    const uint32_t t = wave_kth_largest<31, 0>(hi, q);
+    uint32_t cut = 0;
+    if (__builtin_expect(t == none_hi, 0)) {
+      const int more = q - __popcll(__ballot(hi > t));
+      cut = wave_kth_largest<31, 0>(hi == t ? lo : 0, more);
+    }
+    if (lane == 0) bound[wave] = (static_cast<uint64_t>(t) << 32) | cut;
+    __syncthreads();
+    uint64_t least = bound[0];
+#pragma unroll
+    for (int w = 1; w < kMergeWaves; ++w) least = min(least, bound[w]);
+    limit = max(limit, least);
+    if (tid == 0) count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kEach; ++r) add(v[r], f[r]);
+    __syncthreads();
+  };
+  // Each wave's K-th best list head is a lower bound of the K-th largest value.
   uint64_t head = 0, held_v[kHeld];
   uint32_t held_f[kHeld];
   if (few) {
 #pragma unroll
     for (int r = 0; r < kHeld; ++r) {
       held_v[r] = 0;
+      held_f[r] = 0;
       if (held_k[r] < K) candidate_of(held_l[r], held_k[r], held[r], held_v[r], held_f[r]);
       if (held_k[r] == 0) head = max(head, held_v[r]);
     }
@@ -474,46 +540,53 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a)
     }
   }
   const uint32_t t = wave_kth_largest<31, 0>(static_cast<uint32_t>(head >> 32), K);
-  if (lane == 0) bound[wave] = t;
+  if (lane == 0) bound[wave] = static_cast<uint64_t>(t) << 32;
   __syncthreads();
-  uint32_t limit = bound[0];
 #pragma unroll
-  for (int w = 1; w < kMergeWaves; ++w) limit = max(limit, bound[w]);
-  auto take_if = [&](uint64_t v, uint32_t f) {  // (whole waves)
-    const bool hit = v != 0 && static_cast<uint32_t>(v >> 32) >= limit;
-    const unsigned long long hits = __ballot(hit);
-    if (hits == 0) return;
-    int first = 0;
-    if (lane == 0) first = atomicAdd(&count, __popcll(hits));
-    const int pos = __builtin_amdgcn_readfirstlane(first) + __popcll(hits & ((1ull << lane) - 1));
-    if (hit && pos < kMergeCap) {
-      value[pos] = v;
-      flat[pos] = f;
-    }
-  };
+  for (int w = 0; w < kMergeWaves; ++w) limit = max(limit, bound[w]);
+  bool fits = true;
   if (few) {
 #pragma unroll
-    for (int r = 0; r < kHeld; ++r) take_if(held_v[r], held_f[r]);
+    for (int r = 0; r < kHeld; ++r) add(held_v[r], held_f[r]);
+    __syncthreads();
   } else {
     for (int l = tid; l < lists; l += kMergeThreads) {
       uint64_t v = head;
       uint32_t f;
       if (lists > kMergeThreads) candidate(l, 0, v, f);
-      if (v != 0 && static_cast<uint32_t>(v >> 32) >= limit) {
+      if (v != 0 && static_cast<uint32_t>(v >> 32) >= static_cast<uint32_t>(limit >> 32)) {
         const int pos = atomicAdd(&reached, 1);
-        if (pos < kMergeCap) reach[pos] = l;
+        if (pos < kReachCap) reach[pos] = l;
       }
     }
     __syncthreads();
-    const int nr = min(reached, kMergeCap);
-    for (int i = wave; i < nr; i += kMergeWaves) {
-      uint64_t v = 0;
-      uint32_t f = 0;
-      if (lane < K) candidate(reach[i], lane, v, f);
-      take_if(v, f);
+    // A wave takes one of these lists (of all, where they are too many), a lane one of
+    // its candidates; room for the next lists' is made after every two.
+    const bool listed = reached <= kReachCap;
+    const int n_lists = listed ? reached : lists;
+    constexpr int kRounds = kMergeCap / 2 / (kMergeWaves * kMaxCount);
+    for (int i0 = 0; i0 < n_lists; i0 += kRounds * kMergeWaves) {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const int i = i0 + r * kMergeWaves + wave;
+        uint64_t v = 0;
+        uint32_t f = 0;
+        if (i < n_lists && lane < K) candidate(listed ? reach[i] : i, lane, v, f);
+        add(v, f);
+      }
+      __syncthreads();
+      int m = count;
+      __syncthreads();
+      if (__builtin_expect(m > kMergeCap / 2, 0)) {
+        prune(m);
+        m = count;
+        __syncthreads();
+      }
+      fits = fits && m <= kMergeCap / 2;
     }
+    __syncthreads();
   }
-  __syncthreads();
+  for (int i = 0; i < 2 && __builtin_expect(fits && count > 2 * K + 64, 0); ++i) prune(count);
   const int m = count;
   auto store = [&](int rank, uint64_t v, uint32_t f) {
     const uint32_t at = ~f;
@@ -526,7 +599,7 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a)
     if (a.out_finished != nullptr)
       a.out_finished[o] = token == a.eos || (a.finished != nullptr && a.finished[n * a.W + w]);
   };
-  if (m <= kMergeCap && reached <= kMergeCap) {
+  if (__builtin_expect(fits, 1)) {
     // Eight threads count the candidates above each one.
     const int part = tid & 7;
     for (int i = tid >> 3; i < (m + 7) / 8 * 8; i += kMergeThreads / 8) {
@@ -580,10 +653,11 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a)
   }
 }
 
-// Logits of a row per workgroup: 8192 where that gives a round of workgroups (two
-// to a CU), else 2048, so that a few rows' latency is short.
+// Logits of a row per workgroup: 8192 where that gives every CU a workgroup, else
+// 2048, so that a few rows' latency is short (four times the lists to join: with 31
+// beams of 55157 the join took 17 us, the chunks 11).
 int beam_items(int64_t rows, int64_t V) {
-  return rows * lc_cdiv(V, kBeamThreads * 32) >= 2 * lc_cu_count() ? 32 : 8;
+  return rows * lc_cdiv(V, kBeamThreads * 32) >= lc_cu_count() ? 32 : 8;
 }
 int64_t beam_chunks(int64_t rows, int64_t V) {
   return lc_cdiv(V, kBeamThreads * beam_items(rows, V));

@@ -118,6 +118,34 @@ def test_masked_rows(cuda):
     check_select(x, torch.full((2, 4), -INF), count=8, dev=cuda)
 
 
+def test_a_forced_token_keeps_the_score(cuda):
+    """Rows with one logit left have a log-probability of exactly 0: they tie with finished
+    beams of the same score."""
+    x = torch.full((1, 4, 6000), -INF)
+    for w, at in enumerate((5999, 17, 2048, 300)):
+        x[0, w, at] = 1.4745025634765625 * (w + 1)
+    s = torch.tensor([[-1.0, -1.0, -1.0, -1.0]])
+    for dtype in (F32, BF16):
+        check_select(x.to(dtype), s, count=6, dev=cuda)
+        done = torch.tensor([[False, True, False, True]])
+        check_select(x.to(dtype), s, count=6, finished=done, eos=3, dev=cuda)
+        got = select(x.to(dtype).to(cuda), s.to(cuda))
+        assert (got[0] == -1.0).all()
+
+
+def test_few_logits_left(cuda):
+    """Constrained beams: so few tokens allowed that lists fill up with masked ones, with
+    more candidates wanted than any list has."""
+    for W, V, count, keep in ((27, 9176, 54, 0.001), (64, 4100, 64, 0.0005), (16, 20000, 32, 0.0001),
+                              (200, 3000, 64, 0.001)):
+        x, s = make(1, W, V, BF16, V)
+        g = torch.Generator().manual_seed(W)
+        x.masked_fill_(torch.rand(1, W, V, generator=g) > keep, -INF)
+        check_select(x, s, count=count, dev=cuda)
+        done = torch.rand(1, W, generator=g) < 0.3
+        check_select(x, s, count=count, finished=done, eos=V // 2, dev=cuda)
+
+
 def test_first_step(cuda):
     """Identical beams of which the first stands for all."""
     x, _ = make(2, 1, 5000, F16, 9)
