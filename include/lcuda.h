@@ -511,15 +511,21 @@ LC_API int64_t lc_shared_prefix_decode_workspace_bytes(int64_t B, int64_t groups
  *   prefix_lens int32 [groups] and seq_lens int32 [B] are clamped to the
  *   tables' capacities.
  * workspace: >= lc_shared_prefix_decode_workspace_bytes, 256-byte aligned; calls
- *   that may overlap need their own. */
+ *   that may overlap need their own.
+ * counters: lc_shared_prefix_decode_counter_count() int32 values that are zero at
+ *   entry and are left zero, or NULL. With them a call of few rows joins its token
+ *   ranges in the launch that computes them; without, or with many rows, a second
+ *   launch does, with the same result. Calls that may overlap need their own. */
+LC_API int64_t lc_shared_prefix_decode_counter_count(void);
 LC_API int lc_shared_prefix_decode_fwd(
     const void* q, int64_t q_sb, int64_t q_sh, const void* key_pages, const void* value_pages,
     int64_t kv_s_page, int64_t kv_s_head, int64_t kv_s_tok, int64_t num_pages,
     const int32_t* prefix_table, int64_t pt_stride, int64_t max_prefix_pages,
     const int32_t* prefix_lens, const int32_t* block_table, int64_t bt_stride,
     int64_t max_pages_per_seq, const int32_t* seq_lens, void* out, int64_t o_sb, int64_t o_sh,
-    float* lse, void* workspace, int64_t workspace_bytes, int64_t B, int64_t groups, int64_t Hq,
-    int64_t Hkv, int64_t D, int64_t page_size, float scale, int dtype, void* stream);
+    float* lse, void* workspace, int64_t workspace_bytes, int32_t* counters, int64_t B,
+    int64_t groups, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size, float scale, int dtype,
+    void* stream);
 
 /* Bytes of workspace lc_beam_select needs, or -1 for invalid sizes. */
 LC_API int64_t lc_beam_select_workspace_bytes(int64_t groups, int64_t width, int64_t vocab,

@@ -36,10 +36,24 @@ struct SharedArgs {
   float* part_lse;       // [B*Hq, p_splits + s_splits], log2 units
   int B, W, Hq, Hkv, G, D, P, p_shift, num_pages, p_pages, s_pages, p_splits, s_splits;
   float scale_log2;
+  // Not null: the last workgroup of a group and kv head to finish (its ticket on
+  // counters[n * Hkv + kvh], zero at entry and left zero) writes their output.
+  int* counters;
+  int expected;  // workgroups of a group and kv head
+  void* out;
+  int64_t o_sb, o_sh;
+  float* lse;
 };
 
 // Tokens of a range are a multiple of this.
 constexpr int kSharedStep = 64;
+
+// x as an fp32 value: a product that is converted to f16 next may otherwise be taken
+// by one instruction that rounds once, here and not there.
+__device__ __forceinline__ float rounded(float x) {
+  __asm__("" : "+v"(x));
+  return x;
+}
 
 __device__ __forceinline__ int clamp_len(int len, int pages, int P) {
   const int cap = pages * P;
@@ -233,6 +247,41 @@ __device__ __forceinline__ void operand_addresses(int lane, int row0, int (&kadd
     }
 }
 
+// A partial output or logsumexp. Where another workgroup of the same launch reads it
+// (on another XCD, maybe), it is written through to memory by relaxed stores of
+// device scope, and read by such loads: no cache has to be written back or
+// invalidated (fences did that for every workgroup: 20 us instead of 7).
+__device__ __forceinline__ void put4(const SharedArgs& a, float* to, f32x4_t x) {
+  if (a.counters != nullptr) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    uint64_t* p = reinterpret_cast<uint64_t*>(to);
+    __hip_atomic_store(p, __builtin_bit_cast(uint64_t, f32x2{x[0], x[1]}), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(p + 1, __builtin_bit_cast(uint64_t, f32x2{x[2], x[3]}), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  } else {
+    *reinterpret_cast<f32x4_t*>(to) = x;
+  }
+}
+__device__ __forceinline__ void put(const SharedArgs& a, float* to, float x) {
+  if (a.counters != nullptr)
+    __hip_atomic_store(to, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else
+    *to = x;
+}
+__device__ __forceinline__ float got(const float* from) {
+  return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x4_t got4(const float* from) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const uint64_t* p = reinterpret_cast<const uint64_t*>(from);
+  const f32x2 lo = __builtin_bit_cast(
+      f32x2, __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  const f32x2 hi = __builtin_bit_cast(
+      f32x2, __hip_atomic_load(p + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  return f32x4_t{lo[0], lo[1], hi[0], hi[1]};
+}
+
 // Writes columns dt * 32 .. of a row's partial output.
 __device__ __forceinline__ void store_columns(const SharedArgs& a, int64_t pidx, int dt, int hh,
                                               const f32x16_t& o, float inv_l) {
@@ -244,7 +293,7 @@ __device__ __forceinline__ void store_columns(const SharedArgs& a, int64_t pidx,
       f32x4_t w;
 #pragma unroll
       for (int e = 0; e < 4; ++e) w[e] = o[j * 4 + e] * inv_l;
-      *reinterpret_cast<f32x4_t*>(po + d0) = w;
+      put4(a, po + d0, w);
     }
   }
 }
@@ -521,7 +570,7 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
   const float inv_l = l_tot == 0.f ? 0.f : 1.0f / l_tot;
 #pragma unroll
   for (int dt = 0; dt < DTL; ++dt) store_columns(a, pidx, dt, hh, o[dt], inv_l);
-  if (hh == 0) a.part_lse[pidx] = l_tot == 0.f ? -INFINITY : m_ref + lc_log2(l_tot);
+  if (hh == 0) put(a, a.part_lse + pidx, l_tot == 0.f ? -INFINITY : m_ref + lc_log2(l_tot));
 }
 
 // Up to 32 rows: bound by reading K and V, so the waves stream on their own, without
@@ -722,12 +771,83 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
     }
     if (row_ok) store_columns(a, pidx, dt, hh, sum, inv_l);
   }
-  if (row_ok && wg == 0 && hh == 0) a.part_lse[pidx] = l == 0.f ? -INFINITY : m + lc_log2(l);
+  if (row_ok && wg == 0 && hh == 0)
+    put(a, a.part_lse + pidx, l == 0.f ? -INFINITY : m + lc_log2(l));
+}
+
+// The merge in the same launch, for few rows and ranges: every workgroup of group n
+// and kv head kvh takes a ticket after its partials, and the one with the last joins
+// all ranges of their rows, a thread per 4 columns. Which workgroup that is changes
+// nothing in the sums, which equal shared_merge_kernel's bit for bit. It saves the second launch (2.9 us of the host, 3.8 us of
+// the GPU at 4 beams of 1000 tokens); with many rows one workgroup would be slower
+// at it than the launch.
+constexpr int kJoinRanges = 16;          // most ranges per row
+constexpr int64_t kJoinBytes = 160 << 10;  // most partials of a group and kv head
+constexpr int kJoinCounters = 4096;
+
+template <typename T>
+__device__ __forceinline__ void join_last(const SharedArgs& a, int n, int kvh) {
+  __shared__ int last;
+  // (every wave's stores have reached memory before the ticket is taken)
+  __builtin_amdgcn_s_waitcnt(kWaitVm0Lgkm0);
+  lc_compiler_fence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int* c = a.counters + n * a.Hkv + kvh;
+    const int t = __hip_atomic_fetch_add(c, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = t == a.expected - 1;
+    if (last) __hip_atomic_store(c, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return;
+  lc_compiler_fence();
+  const int chunks = a.D / 4, total = a.W * a.G * chunks, stride = a.p_splits + a.s_splits;
+  const int n_p = range_count(clamp_len(a.plens[n], a.p_pages, a.P), a.p_splits);
+  for (int i = threadIdx.x; i < total; i += 256) {
+    const int r = i / chunks, d = (i - r * chunks) * 4;
+    const int b = n * a.W + r / a.G, h = kvh * a.G + r % a.G;
+    const int n_all = n_p + range_count(clamp_len(a.slens[b], a.s_pages, a.P), a.s_splits);
+    const int64_t base = ((int64_t)b * a.Hq + h) * stride;
+    float w[kJoinRanges], m = -INFINITY;
+    f32x4_t o[kJoinRanges];
+#pragma unroll
+    for (int j = 0; j < kJoinRanges; ++j) {
+      w[j] = -INFINITY;
+      if (j < n_all) {
+        const int64_t at = base + (j < n_p ? j : a.p_splits + (j - n_p));
+        w[j] = got(a.part_lse + at);
+        o[j] = got4(a.part_o + at * a.D + d);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kJoinRanges; ++j) m = fmaxf(m, w[j]);
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kJoinRanges; ++j) {
+      if (j < n_all) {
+        const float f = lc_exp2(w[j] - m_use);  // (NaN passes)
+        sum += f;
+        if (f != 0.f) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, o[j][e], acc[e]);
+        }
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    T* to = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = lc_from_f32<T>(rounded(acc[e] * inv));
+    if (a.lse != nullptr && d == 0)
+      a.lse[(int64_t)b * a.Hq + h] = sum == 0.f ? -INFINITY : (m_use + lc_log2(sum)) * kLn2;
+  }
 }
 
 // Work of block `id` below p_blocks: a range of a prefix and `tile_rows` of its
 // group's rows. A range's row tiles read the same K and V: they get block ids 8
-// apart, which run on one XCD, and find it in its L2. False: no work.
+// apart, which run on one XCD, and find it in its L2. False: a block past the last
+// range. The range may be empty.
 __device__ __forceinline__ bool prefix_item(const SharedArgs& a, int id, int row_tiles,
                                             int tile_rows, RangeItem& it) {
   const int run = id / (8 * row_tiles), rest = id - run * 8 * row_tiles;
@@ -746,7 +866,7 @@ __device__ __forceinline__ bool prefix_item(const SharedArgs& a, int id, int row
   it.rows = a.W * a.G;
   it.row0 = tile * tile_rows;
   it.slot = split;
-  return it.t_begin < it.t_end;
+  return true;
 }
 
 // Item i of the sequences' own ranges: all kv heads of a sequence follow one another
@@ -788,16 +908,19 @@ shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups, i
   const int id = blockIdx.x;
   if (id < p_blocks) {
     if (!prefix_item(a, id, row_tiles, 32 * WR, it)) return;
-    if constexpr (WR > 1)
-      shared_range<T, DPAD, WR>(a, it, k0, k1, v0, v1);
-    else
-      shared_stream<T, DPAD>(a, it, 4, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
+    if (it.t_begin < it.t_end) {
+      if constexpr (WR > 1)
+        shared_range<T, DPAD, WR>(a, it, k0, k1, v0, v1);
+      else
+        shared_stream<T, DPAD>(a, it, 4, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
+    }
   } else {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     own_item(a, (id - p_blocks) * (4 / own_waves) + wave / own_waves, head_groups, it);
-    if (own_waves == 4 && it.t_begin >= it.t_end) return;
-    shared_stream<T, DPAD>(a, it, own_waves, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
+    if (own_waves < 4 || it.t_begin < it.t_end)
+      shared_stream<T, DPAD>(a, it, own_waves, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
   }
+  if (a.counters != nullptr) join_last<T>(a, it.b0 / a.W, it.kvh);
 }
 
 // ---------------------------------------------------------------------------
@@ -810,24 +933,13 @@ shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups, i
 // latency of few steps.
 // ---------------------------------------------------------------------------
 template <int DPAD>
-__global__ __launch_bounds__(256) __attribute__((
-    amdgpu_waves_per_eu(DPAD <= 64 ? 2 : 1, DPAD <= 64 ? 2 : 1))) void
-shared_f32_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
+__device__ __forceinline__ void shared_f32_range(const SharedArgs& a, const RangeItem& it) {
   constexpr int DTL = DPAD / 32, LD = DPAD + 4, NC = DPAD / 8;
   __shared__ __align__(16) float slab[4][32 * LD];
   __shared__ float ms[4][32], ls[4][32];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hh = lane >> 5;
-  RangeItem it;
-  const int id = blockIdx.x;
-  if (id < p_blocks) {
-    if (!prefix_item(a, id, row_tiles, 32, it)) return;
-  } else {
-    own_item(a, id - p_blocks, head_groups, it);
-    if (it.t_begin >= it.t_end) return;
-  }
-
   const int r_abs = it.row0 + l32;
   const bool row_ok = r_abs < it.rows;
   F32Row<DPAD> q, k;
@@ -954,9 +1066,24 @@ shared_f32_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
     f32x4_t out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = acc[i] * inv;
-    *reinterpret_cast<f32x4_t*>(a.part_o + pidx * a.D + d) = out;
-    if (d == 0) a.part_lse[pidx] = lt == 0.f ? -INFINITY : mt + lc_log2(lt);
+    put4(a, a.part_o + pidx * a.D + d, out);
+    if (d == 0) put(a, a.part_lse + pidx, lt == 0.f ? -INFINITY : mt + lc_log2(lt));
   }
+}
+
+template <int DPAD>
+__global__ __launch_bounds__(256) __attribute__((
+    amdgpu_waves_per_eu(DPAD <= 64 ? 2 : 1, DPAD <= 64 ? 2 : 1))) void
+shared_f32_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
+  RangeItem it;
+  const int id = blockIdx.x;
+  if (id < p_blocks) {
+    if (!prefix_item(a, id, row_tiles, 32, it)) return;
+  } else {
+    own_item(a, id - p_blocks, head_groups, it);
+  }
+  if (it.t_begin < it.t_end) shared_f32_range<DPAD>(a, it);
+  if (a.counters != nullptr) join_last<float>(a, it.b0 / a.W, it.kvh);
 }
 
 // Merge: one wave per (sequence, query head) joins the live ranges of its
@@ -995,7 +1122,6 @@ __global__ __launch_bounds__(64) void shared_merge_kernel(SharedArgs a, T* __res
     for (int s0 = 0; s0 < n_all; s0 += 64) {
       const int n = min(64, n_all - s0);
       const float w = lane < n ? lc_exp2(a.part_lse[base + slot(s0 + lane)] - mx) : 0.f;
-      wsum += w;
       for (int j0 = 0; j0 < n; j0 += kBatch) {
         float v[kBatch][VPL];
 #pragma unroll
@@ -1008,7 +1134,8 @@ __global__ __launch_bounds__(64) void shared_merge_kernel(SharedArgs a, T* __res
         for (int jj = 0; jj < kBatch; ++jj) {
           const float wj =
               __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(j0 + jj, 63)));
-          if (j0 + jj < n && wj != 0.f) {
+          if (j0 + jj < n && wj != 0.f) {  // (range after range, as join_last sums them)
+            wsum += wj;
 #pragma unroll
             for (int e = 0; e < VPL; ++e) acc[e] = fmaf(wj, v[jj][e], acc[e]);
           }
@@ -1016,12 +1143,11 @@ __global__ __launch_bounds__(64) void shared_merge_kernel(SharedArgs a, T* __res
       }
     }
   }
-  wsum = lc_wave_sum(wsum);
   const float inv = wsum == 0.f ? 0.f : 1.0f / wsum;
   T* oh = out + (int64_t)b * o_sb + (int64_t)h * o_sh;
 #pragma unroll
   for (int e = 0; e < VPL; ++e)
-    if (d0 + e < a.D) oh[d0 + e] = lc_from_f32<T>(acc[e] * inv);
+    if (d0 + e < a.D) oh[d0 + e] = lc_from_f32<T>(rounded(acc[e] * inv));
   if (lse_out != nullptr && lane == 0)
     lse_out[(int64_t)b * a.Hq + h] = wsum == 0.f ? -INFINITY : (mx + lc_log2(wsum)) * kLn2;
 }
@@ -1127,9 +1253,24 @@ int launch_f32(const SharedArgs& a, hipStream_t st) {
 }
 
 template <typename T>
-int launch_shared(const SharedArgs& a, int wr, int own_waves, bool mfma, void* out, int64_t o_sb, int64_t o_sh,
-                  float* lse, hipStream_t st) {
+int launch_shared(SharedArgs a, int wr, int own_waves, bool mfma, int32_t* counters, void* out,
+                  int64_t o_sb, int64_t o_sh, float* lse, hipStream_t st) {
   const int splits = a.p_splits + a.s_splits;
+  // One launch where the grid is one round of workgroups and each joins little.
+  const int64_t rows = (int64_t)a.W * a.G, tiles = lc_cdiv(rows, 32 * wr);
+  const int64_t expected = tiles * a.p_splits + (int64_t)a.W * lc_cdiv(a.G, 32) * a.s_splits;
+  const int64_t units = (int64_t)(a.B / a.W) * a.Hkv;
+  const bool join = counters != nullptr && mfma && own_waves == 4 && splits > 0 &&
+                    splits <= kJoinRanges && rows * splits * a.D * 4 <= kJoinBytes &&
+                    units <= kJoinCounters && units * expected <= 2 * lc_cu_count();
+  if (join) {
+    a.counters = counters;
+    a.expected = static_cast<int>(expected);
+    a.out = out;
+    a.o_sb = o_sb;
+    a.o_sh = o_sh;
+    a.lse = lse;
+  }
   if (splits > 0 && mfma) {
     if constexpr (sizeof(T) == 2) {
       const int rc = a.D <= 64 ? launch_mfma<T, 64>(a, wr, own_waves, st)
@@ -1144,12 +1285,15 @@ int launch_shared(const SharedArgs& a, int wr, int own_waves, bool mfma, void* o
     const int rc = lc_check_launch("lc_shared_prefix_decode_fwd (generic)");
     if (rc != LC_OK) return rc;
   }
+  if (join) return LC_OK;
   return launch_merge<T>(a, out, o_sb, o_sh, lse, st);
 }
 
 }  // namespace
 
 extern "C" {
+
+int64_t lc_shared_prefix_decode_counter_count(void) { return kJoinCounters; }
 
 int64_t lc_shared_prefix_decode_workspace_bytes(int64_t B, int64_t groups, int64_t Hq, int64_t Hkv,
                                                 int64_t D, int64_t prefix_capacity,
@@ -1168,8 +1312,8 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
                                 const int32_t* prefix_lens, const int32_t* block_table,
                                 int64_t bt_stride, int64_t max_pages_per_seq,
                                 const int32_t* seq_lens, void* out, int64_t o_sb, int64_t o_sh,
-                                float* lse, void* workspace, int64_t workspace_bytes, int64_t B,
-                                int64_t groups, int64_t Hq, int64_t Hkv, int64_t D,
+                                float* lse, void* workspace, int64_t workspace_bytes,
+                                int32_t* counters, int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D,
                                 int64_t page_size, float scale, int dtype, void* stream) {
   static const char* who = "lc_shared_prefix_decode_fwd";
   LC_REQUIRE(B >= 0 && B < 65536, "%s: batch %lld out of range", who, (long long)B);
@@ -1205,6 +1349,7 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
     return lc_fail(LC_EWORKSPACE, "%s: workspace %lld < %lld bytes", who,
                    (long long)workspace_bytes, (long long)need);
   LC_REQUIRE(lc_aligned(workspace, 256), "%s: workspace not 256-byte aligned", who);
+  LC_REQUIRE(lc_aligned(counters, 4), "%s: counters not 4-byte aligned", who);
 
   SharedArgs a{};
   a.q = q;
@@ -1250,11 +1395,11 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
   hipStream_t st = lc_stream(stream);
   switch (dtype) {
     case LC_DTYPE_F32:
-      return launch_shared<float>(a, plan.wr, plan.own_waves, mfma, out, o_sb, o_sh, lse, st);
+      return launch_shared<float>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse, st);
     case LC_DTYPE_BF16:
-      return launch_shared<bf16_t>(a, plan.wr, plan.own_waves, mfma, out, o_sb, o_sh, lse, st);
+      return launch_shared<bf16_t>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse, st);
     default:
-      return launch_shared<f16_t>(a, plan.wr, plan.own_waves, mfma, out, o_sb, o_sh, lse, st);
+      return launch_shared<f16_t>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse, st);
   }
 }
 

@@ -153,9 +153,10 @@ _SIGNATURES = {
     "lc_shared_prefix_decode_fwd": (
         ctypes.c_int,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_i64,
-         _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64,
-         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_int, _c_p],
+         _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_p,
+         _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_int, _c_p],
     ),
+    "lc_shared_prefix_decode_counter_count": (_c_i64, []),
     "lc_beam_select_workspace_bytes": (_c_i64, [_c_i64] * 4),
     "lc_beam_select": (
         ctypes.c_int,

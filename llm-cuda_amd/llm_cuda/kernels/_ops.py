@@ -1364,6 +1364,24 @@ def shared_prefix_decode(q: torch.Tensor, key_pages: torch.Tensor, value_pages: 
                                  seq_lens, scale, return_lse)
 
 
+_JOIN_COUNTERS: dict = {}
+
+
+def _join_counters(kind: str, dev: torch.device, stream: int) -> int | None:
+    """Address of the zeroed tickets of the kernels that join their parts in one launch:
+    one buffer per kind, device and stream, whose calls follow one another and leave it
+    zeroed. None (two launches) while a graph is captured: its replays may run beside
+    each other and beside eager calls."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return None
+    key = (kind, dev.index, stream)
+    buf = _JOIN_COUNTERS.get(key)
+    if buf is None:
+        n = nat.size("lc_shared_prefix_decode_counter_count")
+        buf = _JOIN_COUNTERS[key] = torch.zeros(n, dtype=torch.int32, device=dev)
+    return buf.data_ptr()
+
+
 @functools.lru_cache(maxsize=1024)
 def _shared_prefix_sizes(q, k, v, prefix_table, prefix_lens, block_table, seq_lens, ks, vs, lc_dtype):
     """Checks the shapes of a shared_prefix_decode call; (batch, groups, heads, kv heads,
@@ -1433,14 +1451,17 @@ def _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, 
     lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if return_lse else None
     if B:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        stream = _stream(dev)
+        counters = _join_counters("shared_prefix", dev, stream)
         with _guard(dev):
             rc = nat.load().lc_shared_prefix_decode_fwd(
                 q.data_ptr(), qs[0], qs[1], key_pages.data_ptr(), value_pages.data_ptr(), ks[0],
                 ks[1], ks[2], num_pages, prefix_table.data_ptr(), max(pt_s[0], p_pages), p_pages,
                 prefix_lens.data_ptr(), block_table.data_ptr(), max(bt_s[0], s_pages), s_pages,
                 seq_lens.data_ptr(), out.data_ptr(), os[0], os[1],
-                None if lse is None else lse.data_ptr(), ws.data_ptr(), ws_bytes, B, N, Hq, Hkv,
-                D, P, 1.0 / math.sqrt(D) if scale is None else float(scale), dtype, _stream(dev))
+                None if lse is None else lse.data_ptr(), ws.data_ptr(), ws_bytes, counters, B, N,
+                Hq, Hkv, D, P, 1.0 / math.sqrt(D) if scale is None else float(scale), dtype,
+                stream)
         if rc:
             nat.check(rc, "lc_shared_prefix_decode_fwd")
     return (out, lse) if return_lse else out

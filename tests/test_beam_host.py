@@ -107,14 +107,14 @@ def test_arguments_rejected_before_launch():
     base = (buf.data_ptr() + 255) // 256 * 256
 
     def attend(B=4, N=2, Hq=4, Hkv=2, D=16, P=8, pages=6, ppages=1, pages_seq=1, ws=1 << 15, dtype=0,
-               pt_stride=1, wp=base):
+               pt_stride=1, wp=base, cnt=None):
         return lib.lc_shared_prefix_decode_fwd(
             base, 64, 16, base, base, 256, 128, 16, pages, base, pt_stride, ppages, base, base, 1,
-            pages_seq, base, base, 64, 16, None, wp, ws, B, N, Hq, Hkv, D, P, 0.25, dtype, None)
+            pages_seq, base, base, 64, 16, None, wp, ws, cnt, B, N, Hq, Hkv, D, P, 0.25, dtype, None)
 
     for bad in (dict(B=5), dict(N=0), dict(B=-1), dict(B=65536), dict(Hq=3), dict(D=0), dict(D=257),
                 dict(P=0), dict(pages=0), dict(ppages=-1), dict(pt_stride=0), dict(ws=8), dict(dtype=7),
-                dict(ppages=1 << 30, pt_stride=1 << 30), dict(wp=base + 4), dict(wp=None)):
+                dict(ppages=1 << 30, pt_stride=1 << 30), dict(wp=base + 4), dict(wp=None), dict(cnt=base + 2)):
         assert attend(**bad) < 0, bad
         assert b"lc_shared_prefix_decode_fwd" in lib.lc_last_error()
     assert attend(B=0, N=0) == 0 and attend(B=0) == 0

@@ -231,6 +231,48 @@ def test_captured_and_replayed(cuda, dtype):
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,W,plen,cap", [(128, 4, 300, 20), (64, 4, 9, 20), (32, 1, 70, 0), (128, 8, 900, 130),
+                                          (64, 5, 0, 3)])
+def test_one_launch_equals_two(cuda, monkeypatch, dtype, D, W, plen, cap):
+    """The join by the last workgroup and the merge launch give the same bits, and leave the
+    tickets at zero."""
+    from llm_cuda.kernels import _ops
+    from llm_cuda.kernels.triton.decode_attention import shared_prefix_decode_attention as op
+
+    for seed in range(6):
+        lens = [(7 * seed + 3 * i) % (cap + 1) for i in range(2 * W)]
+        args = [t.to(cuda) for t in make(2, W, 8, 2, D, 8, [plen, plen // 2], lens, dtype, seed=seed)]
+        one = op(*args, return_lse=True)
+        torch.cuda.synchronize()
+        stream = torch.cuda.current_stream().cuda_stream
+        assert not _ops._JOIN_COUNTERS[("shared_prefix", 0, stream)].any()
+        with monkeypatch.context() as m:
+            m.setattr(_ops, "_join_counters", lambda *key: None)
+            two = op(*args, return_lse=True)
+        assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+
+
+def test_two_streams_at_once(cuda):
+    """Calls on two streams in flight together, many of them, each with its own tickets."""
+    from llm_cuda.kernels.triton.decode_attention import shared_prefix_decode_attention as op
+
+    jobs = [[t.to(cuda) for t in make(2, 4, 8, 2, 64, 16, [300, 90], [3 * i for i in range(8)], BF16, seed=s)]
+            for s in range(2)]
+    want = [op(*j, return_lse=True) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(50):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(op(*jobs[i], return_lse=True))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, lse in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+
+
 def test_another_stream(cuda):
     args = make(1, 8, 8, 2, 64, 16, [300], [30] * 8, BF16)
     want, want_lse = run(args, cuda)
