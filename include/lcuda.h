@@ -548,14 +548,19 @@ LC_API int64_t lc_beam_select_workspace_bytes(int64_t groups, int64_t width, int
  * NaN, which rank above all others.
  * 1 <= width <= 256, 1 <= count <= min(64, width * vocab), width * vocab <
  * 2^31. workspace: 256-byte aligned; calls that may overlap need their own.
+ * counters: lc_beam_select_counter_count() int32 values that are zero at entry and
+ * are left zero, or NULL. With them a call of few rows joins its parts in the launch
+ * that computes them; without, or with more rows, a second launch does, with the
+ * same result. Calls that may overlap need their own.
  * No counterpart in the reference (models/llama3/model.py:200-218 decodes
  * greedily). */
+LC_API int64_t lc_beam_select_counter_count(void);
 LC_API int lc_beam_select(const void* logits, int64_t group_stride, int64_t beam_stride,
                           const float* scores, const uint8_t* finished, int64_t eos,
                           int64_t groups, int64_t width, int64_t vocab, int64_t count,
                           float* out_scores, int64_t* out_tokens, int64_t* out_parents,
                           uint8_t* out_finished, void* workspace, int64_t workspace_bytes,
-                          int dtype, void* stream);
+                          int32_t* counters, int dtype, void* stream);
 
 /* Reorders paged K/V caches after a selection: sequence w of group n (row n *
  * width + w of the table) continues what sequence parents[n, w] of the group

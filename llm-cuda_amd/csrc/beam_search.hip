@@ -36,6 +36,10 @@ constexpr int kMaxWidth = 256;     // beams per group: threads of a workgroup
 constexpr int kWaveCap = 256;      // gathered keys of a chunk's wave
 constexpr int kTieSlack = 8;       // lanes at the K-th value before ties are cut by index
 constexpr int kMergeCap = 4096;    // gathered candidates of a group
+constexpr int kMergeThreads = 1024;
+constexpr int kHeldCandidates = 2048;  // most that the merge holds before the sums are joined
+constexpr int kJoinCounters = 4096;
+constexpr int kJoinWidth = 8;  // most beams of a group that are joined in the same launch
 constexpr int kReachCap = 1024;    // lists of a group whose candidates are looked through
 
 // Order-preserving bits of a float (not NaN); -0 counts as +0.
@@ -125,6 +129,7 @@ struct SelectArgs {
   int64_t* out_tokens;
   int64_t* out_parents;
   uint8_t* out_finished;
+  int* counters;  // [N] tickets (beam_select_kernel)
   int W, V, K, chunks, eos;
 };
 
@@ -136,8 +141,341 @@ __device__ __forceinline__ Vec16<T> load16_any(const T* p) {
   return v;
 }
 
-template <typename T, int ITEMS>
-__global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) {
+// A chunk's part (key, sum or largest logit) for the join. Where a workgroup of the
+// same launch reads it, it goes through to memory by relaxed accesses of device scope.
+template <bool JOIN, typename P>
+__device__ __forceinline__ P part(const P* from) {
+  return JOIN ? __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *from;
+}
+template <bool JOIN, typename P, typename X>
+__device__ __forceinline__ void put_part(P* to, X from) {
+  const P x = from;
+  if (JOIN)
+    __hip_atomic_store(to, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  else
+    *to = x;
+}
+
+// One workgroup per group: the beams' lse, then the K best of their chunks' lists.
+// Beams without ordinary values stand for themselves: finished (the eos token at
+// their score, -inf elsewhere), empty (no finite logit, or a score of -inf: -inf
+// everywhere) and undefined (NaN or +inf in the logits or the score: NaN).
+enum : int { kBeamOrdinary = 0, kBeamFinished, kBeamEmpty, kBeamUndefined };
+
+// kMergeThreads threads, room for kMergeCap gathered candidates. JOIN: the chunks' parts
+// were written by other workgroups of this launch.
+template <int kMergeThreads, int kMergeCap, bool JOIN>
+__device__ __forceinline__ void beam_merge(const SelectArgs& a, int64_t n) {
+  constexpr int kMergeWaves = kMergeThreads / 64;
+  __shared__ double base[kMaxWidth];  // score - ln of the sum relative to `peak`
+  __shared__ float peak[kMaxWidth];   // the beam's largest logit
+  __shared__ int kind[kMaxWidth];
+  __shared__ uint64_t value[kMergeCap];
+  __shared__ uint32_t flat[kMergeCap];  // inverted w V + v
+  __shared__ int reach[kReachCap];      // lists whose best candidate reaches the bound
+  __shared__ uint64_t bound[kMergeWaves];
+  __shared__ uint64_t best_v[kMergeWaves];
+  __shared__ uint32_t best_f[kMergeWaves];
+  __shared__ int above[kMergeWaves];
+  __shared__ int count, reached;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int K = a.K, lists = a.W * a.chunks;
+  if (tid == 0) count = reached = 0;
+  // Few candidates: every thread's kHeld of them, the lists' first ones first, are
+  // loaded before the sums are joined; else only the lists that turn out to matter.
+  constexpr int kHeld = kHeldCandidates / kMergeThreads;
+  const bool few = lists * K <= kHeld * kMergeThreads;
+  uint64_t held[kHeld];
+  int held_l[kHeld], held_k[kHeld];
+  if (few) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+      const uint32_t i = tid + r * kMergeThreads;
+      held_k[r] = static_cast<int>(i / static_cast<uint32_t>(lists));
+      held_l[r] = static_cast<int>(i) - held_k[r] * lists;
+      held[r] = part<JOIN>(a.keys + (n * lists + held_l[r]) * K + min(held_k[r], K - 1));
+    }
+  }
+  for (int w = wave; w < a.W; w += kMergeWaves) {
+    const int64_t row = n * a.W + w;
+    const float score = a.scores[row];
+    float t0 = -INFINITY;
+    double s0 = 0;
+    if (lane < a.chunks) {  // (with the score: one round trip for up to 64 chunks)
+      t0 = part<JOIN>(a.tops + row * a.chunks + lane);
+      s0 = part<JOIN>(a.sums + row * a.chunks + lane);
+    }
+    if (a.finished != nullptr && a.finished[row]) {
+      if (lane == 0) {
+        kind[w] = kBeamFinished;
+        base[w] = score;
+      }
+      continue;
+    }
+    float top = t0;
+    for (int c = lane + 64; c < a.chunks; c += 64) top = fmaxf(top, part<JOIN>(a.tops + row * a.chunks + c));
+    top = lc_wave_max(top);
+    auto weighed = [&](float t, double s) {
+      return t == -INFINITY ? s : s * exp(static_cast<double>(t) - top);
+    };
+    double sum = weighed(t0, s0);
+    for (int c = lane + 64; c < a.chunks; c += 64)
+      sum += weighed(part<JOIN>(a.tops + row * a.chunks + c), part<JOIN>(a.sums + row * a.chunks + c));
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) {
+      const bool empty = sum == 0 || score == -INFINITY;
+      kind[w] = sum != sum || !(score < INFINITY) ? kBeamUndefined
+                : empty                           ? kBeamEmpty
+                                                  : kBeamOrdinary;
+      // (the largest logit is taken off the logits, not added to the score: beside a
+      // row of a type's lowest value neither the score nor the log would count)
+      base[w] = score - log(sum);
+      peak[w] = top;
+    }
+  }
+  __syncthreads();
+
+  // Candidate k of list l = w * chunks + c, whose key is e: its value and inverted
+  // flat index; a value of 0 (below every number): none.
+  auto candidate_of = [&](int l, int k, uint64_t e, uint64_t& v, uint32_t& f) {
+    const int w = static_cast<int>(static_cast<uint32_t>(l) / static_cast<uint32_t>(a.chunks));
+    v = 0;
+    f = 0;
+    const int kd = kind[w];
+    uint32_t token = static_cast<uint32_t>(k);
+    if (kd == kBeamOrdinary) {
+      token = ~static_cast<uint32_t>(e);
+      if (token >= static_cast<uint32_t>(a.V)) return;
+      const float x = from_ordered(static_cast<uint32_t>(e >> 32));
+      v = ordered64(base[w] + (static_cast<double>(x) - peak[w]));
+    } else {
+      if (l != w * a.chunks) return;
+      if (kd == kBeamFinished) {
+        // eos first, then the lowest tokens
+        if (k == 0)
+          token = static_cast<uint32_t>(a.eos);
+        else
+          token = static_cast<uint32_t>(k - 1 < a.eos ? k - 1 : k);
+      }
+      if (token >= static_cast<uint32_t>(a.V)) return;
+      v = ordered64(kd == kBeamUndefined               ? static_cast<double>(NAN)
+                    : kd == kBeamFinished && k == 0 ? base[w]
+                                                    : -static_cast<double>(INFINITY));
+    }
+    f = ~(static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V) + token);
+  };
+
+  auto candidate = [&](int l, int k, uint64_t& v, uint32_t& f) {
+    candidate_of(l, k, part<JOIN>(a.keys + (n * lists + l) * K + k), v, f);
+  };
+
+  // Candidates below `limit` are out. A candidate's key is the upper half of its value
+  // and, for -inf alone (where equal halves are equal values), its inverted index.
+  const uint32_t none_hi = static_cast<uint32_t>(ordered64(-static_cast<double>(INFINITY)) >> 32);
+  auto key_of = [&](uint64_t v, uint32_t f) -> uint64_t {
+    const uint32_t hi = static_cast<uint32_t>(v >> 32);
+    return (static_cast<uint64_t>(hi) << 32) | (hi == none_hi ? f : 0);
+  };
+  uint64_t limit = 1;
+  auto add = [&](uint64_t v, uint32_t f) {  // (whole waves)
+    const bool hit = v != 0 && key_of(v, f) >= limit;
+    const unsigned long long hits = __ballot(hit);
+    if (hits == 0) return;
+    int first = 0;
+    if (lane == 0) first = atomicAdd(&count, __popcll(hits));
+    const int pos = __builtin_amdgcn_readfirstlane(first) + __popcll(hits & ((1ull << lane) - 1));
+    if (hit && pos < kMergeCap) {
+      value[pos] = v;
+      flat[pos] = f;
+    }
+  };
+  // Raises the limit to the least of the waves' q-th best gathered candidates, q = K /
+  // kMergeWaves rounded up (so K reach it), and drops what is below.
+  constexpr int kEach = kMergeCap / kMergeThreads;
+  auto prune = [&](int m) {
+    uint64_t v[kEach];
+    uint32_t f[kEach];
+    uint64_t best = 0;
+#pragma unroll
+    for (int r = 0; r < kEach; ++r) {
+      const int i = r * kMergeThreads + lane * kMergeWaves + wave;
+      v[r] = i < m ? value[i] : 0;
+      f[r] = i < m ? flat[i] : 0;
+      if (i < m) best = max(best, key_of(v[r], f[r]));
+    }
+    const int q = (K + kMergeWaves - 1) / kMergeWaves;
+    const uint32_t hi = static_cast<uint32_t>(best >> 32), lo = static_cast<uint32_t>(best);
+    const uint32_t t = wave_kth_largest<31, 0>(hi, q);
+    uint32_t cut = 0;
+    if (__builtin_expect(t == none_hi, 0)) {
+      const int more = q - __popcll(__ballot(hi > t));
+      cut = wave_kth_largest<31, 0>(hi == t ? lo : 0, more);
+    }
+    if (lane == 0) bound[wave] = (static_cast<uint64_t>(t) << 32) | cut;
+    __syncthreads();
+    uint64_t least = bound[0];
+#pragma unroll
+    for (int w = 1; w < kMergeWaves; ++w) least = min(least, bound[w]);
+    limit = max(limit, least);
+    if (tid == 0) count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kEach; ++r) add(v[r], f[r]);
+    __syncthreads();
+  };
+  // The K-th best of a wave's lanes, each with its best value (a list's first, where
+  // there are many), is a lower bound of the K-th largest value; so is the lowest above
+  // -inf where K are above it (one live beam: the others' -inf fill the waves).
+  uint64_t head = 0, held_v[kHeld];
+  uint32_t held_f[kHeld];
+  int n_above = 0;
+  if (few) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) {
+      held_v[r] = 0;
+      held_f[r] = 0;
+      if (held_k[r] < K) candidate_of(held_l[r], held_k[r], held[r], held_v[r], held_f[r]);
+      head = max(head, held_v[r]);
+      n_above += __popcll(__ballot(static_cast<uint32_t>(held_v[r] >> 32) > none_hi));
+    }
+  } else {
+    for (int l = tid; l < lists; l += kMergeThreads) {
+      uint64_t v;
+      uint32_t f;
+      candidate(l, 0, v, f);
+      head = max(head, v);
+    }
+  }
+  const uint32_t t = wave_kth_largest<31, 0>(static_cast<uint32_t>(head >> 32), K);
+  if (lane == 0) {
+    bound[wave] = static_cast<uint64_t>(t) << 32;
+    above[wave] = n_above;
+  }
+  __syncthreads();
+  n_above = 0;
+#pragma unroll
+  for (int w = 0; w < kMergeWaves; ++w) {
+    limit = max(limit, bound[w]);
+    n_above += above[w];
+  }
+  if (n_above >= K) limit = max(limit, (static_cast<uint64_t>(none_hi) + 1) << 32);
+  bool fits = true;
+  if (few) {
+#pragma unroll
+    for (int r = 0; r < kHeld; ++r) add(held_v[r], held_f[r]);
+    __syncthreads();
+  } else {
+    for (int l = tid; l < lists; l += kMergeThreads) {
+      uint64_t v = head;
+      uint32_t f;
+      if (lists > kMergeThreads) candidate(l, 0, v, f);
+      if (v != 0 && static_cast<uint32_t>(v >> 32) >= static_cast<uint32_t>(limit >> 32)) {
+        const int pos = atomicAdd(&reached, 1);
+        if (pos < kReachCap) reach[pos] = l;
+      }
+    }
+    __syncthreads();
+    // A wave takes one of these lists (of all, where they are too many), a lane one of
+    // its candidates; room for the next lists' is made after every two.
+    const bool listed = reached <= kReachCap;
+    const int n_lists = listed ? reached : lists;
+    constexpr int kRounds = kMergeCap / 2 / (kMergeWaves * kMaxCount);
+    for (int i0 = 0; i0 < n_lists; i0 += kRounds * kMergeWaves) {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const int i = i0 + r * kMergeWaves + wave;
+        uint64_t v = 0;
+        uint32_t f = 0;
+        if (i < n_lists && lane < K) candidate(listed ? reach[i] : i, lane, v, f);
+        add(v, f);
+      }
+      __syncthreads();
+      int m = count;
+      __syncthreads();
+      if (__builtin_expect(m > kMergeCap / 2, 0)) {
+        prune(m);
+        m = count;
+        __syncthreads();
+      }
+      fits = fits && m <= kMergeCap / 2;
+    }
+    __syncthreads();
+  }
+  for (int i = 0; i < 2 && __builtin_expect(fits && count > 2 * K + 64, 0); ++i) prune(count);
+  const int m = count;
+  auto store = [&](int rank, uint64_t v, uint32_t f) {
+    const uint32_t at = ~f;
+    const int w = static_cast<int>(at / static_cast<uint32_t>(a.V));
+    const int token = static_cast<int>(at - static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V));
+    const int64_t o = n * K + rank;
+    a.out_scores[o] = static_cast<float>(from_ordered64(v));
+    a.out_tokens[o] = token;
+    a.out_parents[o] = w;
+    if (a.out_finished != nullptr)
+      a.out_finished[o] = token == a.eos || (a.finished != nullptr && a.finished[n * a.W + w]);
+  };
+  if (__builtin_expect(fits, 1)) {
+    // Eight threads count the candidates above each one.
+    const int eighth = tid & 7;
+    for (int i = tid >> 3; i < (m + 7) / 8 * 8; i += kMergeThreads / 8) {
+      const uint64_t v = i < m ? value[i] : 0;
+      const uint32_t f = i < m ? flat[i] : 0;
+      int rank = 0;
+#pragma unroll 4
+      for (int j = eighth; j < m; j += 8) rank += value[j] > v || (value[j] == v && flat[j] > f);
+      rank += __shfl_xor(rank, 1, 64);
+      rank += __shfl_xor(rank, 2, 64);
+      rank += __shfl_xor(rank, 4, 64);
+      if (eighth == 0 && i < m && rank < K) store(rank, v, f);
+    }
+  } else {
+    uint64_t last_v = ~0ull;
+    uint32_t last_f = ~0u;
+    for (int r = 0; r < K; ++r) {
+      uint64_t bv = 0;
+      uint32_t bf = 0;
+      auto take = [&](uint64_t v, uint32_t f) {
+        if (v > bv || (v == bv && f > bf)) {
+          bv = v;
+          bf = f;
+        }
+      };
+      for (int i = tid; i < lists * K; i += kMergeThreads) {
+        uint64_t v;
+        uint32_t f;
+        const int l = i / K;
+        candidate(l, i - l * K, v, f);
+        if (r == 0 || v < last_v || (v == last_v && f < last_f)) take(v, f);
+      }
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) {
+        const uint64_t ov = __shfl_xor(static_cast<unsigned long long>(bv), o, 64);
+        const uint32_t of = __shfl_xor(bf, o, 64);
+        take(ov, of);
+      }
+      __syncthreads();
+      if (lane == 0) {
+        best_v[wave] = bv;
+        best_f[wave] = bf;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kMergeWaves; ++w) take(best_v[w], best_f[w]);
+      if (tid == 0) store(r, bv, bf);
+      last_v = bv;
+      last_f = bf;
+    }
+  }
+}
+
+__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
+  beam_merge<kMergeThreads, kMergeCap, false>(a, blockIdx.x);
+}
+
+template <typename T, int ITEMS, bool JOIN>
+__device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
   constexpr int VEC = 16 / sizeof(T);
   constexpr int CHUNK = kBeamThreads * ITEMS;
   static_assert(ITEMS % VEC == 0, "whole vectors per thread");
@@ -293,8 +631,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
   uint64_t* out = a.keys + (row * a.chunks + chunk) * a.K;
   // (stored with the index in the row, not in the chunk)
   auto store = [&](int rank, uint64_t k) {
-    out[rank] = (k & 0xffffffff00000000ull) |
-                static_cast<uint32_t>(~(~static_cast<uint32_t>(k) + static_cast<uint32_t>(c0)));
+    const uint32_t at = ~(~static_cast<uint32_t>(k) + static_cast<uint32_t>(c0));
+    put_part<JOIN>(out + rank, (k & 0xffffffff00000000ull) | at);
   };
   if (__builtin_expect(most <= kWaveCap, 1)) {
     // Four threads count the keys above each one, a wave's part of the list each.
@@ -347,310 +685,40 @@ __global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) 
     for (int w = 0; w < kBeamWaves; ++w)
       s += w_top[w] == -INFINITY ? static_cast<double>(w_sum[w])
                                  : w_sum[w] * exp(static_cast<double>(w_top[w]) - hi);
-    a.sums[row * a.chunks + chunk] = s;
-    a.tops[row * a.chunks + chunk] = hi;
+    put_part<JOIN>(a.sums + row * a.chunks + chunk, s);
+    put_part<JOIN>(a.tops + row * a.chunks + chunk, hi);
   }
 }
 
-// One workgroup per group: the beams' lse, then the K best of their chunks' lists.
-// Beams without ordinary values stand for themselves: finished (the eos token at
-// their score, -inf elsewhere), empty (no finite logit, or a score of -inf: -inf
-// everywhere) and undefined (NaN or +inf in the logits or the score: NaN).
-enum : int { kBeamOrdinary = 0, kBeamFinished, kBeamEmpty, kBeamUndefined };
+template <typename T, int ITEMS>
+__global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) {
+  beam_chunk<T, ITEMS, false>(a);
+}
 
-constexpr int kMergeThreads = 1024;
-constexpr int kMergeWaves = kMergeThreads / 64;
-
-__global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(SelectArgs a) {
-  __shared__ double base[kMaxWidth];  // score - ln of the sum relative to `peak`
-  __shared__ float peak[kMaxWidth];   // the beam's largest logit
-  __shared__ int kind[kMaxWidth];
-  __shared__ uint64_t value[kMergeCap];
-  __shared__ uint32_t flat[kMergeCap];  // inverted w V + v
-  __shared__ int reach[kReachCap];      // lists whose best candidate reaches the bound
-  __shared__ uint64_t bound[kMergeWaves];
-  __shared__ uint64_t best_v[kMergeWaves];
-  __shared__ uint32_t best_f[kMergeWaves];
-  __shared__ int count, reached;
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t n = blockIdx.x;
-  const int K = a.K, lists = a.W * a.chunks;
-  if (tid == 0) count = reached = 0;
-  // Few candidates: every thread's kHeld of them, the lists' first ones first, are
-  // loaded before the sums are joined; else only the lists that turn out to matter.
-  constexpr int kHeld = 2;
-  const bool few = lists * K <= kHeld * kMergeThreads;
-  uint64_t held[kHeld];
-  int held_l[kHeld], held_k[kHeld];
-  if (few) {
-#pragma unroll
-    for (int r = 0; r < kHeld; ++r) {
-      const uint32_t i = tid + r * kMergeThreads;
-      held_k[r] = static_cast<int>(i / static_cast<uint32_t>(lists));
-      held_l[r] = static_cast<int>(i) - held_k[r] * lists;
-      held[r] = a.keys[(n * lists + held_l[r]) * K + min(held_k[r], K - 1)];
-    }
-  }
-  for (int w = wave; w < a.W; w += kMergeWaves) {
-    const int64_t row = n * a.W + w;
-    const float score = a.scores[row];
-    float t0 = -INFINITY;
-    double s0 = 0;
-    if (lane < a.chunks) {  // (with the score: one round trip for up to 64 chunks)
-      t0 = a.tops[row * a.chunks + lane];
-      s0 = a.sums[row * a.chunks + lane];
-    }
-    if (a.finished != nullptr && a.finished[row]) {
-      if (lane == 0) {
-        kind[w] = kBeamFinished;
-        base[w] = score;
-      }
-      continue;
-    }
-    float top = t0;
-    for (int c = lane + 64; c < a.chunks; c += 64) top = fmaxf(top, a.tops[row * a.chunks + c]);
-    top = lc_wave_max(top);
-    auto weighed = [&](float t, double s) {
-      return t == -INFINITY ? s : s * exp(static_cast<double>(t) - top);
-    };
-    double sum = weighed(t0, s0);
-    for (int c = lane + 64; c < a.chunks; c += 64)
-      sum += weighed(a.tops[row * a.chunks + c], a.sums[row * a.chunks + c]);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) {
-      const bool empty = sum == 0 || score == -INFINITY;
-      kind[w] = sum != sum || !(score < INFINITY) ? kBeamUndefined
-                : empty                           ? kBeamEmpty
-                                                  : kBeamOrdinary;
-      // (the largest logit is taken off the logits, not added to the score: beside a
-      // row of a type's lowest value neither the score nor the log would count)
-      base[w] = score - log(sum);
-      peak[w] = top;
-    }
+// Few beams and candidates: the workgroup of a group that finishes last (its ticket on
+// counters[n], zero at entry and left zero) joins the chunks, in the same launch. The
+// GPU takes as long as in two (4 beams of 32000: 10.9 us for 5.2 + 6.3; 8 of 32000:
+// 14.2 for 5.9 + 6.8; 16 of 1003, beyond the rule: 16.8 for 6.3 + 7.6), and the host,
+// which such a call waits for, a launch less: 17.2 -> 15.4 us a call.
+template <typename T>
+__global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(SelectArgs a) {
+  __shared__ int last;
+  beam_chunk<T, 8, true>(a);
+  const int64_t n = blockIdx.x / (a.W * a.chunks);
+  // (every wave's stores have reached memory before the ticket is taken)
+  __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+  lc_compiler_fence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int t =
+        __hip_atomic_fetch_add(a.counters + n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    last = t == a.W * a.chunks - 1;
+    if (last) __hip_atomic_store(a.counters + n, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-
-  // Candidate k of list l = w * chunks + c, whose key is e: its value and inverted
-  // flat index; a value of 0 (below every number): none.
-  auto candidate_of = [&](int l, int k, uint64_t e, uint64_t& v, uint32_t& f) {
-    const int w = static_cast<int>(static_cast<uint32_t>(l) / static_cast<uint32_t>(a.chunks));
-    v = 0;
-    f = 0;
-    const int kd = kind[w];
-    uint32_t token = static_cast<uint32_t>(k);
-    if (kd == kBeamOrdinary) {
-      token = ~static_cast<uint32_t>(e);
-      if (token >= static_cast<uint32_t>(a.V)) return;
-      const float x = from_ordered(static_cast<uint32_t>(e >> 32));
-      v = ordered64(base[w] + (static_cast<double>(x) - peak[w]));
-    } else {
-      if (l != w * a.chunks) return;
-      if (kd == kBeamFinished) {
-        // eos first, then the lowest tokens
-        if (k == 0)
-          token = static_cast<uint32_t>(a.eos);
-        else
-          token = static_cast<uint32_t>(k - 1 < a.eos ? k - 1 : k);
-      }
-      if (token >= static_cast<uint32_t>(a.V)) return;
-      v = ordered64(kd == kBeamUndefined               ? static_cast<double>(NAN)
-                    : kd == kBeamFinished && k == 0 ? base[w]
-                                                    : -static_cast<double>(INFINITY));
-    }
-    f = ~(static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V) + token);
-  };
-
-  auto candidate = [&](int l, int k, uint64_t& v, uint32_t& f) {
-    candidate_of(l, k, a.keys[(n * lists + l) * K + k], v, f);
-  };
-
-  // Candidates below `limit` are out. A candidate's key is the upper half of its value
-  // and, for -inf alone (where equal halves are equal values), its inverted index.
-  const uint32_t none_hi = static_cast<uint32_t>(ordered64(-static_cast<double>(INFINITY)) >> 32);
-  auto key_of = [&](uint64_t v, uint32_t f) -> uint64_t {
-    const uint32_t hi = static_cast<uint32_t>(v >> 32);
-    return (static_cast<uint64_t>(hi) << 32) | (hi == none_hi ? f : 0);
-  };
-  uint64_t limit = 1;
-  auto add = [&](uint64_t v, uint32_t f) {  // (whole waves)
-    const bool hit = v != 0 && key_of(v, f) >= limit;
-    const unsigned long long hits = __ballot(hit);
-    if (hits == 0) return;
-    int first = 0;
-    if (lane == 0) first = atomicAdd(&count, __popcll(hits));
-    const int pos = __builtin_amdgcn_readfirstlane(first) + __popcll(hits & ((1ull << lane) - 1));
-    if (hit && pos < kMergeCap) {
-      value[pos] = v;
-      flat[pos] = f;
-    }
-  };
-  // Raises the limit to the least of the waves' q-th best gathered candidates, q = K /
-  // 16 rounded up (so K reach it), and drops what is below.
-  constexpr int kEach = kMergeCap / kMergeThreads;
-  auto prune = [&](int m) {
-    uint64_t v[kEach];
-    uint32_t f[kEach];
-    uint64_t best = 0;
-#pragma unroll
-    for (int r = 0; r < kEach; ++r) {
-      const int i = r * kMergeThreads + lane * kMergeWaves + wave;
-      v[r] = i < m ? value[i] : 0;
-      f[r] = i < m ? flat[i] : 0;
-      if (i < m) best = max(best, key_of(v[r], f[r]));
-    }
-    const int q = (K + kMergeWaves - 1) / kMergeWaves;
-    const uint32_t hi = static_cast<uint32_t>(best >> 32), lo = static_cast<uint32_t>(best);
-    const uint32_t t = wave_kth_largest<31, 0>(hi, q);
-    uint32_t cut = 0;
-    if (__builtin_expect(t == none_hi, 0)) {
-      const int more = q - __popcll(__ballot(hi > t));
-      cut = wave_kth_largest<31, 0>(hi == t ? lo : 0, more);
-    }
-    if (lane == 0) bound[wave] = (static_cast<uint64_t>(t) << 32) | cut;
-    __syncthreads();
-    uint64_t least = bound[0];
-#pragma unroll
-    for (int w = 1; w < kMergeWaves; ++w) least = min(least, bound[w]);
-    limit = max(limit, least);
-    if (tid == 0) count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kEach; ++r) add(v[r], f[r]);
-    __syncthreads();
-  };
-  // Each wave's K-th best list head is a lower bound of the K-th largest value.
-  uint64_t head = 0, held_v[kHeld];
-  uint32_t held_f[kHeld];
-  if (few) {
-#pragma unroll
-    for (int r = 0; r < kHeld; ++r) {
-      held_v[r] = 0;
-      held_f[r] = 0;
-      if (held_k[r] < K) candidate_of(held_l[r], held_k[r], held[r], held_v[r], held_f[r]);
-      if (held_k[r] == 0) head = max(head, held_v[r]);
-    }
-  } else {
-    for (int l = tid; l < lists; l += kMergeThreads) {
-      uint64_t v;
-      uint32_t f;
-      candidate(l, 0, v, f);
-      head = max(head, v);
-    }
-  }
-  const uint32_t t = wave_kth_largest<31, 0>(static_cast<uint32_t>(head >> 32), K);
-  if (lane == 0) bound[wave] = static_cast<uint64_t>(t) << 32;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kMergeWaves; ++w) limit = max(limit, bound[w]);
-  bool fits = true;
-  if (few) {
-#pragma unroll
-    for (int r = 0; r < kHeld; ++r) add(held_v[r], held_f[r]);
-    __syncthreads();
-  } else {
-    for (int l = tid; l < lists; l += kMergeThreads) {
-      uint64_t v = head;
-      uint32_t f;
-      if (lists > kMergeThreads) candidate(l, 0, v, f);
-      if (v != 0 && static_cast<uint32_t>(v >> 32) >= static_cast<uint32_t>(limit >> 32)) {
-        const int pos = atomicAdd(&reached, 1);
-        if (pos < kReachCap) reach[pos] = l;
-      }
-    }
-    __syncthreads();
-    // A wave takes one of these lists (of all, where they are too many), a lane one of
-    // its candidates; room for the next lists' is made after every two.
-    const bool listed = reached <= kReachCap;
-    const int n_lists = listed ? reached : lists;
-    constexpr int kRounds = kMergeCap / 2 / (kMergeWaves * kMaxCount);
-    for (int i0 = 0; i0 < n_lists; i0 += kRounds * kMergeWaves) {
-#pragma unroll
-      for (int r = 0; r < kRounds; ++r) {
-        const int i = i0 + r * kMergeWaves + wave;
-        uint64_t v = 0;
-        uint32_t f = 0;
-        if (i < n_lists && lane < K) candidate(listed ? reach[i] : i, lane, v, f);
-        add(v, f);
-      }
-      __syncthreads();
-      int m = count;
-      __syncthreads();
-      if (__builtin_expect(m > kMergeCap / 2, 0)) {
-        prune(m);
-        m = count;
-        __syncthreads();
-      }
-      fits = fits && m <= kMergeCap / 2;
-    }
-    __syncthreads();
-  }
-  for (int i = 0; i < 2 && __builtin_expect(fits && count > 2 * K + 64, 0); ++i) prune(count);
-  const int m = count;
-  auto store = [&](int rank, uint64_t v, uint32_t f) {
-    const uint32_t at = ~f;
-    const int w = static_cast<int>(at / static_cast<uint32_t>(a.V));
-    const int token = static_cast<int>(at - static_cast<uint32_t>(w) * static_cast<uint32_t>(a.V));
-    const int64_t o = n * K + rank;
-    a.out_scores[o] = static_cast<float>(from_ordered64(v));
-    a.out_tokens[o] = token;
-    a.out_parents[o] = w;
-    if (a.out_finished != nullptr)
-      a.out_finished[o] = token == a.eos || (a.finished != nullptr && a.finished[n * a.W + w]);
-  };
-  if (__builtin_expect(fits, 1)) {
-    // Eight threads count the candidates above each one.
-    const int part = tid & 7;
-    for (int i = tid >> 3; i < (m + 7) / 8 * 8; i += kMergeThreads / 8) {
-      const uint64_t v = i < m ? value[i] : 0;
-      const uint32_t f = i < m ? flat[i] : 0;
-      int rank = 0;
-#pragma unroll 4
-      for (int j = part; j < m; j += 8) rank += value[j] > v || (value[j] == v && flat[j] > f);
-      rank += __shfl_xor(rank, 1, 64);
-      rank += __shfl_xor(rank, 2, 64);
-      rank += __shfl_xor(rank, 4, 64);
-      if (part == 0 && i < m && rank < K) store(rank, v, f);
-    }
-  } else {
-    uint64_t last_v = ~0ull;
-    uint32_t last_f = ~0u;
-    for (int r = 0; r < K; ++r) {
-      uint64_t bv = 0;
-      uint32_t bf = 0;
-      auto take = [&](uint64_t v, uint32_t f) {
-        if (v > bv || (v == bv && f > bf)) {
-          bv = v;
-          bf = f;
-        }
-      };
-      for (int i = tid; i < lists * K; i += kMergeThreads) {
-        uint64_t v;
-        uint32_t f;
-        const int l = i / K;
-        candidate(l, i - l * K, v, f);
-        if (r == 0 || v < last_v || (v == last_v && f < last_f)) take(v, f);
-      }
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) {
-        const uint64_t ov = __shfl_xor(static_cast<unsigned long long>(bv), o, 64);
-        const uint32_t of = __shfl_xor(bf, o, 64);
-        take(ov, of);
-      }
-      __syncthreads();
-      if (lane == 0) {
-        best_v[wave] = bv;
-        best_f[wave] = bf;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kMergeWaves; ++w) take(best_v[w], best_f[w]);
-      if (tid == 0) store(r, bv, bf);
-      last_v = bv;
-      last_f = bf;
-    }
-  }
+  if (!last) return;
+  lc_compiler_fence();
+  beam_merge<kBeamThreads, kHeldCandidates, true>(a, n);
 }
 
 // Logits of a row per workgroup: 8192 where that gives every CU a workgroup, else
@@ -667,6 +735,12 @@ template <typename T>
 int launch_select(SelectArgs a, int64_t groups, hipStream_t st) {
   const int64_t rows = groups * a.W;
   const unsigned blocks = static_cast<unsigned>(rows * a.chunks);
+  // One launch where the join is small, since its workgroup has 256 threads.
+  if (a.counters != nullptr && beam_items(rows, a.V) == 8 && groups <= kJoinCounters &&
+      a.W <= kJoinWidth && (int64_t)a.W * a.chunks * a.K <= kHeldCandidates) {
+    beam_select_kernel<T><<<blocks, kBeamThreads, 0, st>>>(a);
+    return lc_check_launch("lc_beam_select");
+  }
   if (beam_items(rows, a.V) == 32)
     beam_chunk_kernel<T, 32><<<blocks, kBeamThreads, 0, st>>>(a);
   else
@@ -800,6 +874,8 @@ __global__ __launch_bounds__(256) void kv_reorder_kernel(ReorderArgs a, int elem
 
 extern "C" {
 
+int64_t lc_beam_select_counter_count(void) { return kJoinCounters; }
+
 int64_t lc_beam_select_workspace_bytes(int64_t groups, int64_t width, int64_t vocab,
                                        int64_t count) {
   if (groups < 0 || width <= 0 || vocab <= 0 || count <= 0) return -1;
@@ -811,7 +887,8 @@ int lc_beam_select(const void* logits, int64_t group_stride, int64_t beam_stride
                    const float* scores, const uint8_t* finished, int64_t eos, int64_t groups,
                    int64_t width, int64_t vocab, int64_t count, float* out_scores,
                    int64_t* out_tokens, int64_t* out_parents, uint8_t* out_finished,
-                   void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+                   void* workspace, int64_t workspace_bytes, int32_t* counters, int dtype,
+                   void* stream) {
   static const char* who = "lc_beam_select";
   LC_REQUIRE(groups >= 0 && groups < (1LL << 31), "%s: %lld groups", who, (long long)groups);
   LC_REQUIRE(width > 0 && width <= kMaxWidth, "%s: width %lld not in [1, %d]", who,
@@ -836,8 +913,10 @@ int lc_beam_select(const void* logits, int64_t group_stride, int64_t beam_stride
     return lc_fail(LC_EWORKSPACE, "%s: workspace %lld < %lld bytes", who,
                    (long long)workspace_bytes, (long long)need);
   LC_REQUIRE(lc_aligned(workspace, 256), "%s: workspace not 256-byte aligned", who);
+  LC_REQUIRE(lc_aligned(counters, 4), "%s: counters not 4-byte aligned", who);
 
   SelectArgs a{};
+  a.counters = counters;
   a.logits = logits;
   a.s_group = group_stride;
   a.s_beam = beam_stride;

@@ -778,11 +778,16 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
 // The merge in the same launch, for few rows and ranges: every workgroup of group n
 // and kv head kvh takes a ticket after its partials, and the one with the last joins
 // all ranges of their rows, a thread per 4 columns. Which workgroup that is changes
-// nothing in the sums, which equal shared_merge_kernel's bit for bit. It saves the second launch (2.9 us of the host, 3.8 us of
-// the GPU at 4 beams of 1000 tokens); with many rows one workgroup would be slower
-// at it than the launch.
-constexpr int kJoinRanges = 16;          // most ranges per row
-constexpr int64_t kJoinBytes = 160 << 10;  // most partials of a group and kv head
+// nothing in the sums, which equal shared_merge_kernel's bit for bit.
+//
+// The GPU takes longer so (4 beams of 1000 tokens: 12.8 us for 6.9 + 3.8 in two
+// launches; 20 with fences, which write the whole L2 back, in place of write-through
+// partials), but the host, which such a call waits for, loses a launch: 17.4 -> 14.9
+// us a call. Where K and V are more than kJoinRead bytes the GPU is what counts (4
+// groups of 8 x 4224 tokens, 69 MB: 22.2 us in two launches, 29.2 in one).
+constexpr int kJoinRanges = 16;             // most ranges per row
+constexpr int64_t kJoinBytes = 96 << 10;    // most partials of a group and kv head
+constexpr int64_t kJoinRead = 16 << 20;     // most bytes of K and V, by the tables' widths
 constexpr int kJoinCounters = 4096;
 
 template <typename T>
@@ -1256,13 +1261,16 @@ template <typename T>
 int launch_shared(SharedArgs a, int wr, int own_waves, bool mfma, int32_t* counters, void* out,
                   int64_t o_sb, int64_t o_sh, float* lse, hipStream_t st) {
   const int splits = a.p_splits + a.s_splits;
-  // One launch where the grid is one round of workgroups and each joins little.
+  // One launch where the grid is one round of workgroups, which read little, and each
+  // joins little.
   const int64_t rows = (int64_t)a.W * a.G, tiles = lc_cdiv(rows, 32 * wr);
   const int64_t expected = tiles * a.p_splits + (int64_t)a.W * lc_cdiv(a.G, 32) * a.s_splits;
   const int64_t units = (int64_t)(a.B / a.W) * a.Hkv;
   const bool join = counters != nullptr && mfma && own_waves == 4 && splits > 0 &&
                     splits <= kJoinRanges && rows * splits * a.D * 4 <= kJoinBytes &&
-                    units <= kJoinCounters && units * expected <= 2 * lc_cu_count();
+                    units <= kJoinCounters && units * expected <= 2 * lc_cu_count() &&
+                    units * ((int64_t)a.p_pages + (int64_t)a.W * a.s_pages) * a.P * a.D * 2 *
+                            (int64_t)sizeof(T) <= kJoinRead;
   if (join) {
     a.counters = counters;
     a.expected = static_cast<int>(expected);

@@ -161,8 +161,9 @@ _SIGNATURES = {
     "lc_beam_select": (
         ctypes.c_int,
         [_c_p, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_p,
-         _c_p, _c_p, _c_p, _c_i64, ctypes.c_int, _c_p],
+         _c_p, _c_p, _c_p, _c_i64, _c_p, ctypes.c_int, _c_p],
     ),
+    "lc_beam_select_counter_count": (_c_i64, []),
     "lc_paged_kv_reorder": (
         ctypes.c_int,
         [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64,

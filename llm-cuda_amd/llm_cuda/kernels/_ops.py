@@ -1377,7 +1377,8 @@ def _join_counters(kind: str, dev: torch.device, stream: int) -> int | None:
     key = (kind, dev.index, stream)
     buf = _JOIN_COUNTERS.get(key)
     if buf is None:
-        n = nat.size("lc_shared_prefix_decode_counter_count")
+        n = max(nat.size("lc_shared_prefix_decode_counter_count"),
+                nat.size("lc_beam_select_counter_count"))
         buf = _JOIN_COUNTERS[key] = torch.zeros(n, dtype=torch.int32, device=dev)
     return buf.data_ptr()
 
@@ -1425,8 +1426,13 @@ def _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, 
     B, N, Hq, Hkv, D, P, num_pages, p_pages, s_pages, ws_bytes, strides_ok = _shared_prefix_sizes(
         q.shape, key_pages.shape, value_pages.shape, prefix_table.shape, prefix_lens.shape,
         block_table.shape, seq_lens.shape, ks, value_pages.stride(), dtype)
-    dev = nat.require_device(q, key_pages, value_pages, prefix_table, prefix_lens, block_table,
-                             seq_lens)
+    i = q.get_device()
+    if not (i >= 0 and key_pages.get_device() == i and value_pages.get_device() == i
+            and prefix_table.get_device() == i and prefix_lens.get_device() == i
+            and block_table.get_device() == i and seq_lens.get_device() == i):
+        nat.require_device(q, key_pages, value_pages, prefix_table, prefix_lens, block_table,
+                           seq_lens)
+    dev = q.device
     if not strides_ok:
         key_pages, value_pages = key_pages.contiguous(), value_pages.contiguous()
         ks = key_pages.stride()
@@ -1540,13 +1546,15 @@ def _beam_select(logits, scores, num_candidates, finished, eos_token_id):
                                                                      device=dev)
     if N:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        stream = _stream(dev)
+        counters = _join_counters("beam_select", dev, stream)
         with _guard(dev):
             rc = nat.load().lc_beam_select(
                 logits.data_ptr(), ls[0], ls[1], scores.data_ptr(),
                 None if finished is None else finished.data_ptr(),
                 0 if finished is None else int(eos_token_id), N, W, V, K, out.data_ptr(),
                 tokens.data_ptr(), parents.data_ptr(), None if done is None else done.data_ptr(),
-                ws.data_ptr(), ws_bytes, dtype, _stream(dev))
+                ws.data_ptr(), ws_bytes, counters, dtype, stream)
         if rc:
             nat.check(rc, "lc_beam_select")
     return (out, tokens, parents) if done is None else (out, tokens, parents, done)

@@ -119,13 +119,13 @@ def test_arguments_rejected_before_launch():
         assert b"lc_shared_prefix_decode_fwd" in lib.lc_last_error()
     assert attend(B=0, N=0) == 0 and attend(B=0) == 0
 
-    def select(groups=2, W=4, V=10, K=4, fin=None, eos=0, ws=1 << 15, dtype=0, wp=base):
+    def select(groups=2, W=4, V=10, K=4, fin=None, eos=0, ws=1 << 15, dtype=0, wp=base, cnt=None):
         return lib.lc_beam_select(base, 40, 10, base, fin, eos, groups, W, V, K, base, base, base, None,
-                                  wp, ws, dtype, None)
+                                  wp, ws, cnt, dtype, None)
 
     for bad in (dict(groups=-1), dict(W=0), dict(W=257), dict(V=0), dict(W=256, V=1 << 23), dict(K=0),
                 dict(K=65), dict(W=1, V=2, K=3), dict(fin=base, eos=10), dict(fin=base, eos=-1),
-                dict(ws=100), dict(dtype=3), dict(wp=base + 16), dict(wp=None)):
+                dict(ws=100), dict(dtype=3), dict(wp=base + 16), dict(wp=None), dict(cnt=base + 1)):
         assert select(**bad) < 0, bad
         assert b"lc_beam_select" in lib.lc_last_error()
     assert select(groups=0) == 0

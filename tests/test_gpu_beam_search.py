@@ -338,3 +338,46 @@ def test_captured_step(cuda):
         want, want_new = step()
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(new, want_new)
         assert torch.equal(k, saved[0]) and torch.equal(v, saved[1])
+
+
+@pytest.mark.parametrize("N,W,V,K", [(1, 4, 32000, 4), (3, 5, 1000, 8), (2, 24, 1397, 24), (1, 32, 700, 64), (40, 2, 999, 2)])
+def test_one_launch_equals_two(cuda, monkeypatch, N, W, V, K):
+    """The join by the last workgroup and the merge launch give the same bits, and leave the
+    tickets at zero."""
+    from llm_cuda.kernels import _ops
+
+    for seed in range(4):
+        x, s = make(N, W, V, BF16, seed)
+        if seed == 3:
+            s[:, 1:] = -INF  # one live beam
+        done = torch.zeros(N, W, dtype=torch.bool)
+        done[:, seed % W] = seed == 2
+        check_select(x, s, count=K, finished=done, eos=7, dev=cuda)
+        args = (x.to(cuda), s.to(cuda))
+        kw = dict(num_candidates=K, finished=done.to(cuda), eos_token_id=7)
+        one = select(*args, **kw)
+        stream = torch.cuda.current_stream().cuda_stream
+        assert not _ops._JOIN_COUNTERS[("beam_select", 0, stream)].any()
+        with monkeypatch.context() as m:
+            m.setattr(_ops, "_join_counters", lambda *key: None)
+            two = select(*args, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(one, two))
+
+
+def test_two_streams_at_once(cuda):
+    """Calls on two streams in flight together, many of them, each with its own tickets."""
+    from llm_cuda.kernels.beam_search import beam_select
+
+    jobs = [tuple(y.to(cuda) for y in make(2, 4, 5000, BF16, s)) for s in range(2)]
+    want = [beam_select(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(50):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(beam_select(*jobs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
