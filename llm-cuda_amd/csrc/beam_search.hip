@@ -63,10 +63,10 @@ __device__ __forceinline__ double from_ordered64(uint64_t k) {
 
 // The largest t with the bits below LOW clear that at least `count` of the wave's
 // keys reach, two bits at a time (the three compares of a step are independent).
+// t: their bits above TOP.
 template <int TOP, int LOW>
-__device__ __forceinline__ uint32_t wave_kth_largest(uint32_t key, int count) {
+__device__ __forceinline__ uint32_t wave_kth_largest(uint32_t key, int count, uint32_t t = 0) {
   static_assert((TOP - LOW) % 2 == 1, "whole pairs of bits");
-  uint32_t t = 0;
 #pragma unroll
   for (int bit = TOP - 1; bit >= LOW; bit -= 2) {
     const uint32_t c1 = t | (1u << bit), c2 = t | (2u << bit), c3 = t | (3u << bit);
@@ -136,8 +136,10 @@ struct SelectArgs {
 // 16 bytes of T from an address that may be unaligned.
 template <typename T>
 __device__ __forceinline__ Vec16<T> load16_any(const T* p) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+  const u4 x = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p));
   Vec16<T> v;
-  __builtin_memcpy(&v, p, 16);
+  __builtin_memcpy(&v, &x, 16);
   return v;
 }
 
@@ -486,12 +488,13 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
   __shared__ int found[kBeamWaves];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t row = blockIdx.x / a.chunks;
-  const int chunk = blockIdx.x - static_cast<int>(row) * a.chunks;
+  // (below 2^24 workgroups)
+  const int row = static_cast<int>(blockIdx.x / static_cast<uint32_t>(a.chunks));
+  const int chunk = static_cast<int>(blockIdx.x) - row * a.chunks;
   // (few rows: the flag arrives with the logits instead of before them)
   const bool done = a.finished != nullptr && a.finished[row] != 0;
   if (ITEMS > 8 && done) return;
-  const int64_t n = row / a.W;
+  const int n = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(a.W));
   const T* x = static_cast<const T*>(a.logits) + n * a.s_group + (row - n * a.W) * a.s_beam;
   const int c0 = chunk * CHUNK;
 
@@ -549,14 +552,27 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
   // the K-th largest of one wave, and the least of the waves' q-th largest, q = K /
   // 4 rounded up. The first always holds enough; the second, where all waves are
   // alike, little more. Elements equal to a bound count up to an index.
+  // Their upper 16 bits do, but where many lanes share the K-th's or it is -inf, whose
+  // upper bits alone would be a NaN's.
   const uint32_t key = ordered(top);
   constexpr int LOW = ordered_low<T>();
   auto whole = [](uint32_t t) {  // (a negative value's bits below LOW are set)
     return t < 0x80000000u ? t | ((1u << LOW) - 1) : t;
   };
-  const uint32_t t = whole(wave_kth_largest<31, LOW>(key, a.K));
+  uint32_t t = wave_kth_largest<31, 16>(key, a.K);
+  if constexpr (LOW < 16) {
+    if (__builtin_expect(
+            t < ordered(-INFINITY) || __popcll(__ballot((key ^ t) < 0x10000u)) > kTieSlack, 0))
+      t = whole(wave_kth_largest<15, LOW>(key, a.K, t));
+  } else {
+    t = whole(t);
+  }
   const int q = (a.K + kBeamWaves - 1) / kBeamWaves;
-  const uint32_t tq = q == 1 ? ordered(w_max) : whole(wave_kth_largest<31, LOW>(key, q));
+  uint32_t tq = ordered(w_max);
+  if (q != 1) {
+    tq = wave_kth_largest<31, 16>(key, q);
+    if (LOW == 16) tq = whole(tq);
+  }
   uint32_t t_index = CHUNK - 1;
   if (__builtin_expect(t == ordered(-INFINITY) || __popcll(__ballot(key == t)) > kTieSlack, 0)) {
     // Many elements at t (all masked ones, say): the lowest indices among them do. A
@@ -628,7 +644,7 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
     m += found[w];
     most = max(most, found[w]);
   }
-  uint64_t* out = a.keys + (row * a.chunks + chunk) * a.K;
+  uint64_t* out = a.keys + (static_cast<int64_t>(row) * a.chunks + chunk) * a.K;
   // (stored with the index in the row, not in the chunk)
   auto store = [&](int rank, uint64_t k) {
     const uint32_t at = ~(~static_cast<uint32_t>(k) + static_cast<uint32_t>(c0));
@@ -685,8 +701,8 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
     for (int w = 0; w < kBeamWaves; ++w)
       s += w_top[w] == -INFINITY ? static_cast<double>(w_sum[w])
                                  : w_sum[w] * exp(static_cast<double>(w_top[w]) - hi);
-    put_part<JOIN>(a.sums + row * a.chunks + chunk, s);
-    put_part<JOIN>(a.tops + row * a.chunks + chunk, hi);
+    put_part<JOIN>(a.sums + static_cast<int64_t>(row) * a.chunks + chunk, s);
+    put_part<JOIN>(a.tops + static_cast<int64_t>(row) * a.chunks + chunk, hi);
   }
 }
 
