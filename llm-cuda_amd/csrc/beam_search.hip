@@ -610,9 +610,8 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
   const float lim = from_ordered(static_cast<uint32_t>(limit >> 32));
   const uint32_t lim_index = CHUNK - static_cast<uint32_t>(limit);
 
-  auto key_of = [&](int i) -> uint64_t {  // (NaN: below every number; its beam's list is not used)
-    const float f = v[i] == v[i] ? v[i] : -INFINITY;
-    return (static_cast<uint64_t>(ordered(f)) << 32) | ~static_cast<uint32_t>(index_of(i));
+  auto key_at = [](float f, uint32_t i) -> uint64_t {  // (NaN: below every number; its beam's list is not used)
+    return (static_cast<uint64_t>(ordered(f == f ? f : -INFINITY)) << 32) | ~i;
   };
   // Gather what reaches the bound, each wave into its own part of the list.
   int n_found = 0;
@@ -623,7 +622,7 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
       const int pos = n_found + __builtin_amdgcn_mbcnt_hi(
                                     static_cast<uint32_t>(hits >> 32),
                                     __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hits), 0));
-      if (hit && pos < kWaveCap) list[wave][pos] = key_of(i);
+      if (hit && pos < kWaveCap) list[wave][pos] = key_at(v[i], index_of(i));
       n_found += __popcll(hits);
     };
     if (__builtin_expect(lim_index == CHUNK - 1, 1)) {
@@ -667,16 +666,23 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
       if (seg == 0 && i < m && rank < a.K) store(rank, k);
     }
   } else {
-    // Values laid out against the bounds (few lanes hold most of the best): the
-    // largest key below the last one, K times.
-    uint64_t last = ~0ull;
+    // Values laid out against the bounds (few lanes hold most of the best): the next
+    // element after the last one, K times. (Floats, not keys: those the compiler would
+    // make before the loop and keep, in registers that the kernel has not.)
+    float last_f = INFINITY;
+    uint32_t last_i = ~0u;
     for (int r = 0; r < a.K; ++r) {
-      uint64_t best = 0;
+      float f = -INFINITY;
+      uint32_t at = ~0u;
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        const uint64_t k = key_of(i);
-        if (k < last && k > best) best = k;
+      for (int i = ITEMS - 1; i >= 0; --i) {
+        const uint32_t here = index_of(i);
+        if ((v[i] < last_f || (v[i] == last_f && here > last_i)) && v[i] >= f) {
+          f = v[i];
+          at = here;
+        }
       }
+      uint64_t best = at == ~0u ? 0 : key_at(f, at);
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) {
         const uint64_t other = __shfl_xor(static_cast<unsigned long long>(best), o, 64);
@@ -688,7 +694,8 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
 #pragma unroll
       for (int w = 0; w < kBeamWaves; ++w) best = max(best, bound_k[w]);
       if (tid == 0) store(r, best);
-      last = best;
+      last_f = from_ordered(static_cast<uint32_t>(best >> 32));  // (0, none left: NaN)
+      last_i = ~static_cast<uint32_t>(best);
     }
   }
   if (tid == 0) {
@@ -706,8 +713,9 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
   }
 }
 
+// (8 waves per SIMD: 256 rows of 128256 fp32, 131 MB, take 29 us, 4.5 TB/s; 32 with 5)
 template <typename T, int ITEMS>
-__global__ __launch_bounds__(kBeamThreads) void beam_chunk_kernel(SelectArgs a) {
+__global__ __launch_bounds__(kBeamThreads, 8) void beam_chunk_kernel(SelectArgs a) {
   beam_chunk<T, ITEMS, false>(a);
 }
 
