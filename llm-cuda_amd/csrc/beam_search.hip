@@ -15,14 +15,20 @@ namespace {
 // Inside a beam the values are ordered as its logits, so the K best of a group
 // are among the K best logits of every beam, and those among the K best of
 // every chunk of a beam. One pass over the logits (they are read once, from HBM,
-// into registers) gives each chunk's K best and its part of the softmax sum; a
-// second, small launch joins the chunks: one workgroup per group.
+// into registers) gives each chunk's K best and its part of the softmax sum; one
+// workgroup per group then joins the chunks, in a launch of its own or, for small
+// calls, in the same one.
 //
 // A chunk's K best without a sort: the k-th largest of a wave's 64 lane maxima
 // (found on ballots, two bits at a time) bounds the chunk's K-th largest from
 // below, so only elements that reach the bound are gathered (little more than K);
-// each one's rank is the number of gathered keys above it. Keys are (order-preserving bits of the logit, inverted index): all are
-// different, and ties rank by index.
+// each one's rank is the number of gathered keys above it. Keys are
+// (order-preserving bits of the logit, inverted index): all are different, and ties
+// rank by index.
+//
+// Bound: HBM for many rows (256 rows of 128256 fp32, 131 MB: chunks 29 us, join 11),
+// the latency of two dependent passes for few (4 rows of 32000: 5.2 + 6.3 us; what
+// the host takes for the call, 15 us, is longer).
 //
 // The order of candidates of different beams hangs on their lse: the terms of
 // its sum are fp32 (v_exp_f32 of exact or once-rounded differences), added in
@@ -787,6 +793,10 @@ int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 // order, and copy the filled slots: no page that is read is written, so the
 // copies need no order among themselves, and column c stays a permutation of
 // the group's own pages.
+//
+// Bound: HBM (4 groups of 8, 3 childless each, 32 layers of 8 x 44 x 128 bf16 slots: 138
+// MB read and written in 38 us) or, for few copies, the launch and the chain parents ->
+// table -> page (5.5 us).
 //
 // One launch: the new table goes to another buffer (its old entries are read by
 // every workgroup), a workgroup per group writes it, and one workgroup per
