@@ -1441,10 +1441,11 @@ def _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, 
         q = q.contiguous()
         qs = q.stride()
     pt_s, bt_s = prefix_table.stride(), block_table.stride()
-    if p_pages > 1 and pt_s[1] != 1:
+    # (rows that overlap, one expanded to all groups say, are copied: the kernels' rows do not)
+    if (p_pages > 1 and pt_s[1] != 1) or (N > 1 and pt_s[0] < p_pages):
         prefix_table = prefix_table.contiguous()
         pt_s = prefix_table.stride()
-    if s_pages > 1 and bt_s[1] != 1:
+    if (s_pages > 1 and bt_s[1] != 1) or (B > 1 and bt_s[0] < s_pages):
         block_table = block_table.contiguous()
         bt_s = block_table.stride()
     prefix_lens, seq_lens = prefix_lens.contiguous(), seq_lens.contiguous()
@@ -1458,8 +1459,8 @@ def _shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens, 
     if B:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         stream = _stream(dev)
-        counters = _join_counters("shared_prefix", dev, stream)
         with _guard(dev):
+            counters = _join_counters("shared_prefix", dev, stream)
             rc = nat.load().lc_shared_prefix_decode_fwd(
                 q.data_ptr(), qs[0], qs[1], key_pages.data_ptr(), value_pages.data_ptr(), ks[0],
                 ks[1], ks[2], num_pages, prefix_table.data_ptr(), max(pt_s[0], p_pages), p_pages,
@@ -1547,8 +1548,8 @@ def _beam_select(logits, scores, num_candidates, finished, eos_token_id):
     if N:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         stream = _stream(dev)
-        counters = _join_counters("beam_select", dev, stream)
         with _guard(dev):
+            counters = _join_counters("beam_select", dev, stream)
             rc = nat.load().lc_beam_select(
                 logits.data_ptr(), ls[0], ls[1], scores.data_ptr(),
                 None if finished is None else finished.data_ptr(),
@@ -1592,7 +1593,7 @@ def paged_kv_reorder(key_pages: torch.Tensor, value_pages: torch.Tensor,
     dtype = nat.lc_dtype(key_pages)
     dev = nat.require_device(key_pages, value_pages, block_table, seq_lens, parents, out)
     ts = block_table.stride()
-    if M > 1 and ts[1] != 1:
+    if (M > 1 and ts[1] != 1) or (N * W > 1 and ts[0] < M):
         block_table = block_table.contiguous()
         ts = block_table.stride()
     seq_lens, parents = seq_lens.contiguous(), parents.contiguous()
@@ -1600,7 +1601,8 @@ def paged_kv_reorder(key_pages: torch.Tensor, value_pages: torch.Tensor,
         out = torch.empty((N * W, M), dtype=torch.int32, device=dev)
         o_stride = M
     else:
-        if out.dtype is not torch.int32 or out.shape != (N * W, M) or (M > 1 and out.stride(1) != 1):
+        if out.dtype is not torch.int32 or out.shape != (N * W, M) or (M > 1 and out.stride(1) != 1) \
+                or (N * W > 1 and out.stride(0) < M):
             raise ValueError(f"out must be int32 {(N * W, M)} with contiguous rows")
         o_stride = max(out.stride(0), M)
     if N * W and M:
@@ -1624,6 +1626,8 @@ def _reorder_sizes(k, v, ks, vs, block_table, seq_lens, parents):
                          "page, dim]")
     if ks != vs or ks[-1] != 1:
         raise ValueError("key_pages and value_pages must share a layout with unit dim stride")
+    if any(n > 1 and stride == 0 for n, stride in zip(k, ks)):
+        raise ValueError("key_pages and value_pages are written: they cannot be expanded")
     L, s_layer = (k[0], ks[0]) if len(k) == 5 else (1, 0)
     num_pages, Hkv, P, D = k[-4:]
     if len(parents) != 2:

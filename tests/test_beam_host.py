@@ -85,6 +85,8 @@ def test_selection_refuses(kw, error):
     (dict(parents=torch.zeros(2, 2, dtype=I32)), TypeError),
     (dict(parents=torch.zeros(4, dtype=I64)), TypeError),
     (dict(parents=torch.zeros(2, 3, dtype=I64)), ValueError),
+    (dict(key_pages=torch.zeros(1, 1, 2, 8, 16).expand(1, 8, 2, 8, 16),
+          value_pages=torch.zeros(1, 1, 2, 8, 16).expand(1, 8, 2, 8, 16)), ValueError),
     (dict(), RuntimeError),
 ])
 def test_reordering_refuses(kw, error):

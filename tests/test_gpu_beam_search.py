@@ -381,3 +381,24 @@ def test_two_streams_at_once(cuda):
     for i in range(2):
         for out in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+
+
+def test_reorder_overlapping_tables(cuda):
+    """A table whose rows are one expanded row is read as such; an out that overlaps the
+    table, or itself, is refused."""
+    from llm_cuda.kernels.beam_search import paged_kv_reorder
+
+    kp, vp, _ = caches(1, 1, 4, 3, 8, 1, 16, BF16)
+    k, v = kp.to(cuda), vp.to(cuda)
+    row = torch.tensor([[3, 1, 2]], dtype=torch.int32, device=cuda)
+    lens = torch.full((4,), 16, dtype=torch.int32, device=cuda)  # whole pages: nothing is copied
+    parents = torch.tensor([[2, 2, 0, 1]], device=cuda)
+    new = paged_kv_reorder(k, v, row.expand(4, 3), lens, parents)
+    assert torch.equal(new, row.repeat(4, 1))
+    assert torch.equal(k.cpu(), kp) and torch.equal(v.cpu(), vp)
+    pool = row.repeat(8, 1)
+    for table, out in ((pool[:4], pool[:4]), (pool[:4], pool[3:7]), (pool[3:7], pool[:4]),
+                       (pool[:4], torch.empty(1, 3, dtype=torch.int32, device=cuda).expand(4, 3))):
+        with pytest.raises(RuntimeError if out.stride(0) else ValueError):
+            paged_kv_reorder(k, v, table, lens, parents, out=out)
+    assert torch.equal(paged_kv_reorder(k, v, pool[:4], lens, parents, out=pool[4:]), row.repeat(4, 1))

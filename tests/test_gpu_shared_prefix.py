@@ -314,3 +314,14 @@ def test_forward_only(cuda):
     args[0].requires_grad_(True)
     with pytest.raises(NotImplementedError, match="shared_prefix_decode"):
         op(*args).sum().backward()
+
+
+def test_expanded_tables(cuda):
+    """One row of a table or of lengths for all groups or sequences, without a copy of it."""
+    from llm_cuda.kernels.triton.decode_attention import shared_prefix_decode_attention as op
+
+    args = [t.to(cuda) for t in make(3, 2, 8, 2, 64, 16, [100] * 3, [20] * 6, BF16)]
+    q, kp, vp, ptab, plens, btab, slens = args
+    wide = op(q, kp, vp, ptab[:1].expand(3, -1), plens[:1].expand(3), btab[:1].expand(6, -1), slens[:1].expand(6))
+    full = op(q, kp, vp, ptab[:1].repeat(3, 1), plens[:1].repeat(3), btab[:1].repeat(6, 1), slens[:1].repeat(6))
+    assert torch.equal(wide, full)
