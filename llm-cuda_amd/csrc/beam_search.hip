@@ -83,6 +83,26 @@ __device__ __forceinline__ uint32_t wave_kth_largest(uint32_t key, int count, ui
   return t;
 }
 
+// The same of four keys a lane.
+template <int TOP, int LOW>
+__device__ __forceinline__ uint32_t wave_kth_of_4(const uint32_t (&key)[4], int count) {
+  static_assert((TOP - LOW) % 2 == 1, "whole pairs of bits");
+  uint32_t t = 0;
+#pragma unroll
+  for (int bit = TOP - 1; bit >= LOW; bit -= 2) {
+    const uint32_t c1 = t | (1u << bit), c2 = t | (2u << bit), c3 = t | (3u << bit);
+    int n1 = 0, n2 = 0, n3 = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      n1 += __popcll(__ballot(key[i] >= c1));
+      n2 += __popcll(__ballot(key[i] >= c2));
+      n3 += __popcll(__ballot(key[i] >= c3));
+    }
+    t = n3 >= count ? c3 : n2 >= count ? c2 : n1 >= count ? c1 : t;
+  }
+  return t;
+}
+
 // The lowest bit of ordered(x) that tells values of T apart; those below it are
 // all clear (x >= 0) or all set.
 template <typename T>
@@ -191,7 +211,8 @@ __device__ __forceinline__ void beam_merge(const SelectArgs& a, int64_t n) {
   const int K = a.K, lists = a.W * a.chunks;
   if (tid == 0) count = reached = 0;
   // Few candidates: every thread's kHeld of them, the lists' first ones first, are
-  // loaded before the sums are joined; else only the lists that turn out to matter.
+  // loaded before the sums are joined; else a list's first and last, and of the rest
+  // only those of lists that turn out to matter.
   constexpr int kHeld = kHeldCandidates / kMergeThreads;
   const bool few = lists * K <= kHeld * kMergeThreads;
   uint64_t held[kHeld];
@@ -204,6 +225,10 @@ __device__ __forceinline__ void beam_merge(const SelectArgs& a, int64_t n) {
       held_l[r] = static_cast<int>(i) - held_k[r] * lists;
       held[r] = part<JOIN>(a.keys + (n * lists + held_l[r]) * K + min(held_k[r], K - 1));
     }
+  } else {
+    const uint64_t* list = a.keys + (n * lists + min(tid, lists - 1)) * K;
+    held[0] = part<JOIN>(list);
+    held[1] = part<JOIN>(list + K - 1);
   }
   for (int w = wave; w < a.W; w += kMergeWaves) {
     const int64_t row = n * a.W + w;
@@ -333,9 +358,9 @@ __device__ __forceinline__ void beam_merge(const SelectArgs& a, int64_t n) {
     for (int r = 0; r < kEach; ++r) add(v[r], f[r]);
     __syncthreads();
   };
-  // The K-th best of a wave's lanes, each with its best value (a list's first, where
-  // there are many), is a lower bound of the K-th largest value; so is the lowest above
-  // -inf where K are above it (one live beam: the others' -inf fill the waves).
+  // The K-th best of a wave's lanes, each with its best value, is a lower bound of the
+  // K-th largest value (where there are many, of all lists' first ones); so is the lowest
+  // above -inf where K are above it (one live beam: the others' -inf fill the waves).
   uint64_t head = 0, held_v[kHeld];
   uint32_t held_f[kHeld];
   int n_above = 0;
@@ -352,11 +377,33 @@ __device__ __forceinline__ void beam_merge(const SelectArgs& a, int64_t n) {
     for (int l = tid; l < lists; l += kMergeThreads) {
       uint64_t v;
       uint32_t f;
-      candidate(l, 0, v, f);
+      candidate_of(l, 0, l == tid ? held[0] : part<JOIN>(a.keys + (n * lists + l) * K), v, f);
       head = max(head, v);
     }
   }
-  const uint32_t t = wave_kth_largest<31, 0>(static_cast<uint32_t>(head >> 32), K);
+  uint32_t t = 0;
+  if (few) {
+    t = wave_kth_largest<31, 0>(static_cast<uint32_t>(head >> 32), K);
+  } else {
+    reach[tid] = static_cast<int>(head >> 32);
+    __syncthreads();
+    if (wave == 0) {  // the K-th best of 256 threads or groups of threads
+      uint32_t best[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < kMergeThreads; i += 64)
+        best[(i >> 6) & 3] = max(best[(i >> 6) & 3], static_cast<uint32_t>(reach[i + lane]));
+      t = wave_kth_of_4<31, 10>(best, K);
+    }
+    // (and a list's K-th is one as well, the highest where a beam stands out)
+    uint64_t v = 0;
+    uint32_t f;
+    if (tid < lists) candidate_of(tid, K - 1, held[1], v, f);
+    uint32_t last = static_cast<uint32_t>(v >> 32);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1)
+      last = max(last, static_cast<uint32_t>(__shfl_xor(static_cast<int>(last), o, 64)));
+    t = max(t, last);
+  }
   if (lane == 0) {
     bound[wave] = static_cast<uint64_t>(t) << 32;
     above[wave] = n_above;
