@@ -26,7 +26,7 @@ namespace {
 // (order-preserving bits of the logit, inverted index): all are different, and ties
 // rank by index.
 //
-// Bound: HBM for many rows (256 rows of 128256 fp32, 131 MB: chunks 29 us, join 11),
+// Bound: HBM for many rows (256 rows of 128256 fp32, 131 MB: chunks 29 us, join 10.6),
 // the latency of two dependent passes for few (4 rows of 32000: 5.2 + 6.3 us; what
 // the host takes for the call, 15 us, is longer).
 //
@@ -45,7 +45,7 @@ constexpr int kMergeCap = 4096;    // gathered candidates of a group
 constexpr int kMergeThreads = 1024;
 constexpr int kHeldCandidates = 2048;  // most that the merge holds before the sums are joined
 constexpr int kJoinCounters = 4096;
-constexpr int kJoinWidth = 8;  // most beams of a group that are joined in the same launch
+constexpr int kJoinWidth = 32;  // most beams of a group that are joined in the same launch
 constexpr int kReachCap = 1024;    // lists of a group whose candidates are looked through
 
 // Order-preserving bits of a float (not NaN); -0 counts as +0.
@@ -777,9 +777,9 @@ __global__ __launch_bounds__(kBeamThreads, 8) void beam_chunk_kernel(SelectArgs 
 
 // Few beams and candidates: the workgroup of a group that finishes last (its ticket on
 // counters[n], zero at entry and left zero) joins the chunks, in the same launch. The
-// GPU takes as long as in two (4 beams of 32000: 10.9 us for 5.2 + 6.3; 8 of 32000:
-// 14.2 for 5.9 + 6.8; 16 of 1003, beyond the rule: 16.8 for 6.3 + 7.6), and the host,
-// which such a call waits for, a launch less: 17.2 -> 15.4 us a call.
+// GPU takes as long as in two (4 beams of 32000: 11.0 us for 5.2 + 6.3; 16 of 1003:
+// 12.2 for 7.7 + 6.7; 32 of 2000: 15.3 for 7.4 + 7.1), and the host, which such a call
+// waits for, a launch less: 17.2 -> 15.4 us a call.
 template <typename T>
 __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(SelectArgs a) {
   __shared__ int last;
