@@ -666,7 +666,8 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
   const float lim = from_ordered(static_cast<uint32_t>(limit >> 32));
   const uint32_t lim_index = CHUNK - static_cast<uint32_t>(limit);
 
-  auto key_at = [](float f, uint32_t i) -> uint64_t {  // (NaN: below every number; its beam's list is not used)
+  // (NaN: below every number; its beam's list is not used)
+  auto key_at = [](float f, uint32_t i) -> uint64_t {
     return (static_cast<uint64_t>(ordered(f == f ? f : -INFINITY)) << 32) | ~i;
   };
   // Gather what reaches the bound, each wave into its own part of the list.

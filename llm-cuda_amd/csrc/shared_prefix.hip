@@ -1327,8 +1327,8 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
                                 int64_t bt_stride, int64_t max_pages_per_seq,
                                 const int32_t* seq_lens, void* out, int64_t o_sb, int64_t o_sh,
                                 float* lse, void* workspace, int64_t workspace_bytes,
-                                int32_t* counters, int64_t B, int64_t groups, int64_t Hq, int64_t Hkv, int64_t D,
-                                int64_t page_size, float scale, int dtype, void* stream) {
+                                int32_t* counters, int64_t B, int64_t groups, int64_t Hq,
+                                int64_t Hkv, int64_t D, int64_t page_size, float scale, int dtype, void* stream) {
   static const char* who = "lc_shared_prefix_decode_fwd";
   LC_REQUIRE(B >= 0 && B < 65536, "%s: batch %lld out of range", who, (long long)B);
   LC_REQUIRE(groups > 0 ? B % groups == 0 : B == 0,
@@ -1409,11 +1409,14 @@ int lc_shared_prefix_decode_fwd(const void* q, int64_t q_sb, int64_t q_sh, const
   hipStream_t st = lc_stream(stream);
   switch (dtype) {
     case LC_DTYPE_F32:
-      return launch_shared<float>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse, st);
+      return launch_shared<float>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse,
+                                 st);
     case LC_DTYPE_BF16:
-      return launch_shared<bf16_t>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse, st);
+      return launch_shared<bf16_t>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse,
+                                  st);
     default:
-      return launch_shared<f16_t>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse, st);
+      return launch_shared<f16_t>(a, plan.wr, plan.own_waves, mfma, counters, out, o_sb, o_sh, lse,
+                                 st);
   }
 }
 
