@@ -325,3 +325,19 @@ def test_expanded_tables(cuda):
     wide = op(q, kp, vp, ptab[:1].expand(3, -1), plens[:1].expand(3), btab[:1].expand(6, -1), slens[:1].expand(6))
     full = op(q, kp, vp, ptab[:1].repeat(3, 1), plens[:1].repeat(3), btab[:1].repeat(6, 1), slens[:1].repeat(6))
     assert torch.equal(wide, full)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("W,plen", [(1, 2700), (2, 3900), (3, 2100)])
+def test_many_ranges(cuda, monkeypatch, dtype, W, plen):
+    """Long prefixes of few rows, with tickets and without: right, and the same bits."""
+    from llm_cuda.kernels import _ops
+    from llm_cuda.kernels.triton.decode_attention import shared_prefix_decode_attention as op
+
+    args = [t.to(cuda) for t in make(1, W, 8, 2, 64, 64, [plen], [5 + 40 * i for i in range(W)], dtype)]
+    check([t.cpu() for t in args], run([t.cpu() for t in args], cuda))
+    one = op(*args, return_lse=True)
+    with monkeypatch.context() as m:
+        m.setattr(_ops, "_join_counters", lambda *key: None)
+        two = op(*args, return_lse=True)
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
