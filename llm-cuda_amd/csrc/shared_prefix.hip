@@ -166,14 +166,29 @@ __global__ __launch_bounds__(64) void shared_generic_kernel(SharedArgs a) {
 // Tokens are named by a table, so every lane finds the address of its own 16-byte
 // chunk of a DMA; lanes whose token is past the range, whose page entry is invalid
 // or whose chunk is past head_dim read zeros instead, and their scores are masked.
-// The weights P are rounded to the data type for the second product, as the
-// matrix instructions take it: 2^-8 relative each in bf16, far below the output's
-// own rounding after they are averaged; their sum stays in fp32.
+// The matrix instructions take the weights P in the data type, so each goes there as
+// two values of it, the rounded weight and what that rounding left (which keeps 2^-16
+// of a bf16 weight, 2^-22 of an f16 one, down to 2^-25); their sum stays in fp32. The
+// rounded weight alone would leave an error as large as the output's own rounding,
+// for values without a common mean average the output down as much as the errors
+// (8448 bf16 tokens: 2.3e-3 rms of the output, 1.66e-3 with both, which is the
+// output's rounding). The second value is free where K and V are streamed (4 groups
+// of 8 x 4224: 22.4 us either way); where a prefix has many rows, PV is twice the
+// matrix work: 64 x (8192 + 625) 52 -> 56 us, 256 x (8192 + 200) 76 -> 86.
 // ---------------------------------------------------------------------------
 constexpr int kTile = 64;  // tokens per tile
 constexpr float kSharedRescaleLog2 = 8.0f;
 
 __device__ __attribute__((aligned(16))) const uint32_t shared_zeros[4] = {0, 0, 0, 0};
+
+// A weight as a value of the data type and what its rounding left, rounded in turn.
+template <typename V>
+__device__ __forceinline__ void split_weight(float p, V& whole, V& rest, int i) {
+  typedef std::remove_reference_t<decltype(whole[0])> T;
+  const T w = static_cast<T>(p);
+  whole[i] = w;
+  rest[i] = static_cast<T>(p - static_cast<float>(w));
+}
 
 struct RangeItem {
   const int32_t* table;  // the token range's table row
@@ -369,7 +384,7 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
   float m_ref = -INFINITY, l_lane = 0.f, l_tile = 0.f;
   f32x16_t x[NKT];  // raw scores of the next tile
   f32x16_t y[NKT];  // exponents of the current tile, relative to m_ref
-  v8 pop[NKT][2];
+  v8 pop[NKT][2], rem[NKT][2];
 
   auto qk = [&](LC_LDS const char* kt_lds) __attribute__((always_inline)) {
 #pragma unroll
@@ -397,6 +412,7 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
               (LC_LDS i16x4_t*)(vt_lds + vaddr[1][dt] + rowoff));
           const i16x8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
           o[dt] = Ops::mma(__builtin_bit_cast(v8, both), pop[kt][jp], o[dt]);
+          o[dt] = Ops::mma(__builtin_bit_cast(v8, both), rem[kt][jp], o[dt]);
         }
   };
   // Scores of tokens that are none are masked; rows without a reference max (only
@@ -437,7 +453,7 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
       for (int r = 0; r < 16; ++r) {
         const float p = lc_exp2(y[kt][r]);
         if (r & 1) s1 += p; else s0 += p;
-        pop[kt][r >> 3][r & 7] = static_cast<T>(p);
+        split_weight(p, pop[kt][r >> 3], rem[kt][r >> 3], r & 7);
       }
     l_tile = s0 + s1;
   };
@@ -707,12 +723,12 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
       m_ref = m_new;
     }
     const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-    v8 pop[2];
+    v8 pop[2], rem[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const float p = lc_exp2(x[r] - m_use);
       l_lane += p;
-      pop[r >> 3][r & 7] = static_cast<T>(p);
+      split_weight(p, pop[r >> 3], rem[r >> 3], r & 7);
     }
 #pragma unroll
     for (int jp = 0; jp < 2; ++jp)
@@ -724,6 +740,7 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
             (LC_LDS i16x4_t*)(lds_v + vaddr[1][dt] + jp * 16 * ROW_B));
         const i16x8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         o[dt] = Ops::mma(__builtin_bit_cast(v8, both), pop[jp], o[dt]);
+        o[dt] = Ops::mma(__builtin_bit_cast(v8, both), rem[jp], o[dt]);
       }
     lc_compiler_fence();
   }
@@ -1172,15 +1189,15 @@ struct SharedPlan {
 // Ranges per prefix and per sequence, such that a range is what one CU would do if
 // all tokens were dealt out evenly: every further range costs its partial outputs
 // (512 bytes a row, written and read back) and a start. A prefix token of a 128-row
-// tile counts as four of a stream's, of a 64-row tile as two (GPU time of a call,
-// us, by ranges per prefix; 8B heads):
-//   256 x (8192 + 200) tokens  2: 109  3: 88  4: 78  5: 78  6: 83  8: 91
-//   64 x (8192 + 625)          8: 52  12: 52  16: 54  20: 69  32: 69
-//   4 groups x 8 x (4096 + 128)  4: 23.8  6: 23.2  8: 27  13: 27  16: 33
+// tile counts as six of a stream's (a QK and two PV products for four times the rows),
+// of a 64-row tile as three (GPU time of a call, us, by ranges per prefix; 8B heads):
+//   256 x (8192 + 200) tokens  2: 125  3: 97  4: 86  5: 93  6: 93  8: 101
+//   64 x (8192 + 625)          8: 58  9: 57  10: 56  12: 56  16: 57  20: 72
+//   4 groups x 8 x (4096 + 128)  4: 25.3  6: 23.1  8: 23.2  13: 29.6  16: 31.1
 // No range is shorter than two tiles.
 // A range of a sequence's own tokens is shared by 4, 2 or 1 waves: one wave has no
 // join at the end and a longer run of steps, which pays with many short ranges
-// (256 x 200 tokens: 88 / 79 / 78 us with 4 / 2 / 1 waves; 64 x 625: 53 / 52 / 59);
+// (256 x 200 tokens: 102 / 92 / 87 us with 4 / 2 / 1 waves; 64 x 625: 56 / 57 / 61);
 // where the ranges are few, four finish sooner.
 SharedPlan shared_plan(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_cap,
                        int64_t s_cap, int dtype) {
@@ -1188,7 +1205,8 @@ SharedPlan shared_plan(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_
   const int64_t G = Hq / Hkv, W = B / N, cus = lc_cu_count();
   const int wr = dtype == LC_DTYPE_F32 || W * G <= 32 ? 1 : W * G <= 64 ? 2 : 4;
   const int64_t up = N * Hkv * lc_cdiv(W * G, 32 * wr), us = B * Hkv * lc_cdiv(G, 32);
-  const int64_t each = lc_cdiv(up * p_cap * wr + us * s_cap, cus);
+  const int64_t weight = wr == 1 ? 1 : wr * 3 / 2;
+  const int64_t each = lc_cdiv(up * p_cap * weight + us * s_cap, cus);
   auto splits = [&](int64_t cap, int64_t tokens) -> int {
     if (cap == 0) return 0;
     const int64_t s = lc_cdiv(cap, tokens < 2 * kSharedStep ? 2 * kSharedStep : tokens);
@@ -1196,7 +1214,7 @@ SharedPlan shared_plan(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_
   };
   SharedPlan p;
   p.wr = wr;
-  p.p_splits = splits(p_cap, lc_cdiv(each, wr));
+  p.p_splits = splits(p_cap, lc_cdiv(each, weight));
   p.s_splits = splits(s_cap, each);
   const int64_t ranges = us * p.s_splits;
   const int64_t steps = p.s_splits > 0 ? lc_cdiv(lc_cdiv(s_cap, p.s_splits), 32) : 0;
