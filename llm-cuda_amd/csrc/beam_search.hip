@@ -186,8 +186,8 @@ __device__ __forceinline__ void put_part(P* to, X from) {
 
 // One workgroup per group: the beams' lse, then the K best of their chunks' lists.
 // Beams without ordinary values stand for themselves: finished (the eos token at
-// their score, -inf elsewhere), empty (no finite logit, or a score of -inf: -inf
-// everywhere) and undefined (NaN or +inf in the logits or the score: NaN).
+// their score, -inf elsewhere), empty (no finite logit, or a score of -inf, finished
+// or not: -inf everywhere) and undefined (NaN or +inf in the logits or the score: NaN).
 enum : int { kBeamOrdinary = 0, kBeamFinished, kBeamEmpty, kBeamUndefined };
 
 // kMergeThreads threads, room for kMergeCap gathered candidates. JOIN: the chunks' parts
@@ -260,11 +260,12 @@ __device__ __forceinline__ void beam_merge(const SelectArgs& a, int64_t n) {
                      part<JOIN>(a.sums + row * a.chunks + c));
     for (int o = lanes / 2; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
     if (c0 == 0 && w < a.W) {
-      const bool empty = sum == 0 || score == -INFINITY;
-      kind[w] = done                                      ? kBeamFinished
+      // (a finished beam's score may be -inf: its eos is one of equal tokens then)
+      const bool dead = score == -INFINITY;
+      kind[w] = done                                ? (dead ? kBeamEmpty : kBeamFinished)
                 : sum != sum || !(score < INFINITY) ? kBeamUndefined
-                : empty                                   ? kBeamEmpty
-                                                          : kBeamOrdinary;
+                : sum == 0 || dead                  ? kBeamEmpty
+                                                    : kBeamOrdinary;
       // (the largest logit is taken off the logits, not added to the score: beside a
       // row of a type's lowest value neither the score nor the log would count)
       base[w] = done ? score : score - log(sum);
