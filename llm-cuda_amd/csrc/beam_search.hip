@@ -539,6 +539,7 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
   constexpr int CHUNK = kBeamThreads * ITEMS;
   static_assert(ITEMS % VEC == 0, "whole vectors per thread");
   static_assert(CHUNK < (1 << 14), "inverted indices inside a chunk are 14 bits");
+  static_assert((CHUNK & (CHUNK - 1)) == 0, "a row's chunks end at 2^31 at most");
   __shared__ uint64_t list[kBeamWaves][kWaveCap];
   __shared__ uint64_t bound_k[kBeamWaves], bound_q[kBeamWaves];
   __shared__ float w_top[kBeamWaves], w_sum[kBeamWaves];
@@ -571,11 +572,11 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) v[i] = lc_to_f32(raw[i / VEC].v[i % VEC]);
     if (ITEMS <= 8 && done) return;
-    if (c0 + CHUNK > a.V) {
+    if (c0 > a.V - CHUNK) {  // (the chunk's end may be 2^31; its indices are below)
 #pragma unroll
       for (int j = 0; j < ITEMS / VEC; ++j) {
         const int at = c0 + static_cast<int>(index_of(j * VEC));
-        if (at + VEC > a.V) {
+        if (at > a.V - VEC) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
             v[j * VEC + e] = at + e < a.V ? lc_to_f32(x[at + e]) : -INFINITY;

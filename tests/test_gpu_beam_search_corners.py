@@ -22,3 +22,19 @@ def test_finished_beams_without_a_score(cuda, N, W, V, K, eos):
     done = torch.zeros(N, W, dtype=torch.bool)
     done[:, 0] = done[:, W - 1] = True
     check_select(x, s, count=K, finished=done, eos=eos, dev=cuda)
+
+
+@pytest.mark.parametrize("V", [2 ** 31 - 1, 2 ** 31 - 8191])
+def test_vocabularies_up_to_the_limit(cuda, V):
+    """One beam whose last chunk ends past 2^31: few tokens allowed, at the row's ends, so that
+    one counted twice shows (their logits, and so the sum, are small whole numbers)."""
+    from llm_cuda.kernels.beam_search import beam_select
+
+    x = torch.full((1, 1, V), -INF, dtype=BF16, device=cuda)
+    at = torch.tensor([0, 7, 2 ** 30, V - 9, V - 8, V - 7, V - 2, V - 1])
+    value = torch.tensor([1.0, 2.0, -1.0, 3.0, 0.5, 2.5, 4.0, 3.5])
+    x[0, 0, at.to(cuda)] = value.to(BF16).to(cuda)
+    scores, tokens, parents = beam_select(x, torch.zeros(1, 1, device=cuda), num_candidates=8)
+    want, order = torch.log_softmax(value.double(), 0).sort(descending=True)
+    assert torch.equal(tokens[0].cpu(), at[order]) and not parents.any()
+    assert (scores[0].double().cpu() - want).abs().max().item() <= 1e-6 + 2 ** -24 * 8
