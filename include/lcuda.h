@@ -578,7 +578,7 @@ LC_API int lc_beam_select(const void* logits, int64_t group_stride, int64_t beam
  * page_size, D] pools with shared strides (head_dim contiguous), one table for
  * all layers; pages with entries outside [0, num_pages) are not copied.
  * out_table: int32 [groups * width, max_pages_per_seq]; must not overlap
- * block_table. width <= 256.
+ * block_table. width <= 256, width * max_pages_per_seq < 2^31 - 256.
  * No counterpart in the reference (see lc_beam_select). */
 LC_API int lc_paged_kv_reorder(void* key_pages, void* value_pages, int64_t kv_s_layer,
                                int64_t kv_s_page, int64_t kv_s_head, int64_t kv_s_tok,

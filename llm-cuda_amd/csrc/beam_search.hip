@@ -1049,6 +1049,8 @@ int lc_paged_kv_reorder(void* key_pages, void* value_pages, int64_t kv_s_layer, 
                  num_pages < (1LL << 31),
              "%s: bad sizes", who);
   LC_REQUIRE(max_pages_per_seq < (1LL << 30) / page_size, "%s: a table of 2^30 tokens or more", who);
+  LC_REQUIRE(width * max_pages_per_seq < (1LL << 31) - 256,
+             "%s: a table of 2^31 entries a group or more", who);
   LC_REQUIRE(Hkv < (1LL << 28) / page_size && D < (1LL << 28) / (page_size * Hkv),
              "%s: pages of 2^28 elements or more", who);
   LC_REQUIRE(dtype == LC_DTYPE_F32 || dtype == LC_DTYPE_F16 || dtype == LC_DTYPE_BF16,
