@@ -1379,7 +1379,8 @@ def _join_counters(kind: str, dev: torch.device, stream: int) -> int | None:
     if buf is None:
         n = max(nat.size("lc_shared_prefix_decode_counter_count"),
                 nat.size("lc_beam_select_counter_count"))
-        buf = _JOIN_COUNTERS[key] = torch.zeros(n, dtype=torch.int32, device=dev)
+        # (of threads that come here together one's buffer stays, for all of them)
+        buf = _JOIN_COUNTERS.setdefault(key, torch.zeros(n, dtype=torch.int32, device=dev))
     return buf.data_ptr()
 
 

@@ -1,4 +1,6 @@
 """Beam operators without a GPU: sizes past the kernels' index arithmetic, and what calls share."""
+import threading
+
 import torch
 
 
@@ -18,3 +20,32 @@ def test_tables_past_32_bits_are_refused():
     for W, M in ((256, 1 << 23), (128, 1 << 24), (255, (1 << 31) // 255), (256, (1 << 27) - 1)):
         assert reorder(W, M) < 0, (W, M)
         assert b"2^31 entries" in lib.lc_last_error()
+
+
+def test_first_calls_of_two_threads_share_their_tickets(monkeypatch):
+    """Two threads that both find no tickets for a stream launch with the same buffer, the one
+    that is kept: the other's memory is free for any tensor as soon as it is dropped."""
+    from llm_cuda.kernels import _ops
+
+    both, zeros, got = threading.Barrier(2), torch.zeros, []
+
+    def zeros_together(*args, **kw):
+        buf = zeros(*args, **kw)
+        try:
+            both.wait(5)  # the other thread has found none either
+        except threading.BrokenBarrierError:
+            pass
+        return buf
+
+    monkeypatch.setattr(_ops, "_JOIN_COUNTERS", {})
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False)
+    monkeypatch.setattr(torch, "zeros", zeros_together)
+    cpu = torch.device("cpu")
+    threads = [threading.Thread(target=lambda: got.append(_ops._join_counters("beam_select", cpu, 0)))
+               for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    (kept,) = _ops._JOIN_COUNTERS.values()
+    assert got == [kept.data_ptr()] * 2
