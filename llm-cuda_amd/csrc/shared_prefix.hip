@@ -473,7 +473,7 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
       for (int dt = 0; dt < DTL; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-      m_ref = m_ref == -INFINITY ? up : m_ref + up;
+      m_ref += up;  // (a row without a finite score so far, up 0, stays without a reference)
 #pragma unroll
       for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
