@@ -32,18 +32,31 @@ def definition(q, kp, vp, pt, pl, bt, sl, scale=None):
         live = (page >= 0) & (page < pages)
         return pool[page[live], :, at[live] % P].double()  # [tokens, Hkv, D]
 
+    def attend(rows, k, v):
+        x = rows.double() @ k.T * scale
+        if not len(k):
+            return torch.zeros(rows.shape, dtype=torch.float64), torch.full(rows.shape[:1], -math.inf).double()
+        return torch.softmax(x, -1) @ v, torch.logsumexp(x, -1)
+
     out = torch.zeros(B, Hq, D, dtype=torch.float64)
     lse = torch.full((B, Hq), -math.inf, dtype=torch.float64)
-    shared = [[tokens(p, pt[n], int(pl[n])) for p in (kp, vp)] for n in range(N)]
-    for b in range(B):
-        k, v = (torch.cat([shared[b // (B // N)][i], tokens(p, bt[b], int(sl[b]))])
-                for i, p in enumerate((kp, vp)))
-        if not len(k):
-            continue
+    W = B // N
+    for n in range(N):
+        ks, vs = (tokens(p, pt[n], int(pl[n])) for p in (kp, vp))
         for h in range(Hkv):
-            s = q[b, h * G:(h + 1) * G, 0].double() @ k[:, h].T * scale
-            lse[b, h * G:(h + 1) * G] = torch.logsumexp(s, -1)
-            out[b, h * G:(h + 1) * G] = torch.softmax(s, -1) @ v[:, h]
+            heads = slice(h * G, (h + 1) * G)
+            seqs = slice(n * W, (n + 1) * W)
+            o, m = attend(q[seqs, heads, 0].reshape(W * G, D), ks[:, h], vs[:, h])
+            out[seqs, heads], lse[seqs, heads] = o.view(W, G, D), m.view(W, G)
+    for b in range(B):
+        ks, vs = (tokens(p, bt[b], int(sl[b])) for p in (kp, vp))
+        for h in range(Hkv if len(ks) else 0):
+            heads = slice(h * G, (h + 1) * G)
+            o, m = attend(q[b, heads, 0], ks[:, h], vs[:, h])
+            both = torch.logaddexp(lse[b, heads], m)
+            out[b, heads] = (out[b, heads] * (lse[b, heads] - both).exp().unsqueeze(-1)
+                             + o * (m - both).exp().unsqueeze(-1))
+            lse[b, heads] = both
     return out, lse
 
 

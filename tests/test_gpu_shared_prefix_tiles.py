@@ -3,8 +3,8 @@ buffers take turns and whose reference maxima move, against the definition in 64
 import pytest
 import torch
 
-from test_gpu_shared_prefix import BF16, F32, make, run
-from test_gpu_shared_prefix_accuracy import definition
+from test_gpu_shared_prefix import BF16, F16, F32, make, run
+from test_gpu_shared_prefix_accuracy import check_rounding, definition
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,53 @@ def test_rows_without_a_score_keep_no_reference(cuda, W, dtype):
     half = torch.finfo(dtype).eps / 2
     err = (got[0].double().cpu().reshape(want.shape) - want).abs()
     assert (err <= half * want.abs() + 1e-3 * vp.nan_to_num(0.0).abs().max()).all()
+
+
+# beams of 4 heads (rows of a prefix: 40, 64: tiles of 64 rows; 72, 128, 136: of 128), then
+# head_dim, type and tiles of a range
+WIDTHS = [10, 16, 18, 32, 34]
+FORMS = [(64, BF16, 3), (64, F16, 5), (72, BF16, 4), (72, F16, 3), (128, BF16, 5), (128, F16, 6), (64, BF16, 2),
+         (128, BF16, 1)]
+
+
+def tiled(W, D, dtype, tiles, P=64, seed=0):
+    """One prompt whose ranges hold `tiles` tiles, the last one less, and short own tokens."""
+    length = 64 * 64 * tiles - 100 if tiles > 1 else 64
+    args = make(1, W, 4, 1, D, P, [length], [(7 * i) % 40 for i in range(W)], dtype, seed=seed)
+    each = range_tokens(args[0], args[3], args[1], length)
+    assert each == tiles * 64
+    return args
+
+
+@pytest.mark.parametrize("D,dtype,tiles", FORMS)
+@pytest.mark.parametrize("W", WIDTHS)
+def test_ranges_of_several_tiles(cuda, W, D, dtype, tiles):
+    args = tiled(W, D, dtype, tiles, P=16 if W == 16 else 64, seed=W + tiles)
+    check_rounding(args, run(args, cuda))
+
+
+@pytest.mark.parametrize("D,dtype,tiles", FORMS[:-1])
+@pytest.mark.parametrize("W", WIDTHS)
+def test_scores_that_rise_in_every_tile(cuda, W, D, dtype, tiles):
+    """By 8 nats a tile, 2^11.5 in the weights: the reference maximum has to move each time."""
+    q, kp, vp, pt, pl, bt, sl = tiled(W, D, dtype, tiles)
+    q = (torch.ones_like(q) + 0.1 * torch.randn(q.shape, generator=torch.Generator().manual_seed(W))).to(dtype)
+    for i, page in enumerate(pt[0].tolist()):
+        rise = 8.0 * (i % tiles) * D ** -0.5
+        kp[page] = torch.where(kp[page].isnan(), kp[page], (kp[page] + rise).to(dtype))
+    args = (q, kp, vp, pt, pl, bt, sl)
+    check_rounding(args, run(args, cuda))
+
+
+@pytest.mark.parametrize("P", [16, 64])
+@pytest.mark.parametrize("D,dtype,tiles", FORMS[:-2])
+@pytest.mark.parametrize("W", [10, 34])
+def test_pages_outside_the_pool(cuda, W, D, dtype, tiles, P):
+    """Entries outside the pool: a range's first tile, its last, a whole range, single pages."""
+    args = tiled(W, D, dtype, tiles, P)
+    pt, pages, per = args[3], args[1].shape[0], 64 // P
+    for first, count in ((0, 1), (tiles - 1, 1), (tiles, tiles), (4 * tiles + 1, tiles - 1)):
+        pt[0, first * per:(first + count) * per] = -1
+    pt[0, 3::7 * per + 1] = pages
+    pt[0, 5::11 * per + 2] = 2 ** 31 - 1
+    check_rounding(args, run(args, cuda))
