@@ -191,7 +191,7 @@ __device__ __forceinline__ void put_part(P* to, X from) {
 enum : int { kBeamOrdinary = 0, kBeamFinished, kBeamEmpty, kBeamUndefined };
 
 // kMergeThreads threads, room for kMergeCap gathered candidates. JOIN: the chunks' parts
-// were written by other workgroups of this launch.
+// were written by other workgroups of this launch, and there are few of them.
 template <int kMergeThreads, int kMergeCap, bool JOIN>
 __device__ __forceinline__ void beam_merge(const SelectArgs& a, int64_t n) {
   constexpr int kMergeWaves = kMergeThreads / 64;
@@ -214,7 +214,7 @@ __device__ __forceinline__ void beam_merge(const SelectArgs& a, int64_t n) {
   // loaded before the sums are joined; else a list's first and last, and of the rest
   // only those of lists that turn out to matter.
   constexpr int kHeld = kHeldCandidates / kMergeThreads;
-  const bool few = lists * K <= kHeld * kMergeThreads;
+  const bool few = JOIN || lists * K <= kHeld * kMergeThreads;  // (launch_select's rule)
   uint64_t held[kHeld];
   int held_l[kHeld], held_k[kHeld];
   if (few) {
