@@ -200,3 +200,26 @@ def test_one_beam_of_many_chunks(cuda, dtype):
         x = (torch.randn(1, 1, V, generator=g, device=cuda) * 3).to(dtype)
         for count in (1, 64):
             check_large(x, torch.full((1, 1), -2.0, device=cuda), count)
+
+
+@pytest.mark.parametrize("dead", [-1e9, -1e30, torch.finfo(F32).min])
+@pytest.mark.parametrize("W,V", [(4, 3000), (40, 20000)])
+def test_beams_switched_off_by_a_large_score(cuda, W, V, dead):
+    """Beams at a large negative score, as masks write it, beside a live one with few tokens left:
+    the live tokens first, then as many others as are wanted, each once, at their beam's score."""
+    from llm_cuda.kernels.beam_search import beam_select
+
+    x, _ = make(1, W, V, F32, V)
+    x[0, 0, 5:] = -INF
+    s = torch.full((1, W), dead)
+    s[0, 0] = -1.0
+    best, tokens, parents = (t.cpu() for t in beam_select(x.to(cuda), s.to(cuda), num_candidates=32))
+    live = torch.log_softmax(x[0, 0, :5].double(), 0) - 1.0
+    want, order = live.sort(descending=True)
+    assert torch.equal(tokens[0, :5], order) and not parents[0, :5].any()
+    assert (best[0, :5].double() - want).abs().max() <= 2e-6
+    assert (parents[0, 5:] > 0).all() and len(set(zip(parents[0].tolist(), tokens[0].tolist()))) == 32
+    value = dead + torch.log_softmax(x[0].double(), -1)[parents[0, 5:], tokens[0, 5:]]
+    assert ((best[0, 5:].double() - value).abs() <= 1e-6 + 2 ** -24 * value.abs()).all()
+    top = (dead + torch.log_softmax(x[0, 1:].double(), -1)).flatten().topk(27).values
+    assert ((best[0, 5:].double() - top).abs() <= 1e-6 + 2 ** -24 * top.abs()).all()
