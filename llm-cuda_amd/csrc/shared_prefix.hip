@@ -803,14 +803,20 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
 // all ranges of their rows, a thread per 4 columns. Which workgroup that is changes
 // nothing in the sums, which equal shared_merge_kernel's bit for bit.
 //
-// The GPU takes longer so (4 beams of 1000 tokens: 12.8 us for 6.9 + 3.8 in two
-// launches; 20 with fences, which write the whole L2 back, in place of write-through
-// partials), but the host, which such a call waits for, loses a launch: 17.4 -> 14.9
-// us a call. Where K and V are more than kJoinRead bytes the GPU is what counts (4
-// groups of 8 x 4224 tokens, 69 MB: 22.2 us in two launches, 29.2 in one).
+// The GPU takes longer so (4 beams of 1000 tokens: 13.1 us for 11.1 in two launches; 20
+// with fences, which write the whole L2 back, in place of write-through partials), but
+// the host, which such a call waits for, loses a launch. Eager calls, us, joined / in
+// two launches (in brackets on the GPU):
+//   8B heads, 4 x 4 beams, K and V 12 MB 15.1 / 17.1 (13.2 / 11.2), 21 MB 15.9 / 16.8,
+//     29 MB 16.7 / 16.8, 37 MB 18.5 / 16.8, 70 MB 21.8 / 20.6
+//   16/8 heads of 64, 8 x 4 beams, 6 to 53 MB 15.0 / 16.9
+// The joining workgroup takes two rounds for 16 rows of 128 there; four rounds (8B, 4 x
+// 8 beams) are no gain, 8 MB 16.7 / 17.1 and 17 MB 19.5 / 17.0, and eight (70B, 2 x 8
+// beams) lose, 5.5 MB 20.9 / 17.0.
 constexpr int kJoinRanges = 16;             // most ranges per row
 constexpr int64_t kJoinBytes = 96 << 10;    // most partials of a group and kv head
 constexpr int64_t kJoinRead = 16 << 20;     // most bytes of K and V, by the tables' widths
+constexpr int64_t kJoinOutputs = 2048;      // most outputs of a group and kv head
 constexpr int kJoinCounters = 4096;
 
 template <typename T>
@@ -1197,8 +1203,11 @@ struct SharedPlan {
 // No range is shorter than two tiles.
 // A range of a sequence's own tokens is shared by 4, 2 or 1 waves: one wave has no
 // join at the end and a longer run of steps, which pays with many short ranges
-// (256 x 200 tokens: 102 / 92 / 87 us with 4 / 2 / 1 waves; 64 x 625: 56 / 57 / 61);
-// where the ranges are few, four finish sooner.
+// (behind 1024 tokens, us with 4 / 2 / 1 waves: 8B heads, 256 x 40 tokens 47 / 37 / 35, 64
+// x 200 27.5 / 27.9 / 24.5, 64 x 800 49 / 49 / 51, 64 x 1600 81 / 83 / 87; 16/8 heads of 64,
+// 200 x 200 33 / 28 / 24, 64 x 1600 47 / 45 / 63); where the ranges are few, four finish
+// sooner (8B, 16 x 100: 13.1 / 14.2 / 16.2). Of 43 such sizes the rule takes the fastest,
+// within 5%, at 39; at the others it loses up to 13% (70B heads, 64 x 100: 28.9 for 25.6).
 SharedPlan shared_plan(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t p_cap,
                        int64_t s_cap, int dtype) {
   if (B == 0) return SharedPlan{1, 4, 0, 0};
@@ -1291,7 +1300,8 @@ int launch_shared(SharedArgs a, int wr, int own_waves, bool mfma, int32_t* count
   const int64_t expected = tiles * a.p_splits + (int64_t)a.W * lc_cdiv(a.G, 32) * a.s_splits;
   const int64_t units = (int64_t)(a.B / a.W) * a.Hkv;
   const bool join = counters != nullptr && mfma && own_waves == 4 && splits > 0 &&
-                    splits <= kJoinRanges && rows * splits * a.D * 4 <= kJoinBytes &&
+                    splits <= kJoinRanges && rows * a.D <= kJoinOutputs &&
+                    rows * splits * a.D * 4 <= kJoinBytes &&
                     units <= kJoinCounters && units * expected <= 2 * lc_cu_count() &&
                     units * ((int64_t)a.p_pages + (int64_t)a.W * a.s_pages) * a.P * a.D * 2 *
                             (int64_t)sizeof(T) <= kJoinRead;
