@@ -167,8 +167,8 @@ __global__ __launch_bounds__(64) void shared_generic_kernel(SharedArgs a) {
 // chunk of a DMA; lanes whose token is past the range, whose page entry is invalid
 // or whose chunk is past head_dim read zeros instead, and their scores are masked.
 // The matrix instructions take the weights P in the data type, so each goes there as
-// two values of it, the rounded weight and what that rounding left (which keeps 2^-16
-// of a bf16 weight, 2^-22 of an f16 one, down to 2^-25); their sum stays in fp32. The
+// two values of it, the weight cut off and what that left (to 2^-15 of a bf16 weight,
+// 2^-21 of an f16 one, down to 2^-25); their sum stays in fp32. The
 // rounded weight alone would leave an error as large as the output's own rounding,
 // for values without a common mean average the output down as much as the errors
 // (8448 bf16 tokens: 2.3e-3 rms of the output, 1.66e-3 with both, which is the
@@ -181,13 +181,27 @@ constexpr float kSharedRescaleLog2 = 8.0f;
 
 __device__ __attribute__((aligned(16))) const uint32_t shared_zeros[4] = {0, 0, 0, 0};
 
-// A weight as a value of the data type and what its rounding left, rounded in turn.
+// Two weights, each as a value of the data type below it and what is left, rounded.
+// Both parts of a weight above 0 are above 0, so that an infinite V stays infinite (a
+// remainder of 0 or of the other sign would make it NaN).
 template <typename V>
-__device__ __forceinline__ void split_weight(float p, V& whole, V& rest, int i) {
+__device__ __forceinline__ void split_weights(float p0, float p1, V& whole, V& rest, int i) {
   typedef std::remove_reference_t<decltype(whole[0])> T;
-  const T w = static_cast<T>(p);
-  whole[i] = w;
-  rest[i] = static_cast<T>(p - static_cast<float>(w));
+  // (the next number below; 0 and a remainder of 0 for 0)
+  const uint32_t u0 = __builtin_elementwise_sub_sat(__float_as_uint(p0), 1u),
+                 u1 = __builtin_elementwise_sub_sat(__float_as_uint(p1), 1u);
+  if constexpr (std::is_same_v<T, bf16_t>) {
+    whole[i] = __builtin_bit_cast(T, static_cast<uint16_t>(u0 >> 16));
+    whole[i + 1] = __builtin_bit_cast(T, static_cast<uint16_t>(u1 >> 16));
+    rest[i] = static_cast<T>(p0 - __uint_as_float(u0 & 0xffff0000u));
+    rest[i + 1] = static_cast<T>(p1 - __uint_as_float(u1 & 0xffff0000u));
+  } else {
+    const auto w = __builtin_amdgcn_cvt_pkrtz(__uint_as_float(u0), __uint_as_float(u1));
+    whole[i] = static_cast<T>(w[0]);
+    whole[i + 1] = static_cast<T>(w[1]);
+    rest[i] = static_cast<T>(p0 - static_cast<float>(w[0]));
+    rest[i + 1] = static_cast<T>(p1 - static_cast<float>(w[1]));
+  }
 }
 
 struct RangeItem {
@@ -450,10 +464,11 @@ __device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeIte
 #pragma unroll
     for (int kt = 0; kt < NKT; ++kt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = lc_exp2(y[kt][r]);
-        if (r & 1) s1 += p; else s0 += p;
-        split_weight(p, pop[kt][r >> 3], rem[kt][r >> 3], r & 7);
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = lc_exp2(y[kt][r]), p1 = lc_exp2(y[kt][r + 1]);
+        s0 += p0;
+        s1 += p1;
+        split_weights(p0, p1, pop[kt][r >> 3], rem[kt][r >> 3], r & 7);
       }
     l_tile = s0 + s1;
   };
@@ -725,10 +740,11 @@ __device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeIt
     const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
     v8 pop[2], rem[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float p = lc_exp2(x[r] - m_use);
-      l_lane += p;
-      split_weight(p, pop[r >> 3], rem[r >> 3], r & 7);
+    for (int r = 0; r < 16; r += 2) {
+      const float p0 = lc_exp2(x[r] - m_use), p1 = lc_exp2(x[r + 1] - m_use);
+      l_lane += p0;
+      l_lane += p1;
+      split_weights(p0, p1, pop[r >> 3], rem[r >> 3], r & 7);
     }
 #pragma unroll
     for (int jp = 0; jp < 2; ++jp)

@@ -92,3 +92,21 @@ def test_outputs_are_rounded_once(cuda, W, Hq, Hkv, D, dtype):
 def test_own_tokens_alone_are_rounded_once(cuda, dtype):
     args = make(4, 3, 8, 2, 128, 32, [0] * 4, [300 + 117 * i for i in range(12)], dtype)
     check_rounding(args, run(args, cuda))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, torch.float32])
+@pytest.mark.parametrize("W,Hq,Hkv,D", [(4, 8, 2, 64), (12, 8, 2, 128), (40, 8, 2, 64)])
+def test_infinite_values_stay_infinite(cuda, W, Hq, Hkv, D, dtype):
+    """An infinite V entry makes that element of its sequences infinite, not NaN: every weight is
+    above 0. (A score at the maximum among them, whose weight has no remainder.)"""
+    args = make(1, W, Hq, Hkv, D, 16, [200], [(5 * i) % 37 for i in range(W)], dtype, seed=W)
+    q, kp, vp, pt, pl, bt, sl = args
+    kp[int(pt[0, 1])] = 0  # (equal scores)
+    vp[int(pt[0, 1]), 0, :4, 3] = math.inf
+    vp[int(pt[0, 5]), 1, 7, 5] = -math.inf
+    vp[int(bt[3, 0]), 0, 2, 9] = math.inf  # 15 tokens
+    out = run(args, cuda)[0].cpu().view(W, Hkv, Hq // Hkv, D)
+    want = definition(*args)[0].view(out.shape)
+    assert torch.equal(torch.isposinf(out), torch.isposinf(want)) and torch.isposinf(want).any()
+    assert torch.equal(torch.isneginf(out), torch.isneginf(want)) and torch.isneginf(want).any()
+    assert not out.isnan().any()
