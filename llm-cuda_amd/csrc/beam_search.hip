@@ -26,9 +26,10 @@ namespace {
 // (order-preserving bits of the logit, inverted index): all are different, and ties
 // rank by index.
 //
-// Bound: HBM for many rows (256 rows of 128256 fp32, 131 MB: chunks 29 us, join 10.6),
-// the latency of two dependent passes for few (4 rows of 32000: 5.2 + 6.3 us; what
-// the host takes for the call, 15 us, is longer).
+// Bound: for many rows the instructions beside the loads (256 rows of 128256 fp32, 131
+// MB: chunks 27.7 us, 4.7 TB/s, where a read stream reaches 6.9; join 10.7), for few the
+// latency of two dependent passes (4 rows of 32000: 5.2 + 6.3 us; what the host takes for
+// the call, 15 us, is longer).
 //
 // The order of candidates of different beams hangs on their lse: the terms of
 // its sum are fp32 (v_exp_f32 of exact or once-rounded differences), added in
@@ -772,7 +773,7 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs& a) {
   }
 }
 
-// (8 waves per SIMD: 256 rows of 128256 fp32, 131 MB, take 29 us, 4.5 TB/s; 32 with 5)
+// (8 waves per SIMD: 256 rows of 128256 fp32, 131 MB, take 27.7 us, 4.7 TB/s; 31.3 with 5)
 template <typename T, int ITEMS>
 __global__ __launch_bounds__(kBeamThreads, 8) void beam_chunk_kernel(SelectArgs a) {
   beam_chunk<T, ITEMS, false>(a);
@@ -780,9 +781,11 @@ __global__ __launch_bounds__(kBeamThreads, 8) void beam_chunk_kernel(SelectArgs 
 
 // Few beams and candidates: the workgroup of a group that finishes last (its ticket on
 // counters[n], zero at entry and left zero) joins the chunks, in the same launch. The
-// GPU takes as long as in two (4 beams of 32000: 11.0 us for 5.2 + 6.3; 16 of 1003:
-// 12.2 for 7.7 + 6.7; 32 of 2000: 15.3 for 7.4 + 7.1), and the host, which such a call
-// waits for, a launch less: 17.2 -> 15.4 us a call.
+// GPU takes about as long as in two (calls in a graph, us: 4 beams of 32000 10.7 / 11.2, 16
+// of 1003 11.9 / 12.4, 32 of 2000 15.4 / 13.5, 8 groups of 4 x 32000 15.9 / 12.1), and the
+// host, which such a call waits for, a launch less: 17.4 -> 15.4 us a call. Of 23 sizes
+// of 1 to 60 groups, 1 to 32 beams and 1000 to 128256 tokens the joined call is 0.5 to 2.4
+// us shorter at 22; with 32 beams and 64 candidates it is 0.5 us longer.
 template <typename T>
 __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(SelectArgs a) {
   __shared__ int last;

@@ -13,9 +13,9 @@
 // that finishes last).
 //
 // Bound: reading K and V once (4 groups of 8 x (4096 + 128) tokens, 8B heads: 84 MB in
-// 19.5 us + merge 3.9; 64 x (8192 + 625): 200 MB in 47 + 5.9), until a prefix has some
-// 300 rows per kv head, from where it is the matrix rate (256 x (8192 + 200): 71 + 8.5
-// us, 470 TFLOP/s).
+// 19.8 us + merge 3.9; 64 x (8192 + 625): 200 MB in 48.8 + 5.9), until a prefix has some
+// 130 rows per kv head, from where it is the matrix rate (256 x (8192 + 200): 77 to 80 +
+// 8.2 us, 400 TFLOP/s of QK and one PV in all).
 #include <math.h>
 
 #include "attn_f32.h"
@@ -168,13 +168,13 @@ __global__ __launch_bounds__(64) void shared_generic_kernel(SharedArgs a) {
 // or whose chunk is past head_dim read zeros instead, and their scores are masked.
 // The matrix instructions take the weights P in the data type, so each goes there as
 // two values of it, the weight cut off and what that left (to 2^-15 of a bf16 weight,
-// 2^-21 of an f16 one, down to 2^-25); their sum stays in fp32. The
-// rounded weight alone would leave an error as large as the output's own rounding,
-// for values without a common mean average the output down as much as the errors
-// (8448 bf16 tokens: 2.3e-3 rms of the output, 1.66e-3 with both, which is the
-// output's rounding). The second value is free where K and V are streamed (4 groups
-// of 8 x 4224: 22.4 us either way); where a prefix has many rows, PV is twice the
-// matrix work: 64 x (8192 + 625) 52 -> 56 us, 256 x (8192 + 200) 76 -> 86.
+// 2^-21 of an f16 one, down to 2^-25); their sum stays in fp32. A rounded weight alone
+// would leave an error as large as the output's own rounding, for values without a
+// common mean average the output down as much as the errors (8448 bf16 tokens: 2.3e-3
+// rms of the output, 1.66e-3 with both, which is the output's rounding). The second
+// value is free where K and V are streamed (4 groups of 8 x 4224, a call in a graph:
+// 22.2 -> 22.7 us); where a prefix has many rows, PV is twice the matrix work: 64 x
+// (8192 + 625) 52 -> 56 us, 256 x (8192 + 200) 75 -> 86.
 // ---------------------------------------------------------------------------
 constexpr int kTile = 64;  // tokens per tile
 constexpr float kSharedRescaleLog2 = 8.0f;
