@@ -538,9 +538,11 @@ LC_API int64_t lc_beam_select_workspace_bytes(int64_t groups, int64_t width, int
  *   value(w, v) = s[w] + x[w, v] - ln sum_u exp(x[w, u])
  * and out_scores (fp32), out_tokens (v) and out_parents (w), int64, all
  * contiguous [groups, count], hold the largest values, largest first, ties by
- * the lowest w * vocab + v. Values are formed and compared in 64 bits; where a
- * score is so large that different logits of its beam give equal ones (below |s| *
- * 2^-53 apart: beside -1e9, 1e-7), any of those may stand for the others.
+ * the lowest w * vocab + v. Values are formed and compared in 64 bits, from sums of
+ * fp32 terms: those of beams with other logits may rank either way where they are
+ * within 1e-6 of each other (beams of equal logits have equal sums). Where a score is
+ * so large that different logits of its beam give equal values (below |s| * 2^-53
+ * apart: beside -1e9, 1e-7), any of those may stand for the others.
  * finished (uint8 [groups, width], may be NULL): a beam that is set has one
  * continuation, the token eos at the beam's own score (its logits are not
  * read); its other tokens have -inf. out_finished (uint8 [groups, count], may

@@ -1483,12 +1483,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_candidates: int 
     beams' summed log-probabilities. Returns (scores fp32, tokens int64, parents
     int64), each [N, K] with K = num_candidates (W by default; at most 64): the
     largest scores[n, w] + log_softmax(logits[n, w])[v], largest first, ties by
-    the lowest w * V + v (values in 64 bits: beside a score of -1e9, logits within 1e-7
-    are equal, and any of them may stand for the others). With finished (bool [N, W];
-    needs eos_token_id) a finished beam's only continuation is eos_token_id at its own
-    score, and a fourth tensor, bool [N, K], says which results are finished. A beam
-    with no logit above -inf or a score of -inf has continuations of -inf; NaN or +inf
-    in its logits or score gives NaN, which ranks first.
+    the lowest w * V + v. Values are 64-bit ones from sums of fp32 terms: of beams with
+    other logits those within 1e-6 of each other may rank either way, and of logits that
+    a large score makes equal (beside -1e9, those within 1e-7) any may stand for the
+    others. With finished (bool [N, W]; needs eos_token_id) a finished beam's only
+    continuation is eos_token_id at its own score, and a fourth tensor, bool [N, K],
+    says which results are finished. A beam with no logit above -inf or a score of -inf
+    has continuations of -inf; NaN or +inf in its logits or score gives NaN, which ranks
+    first.
     """
     if _records_grad(logits, scores):
         return _ForwardOnly.apply(
