@@ -592,6 +592,131 @@ LC_API int lc_paged_kv_reorder(void* key_pages, void* value_pages, int64_t kv_s_
                                const int64_t* parents, int64_t groups, int64_t width, int64_t Hkv,
                                int64_t D, int64_t page_size, int dtype, void* stream);
 
+/* Bytes of workspace lc_paged_extend_fwd needs (fp32 outputs and logsumexps of the
+ * token ranges); capacity: table width x page size. -1 for invalid sizes. */
+LC_API int64_t lc_paged_extend_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                                               int64_t D, int64_t capacity, int dtype);
+
+/* GQA attention of the newest tokens of every sequence over the paged KV cache.
+ * Sequence b holds L = seq_lens[b] tokens, of which the last n = query_lens[b] are
+ * its queries: query i < n stands at position p = L - n + i and sees tokens 0 .. p,
+ *   out[b,h,i,:] = softmax(q[b,h,i,:] . K_b[0..p]^T * scale) V_b[0..p]
+ * lse[b,h,i] (fp32, contiguous [B, Hq, T], may be NULL): natural-log logsumexp of the
+ * scaled scores. Rows i >= n, and rows with p < 0, give out = 0, lse = -inf. Tokens
+ * that a row does not see have no part in it, whatever K and V hold there.
+ * No counterpart in the reference, whose decode takes one token
+ * (kernels/triton/decode_attention.py:204-287) and whose chunks copy the cache
+ * (models/llama3/kv_cache.py:65-83).
+ * q, out: [B, Hq, T, D] with (batch, head, token) strides. key_pages, value_pages:
+ *   [num_pages, Hkv, page_size, D] pools with shared strides; block_table int32 [B,
+ *   max_pages_per_seq] (0 wide allowed); entries outside [0, num_pages) are never
+ *   dereferenced (their tokens are skipped). seq_lens int32 [B] (clamped to the
+ *   table's capacity), query_lens int32 [B] or NULL (T for all; clamped to [0, T]).
+ * workspace: >= lc_paged_extend_workspace_bytes, 256-byte aligned; calls that may
+ *   overlap need their own. */
+LC_API int lc_paged_extend_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+                               const void* key_pages, const void* value_pages, int64_t kv_s_page,
+                               int64_t kv_s_head, int64_t kv_s_tok, int64_t num_pages,
+                               const int32_t* block_table, int64_t bt_stride,
+                               int64_t max_pages_per_seq, const int32_t* seq_lens,
+                               const int32_t* query_lens, void* out, int64_t o_sb, int64_t o_sh,
+                               int64_t o_st, float* lse, void* workspace, int64_t workspace_bytes,
+                               int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                               int64_t page_size, float scale, int dtype, void* stream);
+
+/* Bytes of workspace lc_verify_draft_tokens needs, or -1 for invalid sizes. */
+LC_API int64_t lc_verify_draft_tokens_workspace_bytes(int64_t B, int64_t drafts, int64_t vocab);
+
+/* Speculative decoding's verification: which of a sequence's n = draft_lens[b] drafted
+ * tokens d stand, and the token after them, from given random numbers. With
+ *   p_i = softmax(logits[b, i] / t),  q_i = softmax(draft_logits[b, i] / t)
+ * (draft_logits NULL: q_i is 1 at d_i), draft i stands iff all before it do and
+ * uniforms[b, i] * q_i(d_i) < p_i(d_i). With a drafts standing the next token is the
+ * first v whose running sum of w passes uniforms[b, drafts] times the sum of w, w =
+ * p_a, or max(p_a - q_a, 0) where draft a < n was refused (p_a where that sums to
+ * less than 2^-32: then p and q agree). A temperature t that is not a positive finite
+ * number, or a row whose largest logit is not finite, stands for all mass on the row's
+ * first largest logit (NaN is the largest). Sums that choose a token are formed in 64
+ * bits; those of p_i(d_i) and q_i(d_i) from fp32 terms (to 1e-6 relative).
+ *   tokens int64 [B, drafts + 1]: the drafts that stand, the new token, then -1
+ *   accepted int32 [B]: a
+ * logits [B, drafts + 1, vocab], draft_logits [B, drafts, vocab], unit stride over
+ * vocab, (batch, row) strides given; rows past a sequence's drafts are not read.
+ * draft_tokens int64 [B, drafts] (one outside the vocabulary is refused); uniforms
+ * fp32 [B, drafts + 1] in [0, 1); draft_lens int32 [B] (clamped to [0, drafts]) or
+ * NULL (drafts for all); temperatures fp32 [B] or NULL: `temperature` for all.
+ * drafts < 256. workspace: 256-byte aligned; calls that may overlap need their own.
+ * No counterpart in the reference (models/llama3/model.py:200-218). */
+LC_API int lc_verify_draft_tokens(const void* logits, int64_t l_sb, int64_t l_si,
+                                  const void* draft_logits, int64_t d_sb, int64_t d_si,
+                                  const int64_t* draft_tokens, const float* uniforms,
+                                  const int32_t* draft_lens, const float* temperatures,
+                                  double temperature, int64_t B, int64_t drafts, int64_t vocab,
+                                  int64_t* tokens, int32_t* accepted, void* workspace,
+                                  int64_t workspace_bytes, int dtype, void* stream);
+
+/* Pages of a pool. page_refs int32 [num_pages] counts the block-table entries that name
+ * a page; a page whose count is 0 is free. The three entries below read a table,
+ * lengths and counts and write new ones (contiguous, in other buffers); K and V slots
+ * are copied in the pools, in every layer, and only into pages that are free in
+ * page_refs, so until the new table and counts are taken nothing has changed that the
+ * old ones name (compaction's old table stays right as well). Conventions of all three:
+ * key_pages, value_pages [layers, num_pages, Hkv, page_size, D] pools with shared
+ * strides (head_dim contiguous), one table for all layers; block_table int32 rows of
+ * max_pages_per_seq entries, bt_stride apart; lengths int32, clamped to [0, capacity]. A
+ * row of length L holds its first ceil(L / page_size) entries, whatever the others say;
+ * entries of new tables that are not held are -1. Entries outside [0, num_pages) are
+ * passed on and counted nowhere. `missing` (int32 [1]): how many pages were asked for
+ * beyond those free; such entries are -1, and the result should not be taken.
+ * Workspace: as lc_*_workspace_bytes says (-1 for invalid sizes), 256-byte aligned;
+ * calls that may overlap need their own. No counterpart in the reference, whose cache
+ * owns fixed pages (models/llama3/kv_cache.py:21-36).
+ *
+ * Resize: row b goes from length seq_lens[b] to new_lens[b]. Entries that it needs more
+ * are the lowest free pages, in the order of rows and columns; entries that it gives up
+ * lose a reference. A row that grows out of a page that is partly filled and has other
+ * references too (count above 1) takes a page of its own for it (in its column's place
+ * of that order), into which its filled slots are copied. */
+LC_API int64_t lc_paged_kv_resize_workspace_bytes(int64_t B, int64_t max_pages_per_seq,
+                                                  int64_t num_pages);
+LC_API int lc_paged_kv_resize(void* key_pages, void* value_pages, int64_t kv_s_layer,
+                              int64_t kv_s_page, int64_t kv_s_head, int64_t kv_s_tok,
+                              int64_t layers, int64_t num_pages, const int32_t* block_table,
+                              int64_t bt_stride, int64_t max_pages_per_seq,
+                              const int32_t* seq_lens, const int32_t* new_lens,
+                              const int32_t* page_refs, int32_t* out_table, int32_t* out_refs,
+                              int32_t* missing, void* workspace, int64_t workspace_bytes,
+                              int64_t B, int64_t Hkv, int64_t D, int64_t page_size, int dtype,
+                              void* stream);
+
+/* Fork: row r of the new table ([children, max_pages_per_seq]) continues row parents[r]
+ * of the old one ([B, ...]); a parent outside [0, B) makes an empty row. Whole pages are
+ * shared. The page that a row is filling stays with its first child; its other children
+ * take the lowest free pages, in row order, and copies of the filled slots. The old rows'
+ * references end. out_lens int32 [children]. */
+LC_API int64_t lc_paged_kv_fork_workspace_bytes(int64_t B, int64_t children, int64_t num_pages);
+LC_API int lc_paged_kv_fork(void* key_pages, void* value_pages, int64_t kv_s_layer,
+                            int64_t kv_s_page, int64_t kv_s_head, int64_t kv_s_tok, int64_t layers,
+                            int64_t num_pages, const int32_t* block_table, int64_t bt_stride,
+                            int64_t max_pages_per_seq, const int32_t* seq_lens,
+                            const int64_t* parents, const int32_t* page_refs, int32_t* out_table,
+                            int32_t* out_lens, int32_t* out_refs, int32_t* missing,
+                            void* workspace, int64_t workspace_bytes, int64_t B, int64_t children,
+                            int64_t Hkv, int64_t D, int64_t page_size, int dtype, void* stream);
+
+/* Compaction: with n pages in use (count not 0), those with an index of n or more move,
+ * in order, into the free pages below n, in order. page_map int32 [num_pages]: each
+ * page's new index, -1 for a free one (other holders of pages look theirs up there). */
+LC_API int64_t lc_paged_kv_compact_workspace_bytes(int64_t num_pages);
+LC_API int lc_paged_kv_compact(void* key_pages, void* value_pages, int64_t kv_s_layer,
+                               int64_t kv_s_page, int64_t kv_s_head, int64_t kv_s_tok,
+                               int64_t layers, int64_t num_pages, const int32_t* block_table,
+                               int64_t bt_stride, int64_t max_pages_per_seq,
+                               const int32_t* seq_lens, const int32_t* page_refs,
+                               int32_t* out_table, int32_t* out_refs, int32_t* page_map,
+                               void* workspace, int64_t workspace_bytes, int64_t B, int64_t Hkv,
+                               int64_t D, int64_t page_size, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,317 @@
+// GQA attention of the newest tokens of every sequence over the paged KV cache.
+//
+// Sequence b holds L tokens, n of which (n <= T) are its queries: query i stands at
+// position p = L - n + i and attends to tokens 0 .. p. A kv head's T G query rows (row
+// r = i G + g) share K and V; a tile of them takes tokens 0 .. its last row's p, cut
+// into `splits` equal ranges, whose normalised outputs and logsumexps a merge launch
+// joins:
+//   out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M),  M = max_i lse_i
+// (lse in log2 units).
+#include <math.h>
+
+#include "lc_common.h"
+
+namespace {
+
+struct ExtendArgs {
+  const void* q;
+  int64_t q_sb, q_sh, q_st;
+  const void* kp;
+  const void* vp;
+  int64_t s_page, s_head, s_tok;
+  const int32_t* table;  // [B, pages]
+  int64_t t_stride;
+  const int32_t* lens;   // [B]
+  const int32_t* qlens;  // [B] or null: T
+  void* out;
+  int64_t o_sb, o_sh, o_st;
+  float* lse;       // [B, Hq, T] or null
+  float* part_o;    // [B, Hq, T, splits, D]
+  float* part_lse;  // [B, Hq, T, splits], log2 units
+  int B, T, Hq, Hkv, G, D, P, p_shift, num_pages, pages, splits, tile_rows;
+  float scale_log2;
+};
+
+// Tokens of a range are a multiple of this.
+constexpr int kStep = 64;
+
+// Length and queries of a sequence.
+struct Seq {
+  int len, n;
+};
+__device__ __forceinline__ Seq sequence(const ExtendArgs& a, int b) {
+  const int cap = a.pages * a.P, len = a.lens[b];
+  const int n = a.qlens == nullptr ? a.T : a.qlens[b];
+  return Seq{len < 0 ? 0 : len > cap ? cap : len, n < 0 ? 0 : n > a.T ? a.T : n};
+}
+// Tokens that query i sees.
+__device__ __forceinline__ int visible(const Seq& s, int i) {
+  return i < s.n ? max(0, s.len - s.n + i + 1) : 0;
+}
+// Tokens that a tile of rows from row0 on needs: those of its last live row.
+__device__ __forceinline__ int tile_len(const ExtendArgs& a, const Seq& s, int row0) {
+  const int last = min(min(row0 + a.tile_rows, a.T * a.G) - 1, s.n * a.G - 1);
+  return last < row0 ? 0 : visible(s, last / a.G);
+}
+__device__ __forceinline__ int range_tokens(int len, int splits) {
+  const int each = (len + splits - 1) / splits;
+  return (each + kStep - 1) / kStep * kStep;
+}
+__device__ __forceinline__ int range_count(int len, int splits) {
+  if (len <= 0) return 0;
+  const int each = range_tokens(len, splits);
+  return (len + each - 1) / each;
+}
+
+// Element offset of token tok of a table row and kv head; -1 where its page entry
+// is invalid. tok is within the row's capacity.
+__device__ __forceinline__ int64_t token_offset(const ExtendArgs& a, const int32_t* row, int kvh,
+                                                int tok) {
+  const int page = a.p_shift >= 0 ? tok >> a.p_shift : tok / a.P;
+  const int slot = tok - page * a.P;
+  const int phys = row[page];
+  if (static_cast<unsigned>(phys) >= static_cast<unsigned>(a.num_pages)) return -1;
+  return (int64_t)phys * a.s_page + (int64_t)kvh * a.s_head + (int64_t)slot * a.s_tok;
+}
+
+// Generic kernel: one wave per (row, range), lanes across head_dim, one token at a
+// time. Any dtype, head_dim <= 256 and strides.
+template <typename T>
+__global__ __launch_bounds__(64) void extend_generic_kernel(ExtendArgs a) {
+  const int lane = threadIdx.x;
+  const int i = blockIdx.x % a.T, rest = blockIdx.x / a.T;
+  const int split = rest % a.splits, bh = rest / a.splits;
+  const int h = bh % a.Hq, b = bh / a.Hq;
+  const int kvh = h / a.G, r = i * a.G + h % a.G;
+  const Seq s = sequence(a, b);
+  const int len = tile_len(a, s, r / a.tile_rows * a.tile_rows);
+  const int each = range_tokens(len, a.splits);
+  const int t_begin = split * each;
+  if (t_begin >= len) return;
+  const int t_end = min(min(len, t_begin + each), visible(s, i));
+  const int32_t* row = a.table + (int64_t)b * a.t_stride;
+  const T* kp = static_cast<const T*>(a.kp);
+  const T* vp = static_cast<const T*>(a.vp);
+  const T* qh = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh +
+                (int64_t)i * a.q_st;
+
+  float qv[4], acc[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int d = lane + 64 * j;
+    qv[j] = d < a.D ? lc_to_f32(qh[d]) : 0.f;
+    acc[j] = 0.f;
+  }
+  float m_run = -INFINITY, l_run = 0.f;
+  for (int t = t_begin; t < t_end; ++t) {
+    const int64_t off = token_offset(a, row, kvh, t);
+    if (off < 0) continue;  // uniform across the wave
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = lane + 64 * j;
+      if (d < a.D) dot = fmaf(qv[j], lc_to_f32(kp[off + d]), dot);
+    }
+    const float x = lc_wave_sum(dot) * a.scale_log2;
+    if (x == -INFINITY) continue;
+    const float m_new = fmaxf(m_run, x);
+    const float alpha = lc_exp2(m_run - m_new);
+    const float p = lc_exp2(x - m_new);
+    l_run = l_run * alpha + p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = lane + 64 * j;
+      const float vv = d < a.D ? lc_to_f32(vp[off + d]) : 0.f;
+      acc[j] = fmaf(p, vv, acc[j] * alpha);
+    }
+    m_run = m_new;
+  }
+  const int64_t pidx = (((int64_t)b * a.Hq + h) * a.T + i) * a.splits + split;
+  const float inv_l = l_run > 0.f ? 1.0f / l_run : l_run;  // (NaN stays NaN)
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int d = lane + 64 * j;
+    if (d < a.D) a.part_o[pidx * a.D + d] = acc[j] * inv_l;
+  }
+  if (lane == 0) a.part_lse[pidx] = l_run == 0.f ? -INFINITY : m_run + lc_log2(l_run);
+}
+
+// Merge: one wave per row joins its tile's ranges; each lane owns VPL consecutive
+// floats of head_dim. A row that sees no token gets out = 0, lse = -inf.
+template <typename T, int VPL>
+__global__ __launch_bounds__(256) void extend_merge_kernel(ExtendArgs a, int64_t rows) {
+  constexpr int kBatch = 8;
+  const int lane = threadIdx.x & 63;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const int i = static_cast<int>(at % a.T);
+  const int64_t bh = at / a.T;
+  const int h = static_cast<int>(bh % a.Hq), b = static_cast<int>(bh / a.Hq);
+  const Seq s = sequence(a, b);
+  const int r = i * a.G + h % a.G;
+  const int n_all = visible(s, i) == 0
+                        ? 0
+                        : range_count(tile_len(a, s, r / a.tile_rows * a.tile_rows), a.splits);
+  const int d0 = lane * VPL, dl = d0 < a.D ? d0 : 0;
+  const float* part = a.part_o + at * a.splits * a.D + dl;
+  const float* plse = a.part_lse + at * a.splits;
+  float w = lane < n_all ? plse[lane] : -INFINITY;  // (splits <= 64)
+  float mx = lc_wave_max(w);
+  if (__ballot(w != w)) mx = NAN;
+  float acc[VPL], wsum = 0.f;
+#pragma unroll
+  for (int e = 0; e < VPL; ++e) acc[e] = 0.f;
+  if (mx != -INFINITY) {
+    w = lane < n_all ? lc_exp2(w - mx) : 0.f;
+    for (int j0 = 0; j0 < n_all; j0 += kBatch) {
+      float v[kBatch][VPL];
+#pragma unroll
+      for (int jj = 0; jj < kBatch; ++jj)
+#pragma unroll
+        for (int e = 0; e < VPL; ++e) v[jj][e] = part[(int64_t)min(j0 + jj, n_all - 1) * a.D + e];
+#pragma unroll
+      for (int jj = 0; jj < kBatch; ++jj) {
+        const float wj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(j0 + jj, 63)));
+        if (j0 + jj < n_all && wj != 0.f) {
+          wsum += wj;
+#pragma unroll
+          for (int e = 0; e < VPL; ++e) acc[e] = fmaf(wj, v[jj][e], acc[e]);
+        }
+      }
+    }
+  }
+  const float inv = wsum == 0.f ? 0.f : 1.0f / wsum;
+  T* oh = static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + (int64_t)i * a.o_st;
+#pragma unroll
+  for (int e = 0; e < VPL; ++e)
+    if (d0 + e < a.D) oh[d0 + e] = lc_from_f32<T>(acc[e] * inv);
+  if (a.lse != nullptr && lane == 0)
+    a.lse[at] = wsum == 0.f ? -INFINITY : (mx + lc_log2(wsum)) * kLn2;
+}
+
+struct ExtendPlan {
+  int tile_rows, splits;
+};
+ExtendPlan extend_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t cap) {
+  const int64_t units = B * Hq * T, cus = lc_cu_count();
+  int64_t s = units == 0 ? 1 : lc_cdiv(16 * cus, units);
+  const int64_t most = lc_cdiv(cap, 128);
+  s = s > most ? most : s;
+  return ExtendPlan{32, static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s)};
+}
+int64_t extend_bytes(int64_t rows, int64_t D, const ExtendPlan& p) {
+  const int64_t n = rows * p.splits;
+  return (n * D * 4 + 255) / 256 * 256 + n * 4;
+}
+
+template <typename T>
+int launch_extend(const ExtendArgs& a, hipStream_t st) {
+  static const char* who = "lc_paged_extend_fwd";
+  const int64_t rows = (int64_t)a.B * a.Hq * a.T;
+  extend_generic_kernel<T><<<static_cast<unsigned>(rows * a.splits), 64, 0, st>>>(a);
+  const int rc = lc_check_launch(who);
+  if (rc != LC_OK) return rc;
+  const unsigned blocks = static_cast<unsigned>(lc_cdiv(rows, 4));
+  if (a.D <= 64)
+    extend_merge_kernel<T, 1><<<blocks, 256, 0, st>>>(a, rows);
+  else if (a.D <= 128)
+    extend_merge_kernel<T, 2><<<blocks, 256, 0, st>>>(a, rows);
+  else
+    extend_merge_kernel<T, 4><<<blocks, 256, 0, st>>>(a, rows);
+  return lc_check_launch(who);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t lc_paged_extend_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                        int64_t capacity, int dtype) {
+  if (B < 0 || T < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || D <= 0 || capacity < 0) return -1;
+  return extend_bytes(B * Hq * T, D, extend_plan(B, T, Hq, Hkv, capacity));
+}
+
+int lc_paged_extend_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st,
+                        const void* key_pages, const void* value_pages, int64_t kv_s_page,
+                        int64_t kv_s_head, int64_t kv_s_tok, int64_t num_pages,
+                        const int32_t* block_table, int64_t bt_stride, int64_t max_pages_per_seq,
+                        const int32_t* seq_lens, const int32_t* query_lens, void* out,
+                        int64_t o_sb, int64_t o_sh, int64_t o_st, float* lse, void* workspace,
+                        int64_t workspace_bytes, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                        int64_t D, int64_t page_size, float scale, int dtype, void* stream) {
+  static const char* who = "lc_paged_extend_fwd";
+  LC_REQUIRE(B >= 0 && B < 65536 && T >= 0 && T < (1LL << 20), "%s: batch %lld of %lld queries",
+             who, (long long)B, (long long)T);
+  LC_REQUIRE(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq < 65536,
+             "%s: n_heads (%lld) must be a multiple of n_kv_heads (%lld)", who, (long long)Hq,
+             (long long)Hkv);
+  LC_REQUIRE(D > 0 && D <= 256, "%s: head_dim %lld not in [1, 256]", who, (long long)D);
+  LC_REQUIRE(dtype == LC_DTYPE_F32 || dtype == LC_DTYPE_F16 || dtype == LC_DTYPE_BF16,
+             "%s: unknown dtype %d", who, dtype);
+  if (B == 0 || T == 0) return LC_OK;
+  LC_REQUIRE(q && key_pages && value_pages && seq_lens && out && workspace, "%s: null pointer", who);
+  LC_REQUIRE(page_size > 0 && num_pages > 0 && num_pages < (1LL << 31) && max_pages_per_seq >= 0,
+             "%s: page_size and num_pages must be > 0, the table's width >= 0", who);
+  LC_REQUIRE(block_table || max_pages_per_seq == 0, "%s: null table", who);
+  LC_REQUIRE(max_pages_per_seq < (1LL << 30) / page_size, "%s: a table of 2^30 tokens or more", who);
+  LC_REQUIRE(bt_stride >= max_pages_per_seq, "%s: table stride < row length", who);
+  LC_REQUIRE(q_sb >= 0 && q_sh >= 0 && q_st >= 0 && o_sb >= 0 && o_sh >= 0 && o_st >= 0 &&
+                 kv_s_page >= 0 && kv_s_head >= 0 && kv_s_tok >= 0,
+             "%s: negative stride", who);
+  const ExtendPlan plan = extend_plan(B, T, Hq, Hkv, max_pages_per_seq * page_size);
+  LC_REQUIRE(B * Hq * T < (1LL << 26) / plan.splits, "%s: %lld query rows", who,
+             (long long)(B * Hq * T));
+  const int64_t need = extend_bytes(B * Hq * T, D, plan);
+  if (workspace_bytes < need)
+    return lc_fail(LC_EWORKSPACE, "%s: workspace %lld < %lld bytes", who,
+                   (long long)workspace_bytes, (long long)need);
+  LC_REQUIRE(lc_aligned(workspace, 256), "%s: workspace not 256-byte aligned", who);
+
+  ExtendArgs a{};
+  a.q = q;
+  a.q_sb = q_sb;
+  a.q_sh = q_sh;
+  a.q_st = q_st;
+  a.kp = key_pages;
+  a.vp = value_pages;
+  a.s_page = kv_s_page;
+  a.s_head = kv_s_head;
+  a.s_tok = kv_s_tok;
+  a.table = block_table;
+  a.t_stride = bt_stride;
+  a.lens = seq_lens;
+  a.qlens = query_lens;
+  a.out = out;
+  a.o_sb = o_sb;
+  a.o_sh = o_sh;
+  a.o_st = o_st;
+  a.lse = lse;
+  const int64_t n = B * Hq * T * plan.splits;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_lse =
+      reinterpret_cast<float*>(static_cast<char*>(workspace) + (n * D * 4 + 255) / 256 * 256);
+  a.B = static_cast<int>(B);
+  a.T = static_cast<int>(T);
+  a.Hq = static_cast<int>(Hq);
+  a.Hkv = static_cast<int>(Hkv);
+  a.G = static_cast<int>(Hq / Hkv);
+  a.D = static_cast<int>(D);
+  a.P = static_cast<int>(page_size);
+  a.p_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll(page_size) : -1;
+  a.num_pages = static_cast<int>(num_pages);
+  a.pages = static_cast<int>(max_pages_per_seq);
+  a.splits = plan.splits;
+  a.tile_rows = plan.tile_rows;
+  a.scale_log2 = scale * kLog2e;
+  hipStream_t st = lc_stream(stream);
+  switch (dtype) {
+    case LC_DTYPE_F32:
+      return launch_extend<float>(a, st);
+    case LC_DTYPE_BF16:
+      return launch_extend<bf16_t>(a, st);
+    default:
+      return launch_extend<f16_t>(a, st);
+  }
+}
+
+}  // extern "C"

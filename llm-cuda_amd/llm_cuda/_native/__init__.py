@@ -169,6 +169,37 @@ _SIGNATURES = {
         [_c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64,
          _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_p],
     ),
+    "lc_paged_extend_workspace_bytes": (_c_i64, [_c_i64] * 6 + [ctypes.c_int]),
+    "lc_paged_extend_fwd": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_i64, _c_p, _c_i64,
+         _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_i64, _c_i64, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, ctypes.c_int, _c_p],
+    ),
+    "lc_verify_draft_tokens_workspace_bytes": (_c_i64, [_c_i64] * 3),
+    "lc_verify_draft_tokens": (
+        ctypes.c_int,
+        [_c_p, _c_i64, _c_i64, _c_p, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_p, ctypes.c_double,
+         _c_i64, _c_i64, _c_i64, _c_p, _c_p, _c_p, _c_i64, ctypes.c_int, _c_p],
+    ),
+    "lc_paged_kv_resize_workspace_bytes": (_c_i64, [_c_i64] * 3),
+    "lc_paged_kv_resize": (
+        ctypes.c_int,
+        [_c_p, _c_p] + [_c_i64] * 6 + [_c_p, _c_i64, _c_i64] + [_c_p] * 7
+        + [_c_i64] * 5 + [ctypes.c_int, _c_p],
+    ),
+    "lc_paged_kv_fork_workspace_bytes": (_c_i64, [_c_i64] * 3),
+    "lc_paged_kv_fork": (
+        ctypes.c_int,
+        [_c_p, _c_p] + [_c_i64] * 6 + [_c_p, _c_i64, _c_i64] + [_c_p] * 8
+        + [_c_i64] * 6 + [ctypes.c_int, _c_p],
+    ),
+    "lc_paged_kv_compact_workspace_bytes": (_c_i64, [_c_i64]),
+    "lc_paged_kv_compact": (
+        ctypes.c_int,
+        [_c_p, _c_p] + [_c_i64] * 6 + [_c_p, _c_i64, _c_i64] + [_c_p] * 6
+        + [_c_i64] * 5 + [ctypes.c_int, _c_p],
+    ),
 }
 
 EXPORTS = tuple(_SIGNATURES)

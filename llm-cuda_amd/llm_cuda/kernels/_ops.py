@@ -1643,3 +1643,358 @@ def _reorder_sizes(k, v, ks, vs, block_table, seq_lens, parents):
     if N and not 1 <= W <= 256:
         raise ValueError(f"{W} beams: 1 to 256")
     return L, num_pages, Hkv, P, D, N, W, block_table[1], s_layer
+
+
+# ---------------------------------------------------------------------------
+# Speculative decoding: attention of the newest tokens, verification of drafts
+# (no counterpart in the reference, which decodes greedily: model.py:200-218)
+# ---------------------------------------------------------------------------
+def paged_extend(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                 block_table: torch.Tensor, seq_lens: torch.Tensor,
+                 query_lens: torch.Tensor | None = None, scale: float | None = None,
+                 return_lse: bool = False):
+    """GQA attention of the newest tokens of every sequence over a paged K/V pool (forward
+    only).
+
+    q [B, Hq, T, D]; key_pages, value_pages [num_pages, Hkv, P, D]; block_table int32 [B,
+    pages]; seq_lens int32 [B]: tokens that a sequence holds, its queries' own (appended
+    before the call) among them; query_lens int32 [B]: how many of its T rows are queries
+    (T for all by default). Query i < query_lens[b] stands at position seq_lens[b] -
+    query_lens[b] + i and sees the tokens up to there; other rows, and queries before the
+    first token, give zeros (lse -inf). Returns out with q's shape (and lse [B, Hq, T] fp32
+    if return_lse).
+    """
+    if _records_grad(q, key_pages, value_pages):
+        return _ForwardOnly.apply(
+            "paged_extend",
+            lambda a, k, v: _paged_extend(a, k, v, block_table, seq_lens, query_lens, scale,
+                                          return_lse), q, key_pages, value_pages)
+    return _paged_extend(q, key_pages, value_pages, block_table, seq_lens, query_lens, scale,
+                         return_lse)
+
+
+@functools.lru_cache(maxsize=1024)
+def _extend_sizes(q, k, v, block_table, seq_lens, query_lens, ks, vs, lc_dtype):
+    """Checks the shapes of a paged_extend call; (batch, heads, queries, head_dim, kv heads,
+    page size, pages of the pool, table width, workspace bytes, whether the pools' strides
+    do). A function of its arguments alone, run once for each."""
+    if len(q) != 4:
+        raise ValueError(f"q must be [batch, heads, queries, head_dim], got {tuple(q)}")
+    if len(k) != 4 or k != v:
+        raise ValueError("key_pages and value_pages must both be [num_pages, kv_heads, page, dim]")
+    B, Hq, T, D = q
+    N, Hkv, P, Dk = k
+    if Dk != D:
+        raise ValueError(f"head_dim mismatch: q {D}, pages {Dk}")
+    if Hkv == 0 or Hq == 0 or Hq % Hkv != 0:
+        raise ValueError(f"n_heads ({Hq}) must be a multiple of n_kv_heads ({Hkv})")
+    if len(block_table) != 2 or block_table[0] != B or tuple(seq_lens) != (B,):
+        raise ValueError("block_table must be [batch, max_pages] and seq_lens [batch]")
+    if query_lens is not None and tuple(query_lens) != (B,):
+        raise ValueError("query_lens must be [batch]")
+    M = block_table[1]
+    need = nat.size("lc_paged_extend_workspace_bytes", B, T, Hq, Hkv, D, M * P, lc_dtype)
+    return B, Hq, T, D, Hkv, P, N, M, max(need, 256), ks == vs and ks[-1] == 1
+
+
+def _paged_extend(q, key_pages, value_pages, block_table, seq_lens, query_lens, scale, return_lse):
+    i32 = torch.int32
+    if not (block_table.dtype is i32 and seq_lens.dtype is i32
+            and (query_lens is None or query_lens.dtype is i32)):
+        raise TypeError("block_table, seq_lens and query_lens must be int32")
+    if not q.dtype is key_pages.dtype is value_pages.dtype:
+        raise TypeError("q and the page pools must share a dtype")
+    dtype = nat.lc_dtype(q)
+    ks = key_pages.stride()
+    B, Hq, T, D, Hkv, P, N, M, ws_bytes, strides_ok = _extend_sizes(
+        q.shape, key_pages.shape, value_pages.shape, block_table.shape, seq_lens.shape,
+        None if query_lens is None else query_lens.shape, ks, value_pages.stride(), dtype)
+    dev = nat.require_device(q, key_pages, value_pages, block_table, seq_lens, query_lens)
+    if not strides_ok:
+        key_pages, value_pages = key_pages.contiguous(), value_pages.contiguous()
+        ks = key_pages.stride()
+    qs = q.stride()
+    if qs[-1] != 1:
+        q = q.contiguous()
+        qs = q.stride()
+    ts = block_table.stride()
+    # (rows that overlap, one expanded to the batch say, are copied: the kernels' rows do not)
+    if (M > 1 and ts[1] != 1) or (B > 1 and ts[0] < M):
+        block_table = block_table.contiguous()
+        ts = block_table.stride()
+    seq_lens = seq_lens.contiguous()
+    if query_lens is not None:
+        query_lens = query_lens.contiguous()
+    # (in q's order of dimensions: the token's heads side by side for a projection's view)
+    out = torch.empty_like(q)
+    os = out.stride()
+    if os[-1] != 1:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        os = out.stride()
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if return_lse else None
+    if B and T:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        with _guard(dev):
+            rc = nat.load().lc_paged_extend_fwd(
+                q.data_ptr(), qs[0], qs[1], qs[2], key_pages.data_ptr(), value_pages.data_ptr(),
+                ks[0], ks[1], ks[2], N, block_table.data_ptr(), max(ts[0], M), M,
+                seq_lens.data_ptr(), None if query_lens is None else query_lens.data_ptr(),
+                out.data_ptr(), os[0], os[1], os[2], None if lse is None else lse.data_ptr(),
+                ws.data_ptr(), ws_bytes, B, T, Hq, Hkv, D, P,
+                1.0 / math.sqrt(D) if scale is None else float(scale), dtype, _stream(dev))
+        if rc:
+            nat.check(rc, "lc_paged_extend_fwd")
+    return (out, lse) if return_lse else out
+
+
+def verify_draft_tokens(logits: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
+                        draft_logits: torch.Tensor | None = None,
+                        draft_lens: torch.Tensor | None = None,
+                        temperature: float | torch.Tensor = 1.0):
+    """Which of every sequence's drafted tokens stand, and the token after them (forward
+    only). Returns (tokens int64 [B, K + 1]: the drafts that stand, the new token, then -1;
+    accepted int32 [B]: how many stand).
+
+    logits [B, K + 1, V] (float32, float16 or bfloat16): the target's, row i those of draft
+    i's place; draft_tokens int64 [B, K]; uniforms float32 [B, K + 1], random numbers in
+    [0, 1); draft_logits [B, K, V] in logits' dtype: what the drafts were drawn from (None:
+    drafts without probabilities); draft_lens int32 [B]: how many drafts a sequence has (K for
+    all by default); temperature: a number, or float32 [B]. With p and q the softmax of
+    logits and draft_logits over temperature (q 1 at the draft without draft_logits), draft i
+    stands iff all before it do and uniforms[b, i] * q_i(draft) < p_i(draft). The new token
+    is drawn by uniforms[b, K] on the running sum of p behind the last draft, or, where
+    draft a was refused, of max(p_a - q_a, 0) (of p_a where that sums to under 2^-32); so
+    all tokens are distributed as the target's own. A temperature that is not a positive
+    finite number, or a row whose largest logit is not finite, stands for all mass on the
+    first largest logit (NaN is the largest): greedy decoding. K may be 0: sampling.
+    """
+    if _records_grad(logits, draft_logits):
+        return _ForwardOnly.apply(
+            "verify_draft_tokens",
+            lambda x, y: _verify_draft_tokens(x, draft_tokens, uniforms, y, draft_lens,
+                                              temperature), logits, draft_logits)
+    return _verify_draft_tokens(logits, draft_tokens, uniforms, draft_logits, draft_lens,
+                                temperature)
+
+
+@functools.lru_cache(maxsize=1024)
+def _verify_sizes(logits, draft_tokens, uniforms, draft_logits, draft_lens, temperature):
+    """Checks the shapes of a verify_draft_tokens call; (batch, drafts, vocab, workspace
+    bytes). A function of its arguments alone, run once for each."""
+    if len(logits) != 3 or logits[1] < 1 or logits[2] < 1:
+        raise ValueError(f"logits must be [batch, drafts + 1, vocab], got {tuple(logits)}")
+    B, T, V = logits
+    K = T - 1
+    if tuple(draft_tokens) != (B, K):
+        raise ValueError(f"draft_tokens must be {(B, K)}, got {tuple(draft_tokens)}")
+    if tuple(uniforms) != (B, T):
+        raise ValueError(f"uniforms must be {(B, T)}, got {tuple(uniforms)}")
+    if draft_logits is not None and tuple(draft_logits) != (B, K, V):
+        raise ValueError(f"draft_logits must be {(B, K, V)}, got {tuple(draft_logits)}")
+    if draft_lens is not None and tuple(draft_lens) != (B,):
+        raise ValueError(f"draft_lens must be {(B,)}, got {tuple(draft_lens)}")
+    if temperature is not None and tuple(temperature) != (B,):
+        raise ValueError(f"temperature must be a number or {(B,)}, got {tuple(temperature)}")
+    return B, K, V, nat.size("lc_verify_draft_tokens_workspace_bytes", B, K, V)
+
+
+def _verify_draft_tokens(logits, draft_tokens, uniforms, draft_logits, draft_lens, temperature):
+    temps = temperature if isinstance(temperature, torch.Tensor) else None
+    if temps is not None and temps.dtype is not torch.float32:
+        raise TypeError(f"temperature must be a number or float32, got {temps.dtype}")
+    if draft_tokens.dtype is not torch.int64:
+        raise TypeError(f"draft_tokens must be int64, got {draft_tokens.dtype}")
+    if uniforms.dtype is not torch.float32:
+        raise TypeError(f"uniforms must be float32, got {uniforms.dtype}")
+    if draft_lens is not None and draft_lens.dtype is not torch.int32:
+        raise TypeError(f"draft_lens must be int32, got {draft_lens.dtype}")
+    if draft_logits is not None and draft_logits.dtype is not logits.dtype:
+        raise TypeError("logits and draft_logits must share a dtype")
+    dtype = nat.lc_dtype(logits)
+    B, K, V, ws_bytes = _verify_sizes(
+        logits.shape, draft_tokens.shape, uniforms.shape,
+        None if draft_logits is None else draft_logits.shape,
+        None if draft_lens is None else draft_lens.shape, None if temps is None else temps.shape)
+    dev = nat.require_device(logits, draft_tokens, uniforms, draft_logits, draft_lens, temps)
+    xs = logits.stride()
+    if V > 1 and xs[2] != 1:
+        logits = logits.contiguous()
+        xs = logits.stride()
+    ys = (0, 0)
+    if draft_logits is not None:
+        ys = draft_logits.stride()
+        if V > 1 and ys[2] != 1:
+            draft_logits = draft_logits.contiguous()
+            ys = draft_logits.stride()
+    draft_tokens, uniforms = draft_tokens.contiguous(), uniforms.contiguous()
+    if draft_lens is not None:
+        draft_lens = draft_lens.contiguous()
+    if temps is not None:
+        temps = temps.contiguous()
+    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=dev)
+    accepted = torch.empty((B,), dtype=torch.int32, device=dev)
+    if B:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        with _guard(dev):
+            rc = nat.load().lc_verify_draft_tokens(
+                logits.data_ptr(), xs[0], xs[1],
+                None if draft_logits is None else draft_logits.data_ptr(), ys[0], ys[1],
+                draft_tokens.data_ptr(), uniforms.data_ptr(),
+                None if draft_lens is None else draft_lens.data_ptr(),
+                None if temps is None else temps.data_ptr(),
+                1.0 if temps is not None else float(temperature), B, K, V, tokens.data_ptr(),
+                accepted.data_ptr(), ws.data_ptr(), ws_bytes, dtype, _stream(dev))
+        if rc:
+            nat.check(rc, "lc_verify_draft_tokens")
+    return tokens, accepted
+
+
+# ---------------------------------------------------------------------------
+# Pages of a pool: resizing, forking, compaction (no counterpart in the reference,
+# whose cache owns fixed pages: models/llama3/kv_cache.py:21-36)
+# ---------------------------------------------------------------------------
+@functools.lru_cache(maxsize=1024)
+def _pool_sizes(k, v, ks, vs, block_table, seq_lens, page_refs, rows):
+    """Checks the shapes of a call on a page pool; (layers, pages, kv heads, page size,
+    head_dim, table rows, table width, layer stride). A function of its arguments alone, run
+    once for each."""
+    if len(k) not in (4, 5) or k != v:
+        raise ValueError("key_pages and value_pages must both be [layers, num_pages, kv_heads, "
+                         "page, dim]")
+    if ks != vs or ks[-1] != 1:
+        raise ValueError("key_pages and value_pages must share a layout with unit dim stride")
+    if any(n > 1 and stride == 0 for n, stride in zip(k, ks)):
+        raise ValueError("key_pages and value_pages are written: they cannot be expanded")
+    if len(block_table) != 2 or tuple(seq_lens) != (block_table[0],):
+        raise ValueError("block_table must be [batch, pages] and seq_lens [batch]")
+    L, s_layer = (k[0], ks[0]) if len(k) == 5 else (1, 0)
+    N, Hkv, P, D = k[-4:]
+    if tuple(page_refs) != (N,):
+        raise ValueError(f"page_refs must be [{N}], the pool's pages, got {tuple(page_refs)}")
+    if rows is not None and tuple(rows) != tuple(seq_lens):
+        raise ValueError(f"new_lens must be {tuple(seq_lens)}, got {tuple(rows)}")
+    return L, N, Hkv, P, D, block_table[0], block_table[1], s_layer
+
+
+def _pool_call(name, key_pages, value_pages, block_table, seq_lens, page_refs, rows=None):
+    """Checks of a call on a page pool: its sizes, the tensors that it reads, the device."""
+    sizes = _pool_sizes(key_pages.shape, value_pages.shape, key_pages.stride(),
+                        value_pages.stride(), block_table.shape, seq_lens.shape, page_refs.shape,
+                        rows)
+    if key_pages.dtype is not value_pages.dtype:
+        raise TypeError("key_pages and value_pages must share a dtype")
+    if key_pages.requires_grad or value_pages.requires_grad:
+        raise NotImplementedError(f"{name} writes the pools in place: they cannot require grad")
+    i32 = torch.int32
+    if not (block_table.dtype is i32 and seq_lens.dtype is i32 and page_refs.dtype is i32):
+        raise TypeError("block_table, seq_lens and page_refs must be int32")
+    dev = nat.require_device(key_pages, value_pages, block_table, seq_lens, page_refs)
+    B, M = sizes[5:7]
+    ts = block_table.stride()
+    if (M > 1 and ts[1] != 1) or (B > 1 and ts[0] < M):
+        block_table = block_table.contiguous()
+        ts = block_table.stride()
+    return (*sizes, block_table, max(ts[0], M), seq_lens.contiguous(), page_refs.contiguous(), dev)
+
+
+def paged_kv_resize(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, new_lens: torch.Tensor, page_refs: torch.Tensor):
+    """Pages for sequences that go from seq_lens to new_lens tokens; returns (block_table,
+    page_refs, missing).
+
+    key_pages, value_pages [layers, num_pages, Hkv, P, D] (or 4-D: one layer), which share
+    one block_table int32 [B, pages]; seq_lens, new_lens int32 [B] (clamped to the table's
+    capacity); page_refs int32 [num_pages]: how many table entries name a page, 0 for a
+    free one. A row of length L holds its first ceil(L / P) entries; the others of the new
+    table are -1. New entries are the lowest free pages, in the order of rows and
+    columns. A row that grows out of a partly filled page which other entries name too gets a
+    page of its own in its place, with its slots copied (in every layer, in the pools).
+    missing int32 [1]: pages asked for beyond the free ones; then entries are -1 and the
+    caller keeps what it had. Nothing that the old table names changes.
+    """
+    if new_lens.dtype is not torch.int32:
+        raise TypeError("new_lens must be int32")
+    (L, N, Hkv, P, D, B, M, s_layer, block_table, t_stride, seq_lens, page_refs, dev) = _pool_call(
+        "paged_kv_resize", key_pages, value_pages, block_table, seq_lens, page_refs,
+        new_lens.shape)
+    nat.require_device(seq_lens, new_lens)
+    new_lens = new_lens.contiguous()
+    dtype, ks = nat.lc_dtype(key_pages), key_pages.stride()
+    table = torch.empty((B, M), dtype=torch.int32, device=dev)
+    refs = torch.empty((N,), dtype=torch.int32, device=dev)
+    missing = torch.empty((1,), dtype=torch.int32, device=dev)
+    ws_bytes = nat.size("lc_paged_kv_resize_workspace_bytes", B, M, N)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _guard(dev):
+        rc = nat.load().lc_paged_kv_resize(
+            key_pages.data_ptr(), value_pages.data_ptr(), s_layer, ks[-4], ks[-3], ks[-2], L, N,
+            block_table.data_ptr(), t_stride, M, seq_lens.data_ptr(), new_lens.data_ptr(),
+            page_refs.data_ptr(), table.data_ptr(), refs.data_ptr(), missing.data_ptr(),
+            ws.data_ptr(), ws_bytes, B, Hkv, D, P, dtype, _stream(dev))
+    if rc:
+        nat.check(rc, "lc_paged_kv_resize")
+    return table, refs, missing
+
+
+def paged_kv_fork(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor,
+                  seq_lens: torch.Tensor, parents: torch.Tensor, page_refs: torch.Tensor):
+    """The batch becomes continuations of its rows: row r of the result continues row
+    parents[r] (int64 [R]; outside the batch: an empty row). Returns (block_table [R, pages],
+    seq_lens [R], page_refs, missing).
+
+    Arguments as in paged_kv_resize. Whole pages are shared through the table; the page
+    that a row is filling stays with its first child, and the others get copies of its
+    slots in the lowest free pages. Rows without children give up their pages.
+    """
+    if parents.dtype is not torch.int64 or parents.dim() != 1:
+        raise TypeError("parents must be int64 [rows]")
+    (L, N, Hkv, P, D, B, M, s_layer, block_table, t_stride, seq_lens, page_refs, dev) = _pool_call(
+        "paged_kv_fork", key_pages, value_pages, block_table, seq_lens, page_refs)
+    if M == 0:
+        raise ValueError("block_table has no columns")
+    nat.require_device(seq_lens, parents)
+    parents = parents.contiguous()
+    R = parents.shape[0]
+    dtype, ks = nat.lc_dtype(key_pages), key_pages.stride()
+    table = torch.empty((R, M), dtype=torch.int32, device=dev)
+    lens = torch.empty((R,), dtype=torch.int32, device=dev)
+    refs = torch.empty((N,), dtype=torch.int32, device=dev)
+    missing = torch.empty((1,), dtype=torch.int32, device=dev)
+    ws_bytes = nat.size("lc_paged_kv_fork_workspace_bytes", B, R, N)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _guard(dev):
+        rc = nat.load().lc_paged_kv_fork(
+            key_pages.data_ptr(), value_pages.data_ptr(), s_layer, ks[-4], ks[-3], ks[-2], L, N,
+            block_table.data_ptr(), t_stride, M, seq_lens.data_ptr(), parents.data_ptr(),
+            page_refs.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
+            missing.data_ptr(), ws.data_ptr(), ws_bytes, B, R, Hkv, D, P, dtype, _stream(dev))
+    if rc:
+        nat.check(rc, "lc_paged_kv_fork")
+    return table, lens, refs, missing
+
+
+def paged_kv_compact(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor,
+                     seq_lens: torch.Tensor, page_refs: torch.Tensor):
+    """The n pages in use become the pool's first n; returns (block_table, page_refs,
+    page_map int32 [num_pages]: each page's new index, -1 for a free one).
+
+    Arguments as in paged_kv_resize. Pages with an index of n or more move, in order, into
+    the free ones below n (copied in the pools; the old places keep their contents).
+    Holders of pages other than block_table look theirs up in page_map.
+    """
+    (L, N, Hkv, P, D, B, M, s_layer, block_table, t_stride, seq_lens, page_refs, dev) = _pool_call(
+        "paged_kv_compact", key_pages, value_pages, block_table, seq_lens, page_refs)
+    dtype, ks = nat.lc_dtype(key_pages), key_pages.stride()
+    table = torch.empty((B, M), dtype=torch.int32, device=dev)
+    refs, page_map = torch.empty((2, N), dtype=torch.int32, device=dev).unbind()
+    ws_bytes = nat.size("lc_paged_kv_compact_workspace_bytes", N)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _guard(dev):
+        rc = nat.load().lc_paged_kv_compact(
+            key_pages.data_ptr(), value_pages.data_ptr(), s_layer, ks[-4], ks[-3], ks[-2], L, N,
+            block_table.data_ptr(), t_stride, M, seq_lens.data_ptr(), page_refs.data_ptr(),
+            table.data_ptr(), refs.data_ptr(), page_map.data_ptr(), ws.data_ptr(), ws_bytes, B,
+            Hkv, D, P, dtype, _stream(dev))
+    if rc:
+        nat.check(rc, "lc_paged_kv_compact")
+    return table, refs, page_map

@@ -13,9 +13,12 @@
   prefix_lens, block_table, seq_lens)` decodes a batch whose groups of sequences
   share a prefix (the beams of a prompt, requests behind one system prompt): the
   prefix's pages are read and multiplied once per group, not once per sequence.
+* `paged_extend_attention(q, key_pages, value_pages, block_table, seq_lens)`
+  attends from the newest tokens of every sequence (drafts under verification,
+  chunks of a prompt), which may be unequal in number, to the cache in place.
 
 All return out shaped like q; `return_lse=True` adds the fp32 natural-log
-logsumexp [B, Hq] of the scaled scores. The paged entry also takes the
+logsumexp of the scaled scores, [B, Hq] ([B, Hq, T] for T tokens). The paged entry also takes the
 reference's additive attention_mask (the reference's decode predicate refuses
 masks and falls back to torch; that predicate keeps its answer here).
 """
@@ -145,3 +148,21 @@ def shared_prefix_decode_attention(
     without tokens gives zeros (lse -inf)."""
     return _ops.shared_prefix_decode(q, key_pages, value_pages, prefix_table, prefix_lens,
                                      block_table, seq_lens, scale=scale, return_lse=return_lse)
+
+
+def paged_extend_attention(
+    q: torch.Tensor,
+    key_pages: torch.Tensor,
+    value_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_lens: torch.Tensor | None = None,
+    scale: float | None = None,
+    return_lse: bool = False,
+):
+    """q [B, Hq, T, D]: the newest tokens of every sequence, already in the cache. Of
+    sequence b's T rows the first query_lens[b] (int32 [B]; T by default) are queries, at
+    positions seq_lens[b] - query_lens[b] + i; each attends to the tokens up to its own.
+    Table entries outside the pool are skipped; other rows give zeros (lse -inf)."""
+    return _ops.paged_extend(q, key_pages, value_pages, block_table, seq_lens,
+                             query_lens=query_lens, scale=scale, return_lse=return_lse)
