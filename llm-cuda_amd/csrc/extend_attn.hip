@@ -10,8 +10,11 @@
 #include <math.h>
 
 #include "lc_common.h"
+#include "paged_tiles.h"
 
 namespace {
+
+using namespace lc_attn;
 
 struct ExtendArgs {
   const void* q;
@@ -136,6 +139,139 @@ __global__ __launch_bounds__(64) void extend_generic_kernel(ExtendArgs a) {
   if (lane == 0) a.part_lse[pidx] = l_run == 0.f ? -INFINITY : m_run + lc_log2(l_run);
 }
 
+// A range of a sequence's tokens and a tile of a kv head's rows, row r = i G + g.
+template <typename T>
+struct ExtendItem {
+  static constexpr bool kCausal = true;
+  const int32_t* table;
+  Seq seq;
+  int b, kvh, row0, rows, t_begin, t_end, split, all_see;
+
+  template <typename Q>
+  __device__ __forceinline__ const Q* query(const ExtendArgs& a, int r) const {
+    const int i = r / a.G;
+    return static_cast<const Q*>(a.q) + (int64_t)b * a.q_sb + (int64_t)i * a.q_st +
+           (int64_t)(kvh * a.G + (r - i * a.G)) * a.q_sh;
+  }
+  __device__ __forceinline__ int limit(const ExtendArgs& a, int r) const {
+    return visible(seq, r / a.G);
+  }
+  // Where a row's results go: with one range they are the row's output.
+  struct Row {
+    T* out;
+    float* part;
+    int64_t lse;
+  };
+  __device__ __forceinline__ Row row(const ExtendArgs& a, int r) const {
+    const int i = r / a.G, h = kvh * a.G + (r - i * a.G);
+    const int64_t at = (((int64_t)b * a.Hq + h) * a.T + i) * a.splits + split;
+    return Row{static_cast<T*>(a.out) + (int64_t)b * a.o_sb + (int64_t)i * a.o_st + (int64_t)h * a.o_sh,
+               a.part_o + at * a.D, at};
+  }
+  __device__ __forceinline__ void store4(const ExtendArgs& a, const Row& row, int d, f32x4_t x) const {
+    if (a.splits == 1) {
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      t4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = lc_from_f32<T>(x[e]);
+      *reinterpret_cast<t4*>(row.out + d) = y;
+    } else {
+      *reinterpret_cast<f32x4_t*>(row.part + d) = x;
+    }
+  }
+  __device__ __forceinline__ void store_lse(const ExtendArgs& a, const Row& row, float x) const {
+    if (a.splits > 1)
+      a.part_lse[row.lse] = x;
+    else if (a.lse != nullptr)
+      a.lse[row.lse] = x * kLn2;
+  }
+};
+
+// Work item `at` of the grid. A range's row tiles read the same K and V: they get items 8
+// apart, which run on one XCD, and find it in its L2; the last tile, which sees the
+// most tokens, first. False: an item past the last range. The range may be empty.
+template <typename T>
+__device__ __forceinline__ bool extend_item(const ExtendArgs& a, int at, int row_tiles,
+                                            ExtendItem<T>& it) {
+  const int run = at / (8 * row_tiles), rest = at - run * 8 * row_tiles;
+  const int pair = run * 8 + (rest & 7), tile = row_tiles - 1 - (rest >> 3);
+  const int units = a.B * a.Hkv;
+  const int split = pair / units, u = pair - split * units;
+  const bool live = split < a.splits;
+  it.split = live ? split : 0;
+  it.b = live ? u / a.Hkv : 0;
+  it.kvh = live ? u - it.b * a.Hkv : 0;
+  it.table = a.table + (int64_t)it.b * a.t_stride;
+  it.seq = sequence(a, it.b);
+  it.rows = a.T * a.G;
+  it.row0 = tile * a.tile_rows;
+  const int len = live ? tile_len(a, it.seq, it.row0) : 0;
+  const int each = range_tokens(len, a.splits);
+  it.t_begin = it.split * each;
+  it.t_end = min(len, it.t_begin + each);
+  it.all_see = max(1, visible(it.seq, it.row0 / a.G));
+  return live;
+}
+
+// Outputs of a tile that sees no token, written by `threads` threads.
+template <typename T>
+__device__ __forceinline__ void clear_rows(const ExtendArgs& a, const ExtendItem<T>& it, int thread,
+                                           int threads) {
+  const int chunks = a.D / 4, end = min(it.rows, it.row0 + a.tile_rows);
+  for (int e = thread; e < (end - it.row0) * chunks; e += threads) {
+    const int r = it.row0 + e / chunks, d = e % chunks * 4;
+    const auto row = it.row(a, r);
+    it.store4(a, row, d, f32x4_t{0.f, 0.f, 0.f, 0.f});
+    if (d == 0) it.store_lse(a, row, -INFINITY);
+  }
+}
+
+// bf16/f16, head_dim a multiple of 8 up to 128, pages of a power of two from 8 up (see
+// paged_tiles.h): a workgroup of 4 waves per range and tile of 32 WR rows; with one
+// tile of 32 rows, `waves` of its waves per range.
+template <typename T, int DPAD, int WR>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+extend_mfma_kernel(ExtendArgs a, int row_tiles, int waves) {
+  constexpr int TILE_B = kTile * DPAD * (int)sizeof(T);
+  // (separate arrays: the compiler tracks a DMA by the array that it writes)
+  __shared__ __align__(16) char lds_k0[TILE_B];
+  __shared__ __align__(16) char lds_k1[TILE_B];
+  __shared__ __align__(16) char lds_v0[TILE_B];
+  __shared__ __align__(16) char lds_v1[TILE_B];
+  __shared__ float lds_scratch[4 * 512];
+  LC_LDS char *k0 = (LC_LDS char*)lds_k0, *k1 = (LC_LDS char*)lds_k1;
+  LC_LDS char *v0 = (LC_LDS char*)lds_v0, *v1 = (LC_LDS char*)lds_v1;
+  ExtendItem<T> it;
+  if constexpr (WR > 1) {
+    if (!extend_item(a, blockIdx.x, row_tiles, it)) return;
+    if (it.t_begin < it.t_end)
+      paged_range<T, DPAD, WR>(a, it, k0, k1, v0, v1, (LC_LDS float*)lds_scratch);
+    else if (a.splits == 1)
+      clear_rows(a, it, threadIdx.x, 256);
+  } else {
+    __shared__ float lds_ml[4 * 128];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool live = extend_item(a, blockIdx.x * (4 / waves) + wave / waves, row_tiles, it);
+    if (waves < 4 || it.t_begin < it.t_end)
+      paged_stream<T, DPAD>(a, it, waves, k0, k1, v0, v1, (LC_LDS float*)lds_ml,
+                            (LC_LDS float*)lds_scratch);
+    if (live && it.t_begin >= it.t_end && a.splits == 1)
+      clear_rows(a, it, threadIdx.x % (64 * waves), 64 * waves);
+  }
+}
+
+template <int DPAD>
+__global__ __launch_bounds__(256) __attribute__((
+    amdgpu_waves_per_eu(DPAD <= 64 ? 2 : 1, DPAD <= 64 ? 2 : 1))) void
+extend_f32_kernel(ExtendArgs a, int row_tiles) {
+  ExtendItem<float> it;
+  if (!extend_item(a, blockIdx.x, row_tiles, it)) return;
+  if (it.t_begin < it.t_end)
+    paged_f32_range<DPAD>(a, it);
+  else if (a.splits == 1)
+    clear_rows(a, it, threadIdx.x, 256);
+}
+
 // Merge: one wave per row joins its tile's ranges; each lane owns VPL consecutive
 // floats of head_dim. A row that sees no token gets out = 0, lse = -inf.
 template <typename T, int VPL>
@@ -190,27 +326,75 @@ __global__ __launch_bounds__(256) void extend_merge_kernel(ExtendArgs a, int64_t
 }
 
 struct ExtendPlan {
-  int tile_rows, splits;
+  int wr;      // row tiles of 32 of a workgroup
+  int splits;  // ranges of a tile's tokens
+  int waves;   // waves that share a range where wr is 1
 };
-ExtendPlan extend_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t cap) {
-  const int64_t units = B * Hq * T, cus = lc_cu_count();
-  int64_t s = units == 0 ? 1 : lc_cdiv(16 * cus, units);
-  const int64_t most = lc_cdiv(cap, 128);
-  s = s > most ? most : s;
-  return ExtendPlan{32, static_cast<int>(s < 1 ? 1 : s > 64 ? 64 : s)};
+
+ExtendPlan extend_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t cap, int dtype) {
+  const int64_t rows = T * (Hq / Hkv), cus = lc_cu_count();
+  ExtendPlan p{1, 1, 4};
+  if (dtype != LC_DTYPE_F32) p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  const int64_t units = B * Hkv * lc_cdiv(rows, 32 * p.wr);
+  if (units == 0 || cap == 0) return p;
+  int64_t s = lc_cdiv(p.wr == 1 ? cus : 2 * cus, units);
+  const int64_t most = lc_cdiv(cap, 2 * kStep);
+  s = s < most ? s : most;
+  p.splits = static_cast<int>(s < 64 ? s : 64);
+  const int64_t steps = lc_cdiv(lc_cdiv(cap, p.splits), 32);
+  p.waves = units * p.splits < 2 * cus || steps > 40 ? 4 : steps > 12 ? 2 : 1;
+  return p;
 }
 int64_t extend_bytes(int64_t rows, int64_t D, const ExtendPlan& p) {
   const int64_t n = rows * p.splits;
   return (n * D * 4 + 255) / 256 * 256 + n * 4;
 }
 
+template <typename T, int DPAD>
+int launch_mfma(const ExtendArgs& a, const ExtendPlan& p, hipStream_t st) {
+  const int64_t row_tiles = lc_cdiv((int64_t)a.T * a.G, a.tile_rows);
+  const int64_t items = lc_cdiv((int64_t)a.B * a.Hkv * a.splits, 8) * 8 * row_tiles;
+  const int64_t blocks = p.wr == 1 ? lc_cdiv(items, 4 / p.waves) : items;
+  LC_REQUIRE(blocks < (1LL << 24), "lc_paged_extend_fwd: %lld workgroups", (long long)blocks);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  const int rt = static_cast<int>(row_tiles);
+  if (p.wr == 1)
+    extend_mfma_kernel<T, DPAD, 1><<<grid, 256, 0, st>>>(a, rt, p.waves);
+  else if (p.wr == 2)
+    extend_mfma_kernel<T, DPAD, 2><<<grid, 256, 0, st>>>(a, rt, p.waves);
+  else
+    extend_mfma_kernel<T, DPAD, 4><<<grid, 256, 0, st>>>(a, rt, p.waves);
+  return lc_check_launch("lc_paged_extend_fwd (mfma)");
+}
+
+int launch_f32(const ExtendArgs& a, hipStream_t st) {
+  const int64_t row_tiles = lc_cdiv((int64_t)a.T * a.G, a.tile_rows);
+  const int64_t blocks = lc_cdiv((int64_t)a.B * a.Hkv * a.splits, 8) * 8 * row_tiles;
+  LC_REQUIRE(blocks < (1LL << 24), "lc_paged_extend_fwd: %lld workgroups", (long long)blocks);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  const int rt = static_cast<int>(row_tiles);
+  if (a.D <= 32)
+    extend_f32_kernel<32><<<grid, 256, 0, st>>>(a, rt);
+  else if (a.D <= 64)
+    extend_f32_kernel<64><<<grid, 256, 0, st>>>(a, rt);
+  else
+    extend_f32_kernel<128><<<grid, 256, 0, st>>>(a, rt);
+  return lc_check_launch("lc_paged_extend_fwd (fp32 mfma)");
+}
+
 template <typename T>
-int launch_extend(const ExtendArgs& a, hipStream_t st) {
-  static const char* who = "lc_paged_extend_fwd";
+int launch_extend(const ExtendArgs& a, const ExtendPlan& p, bool mfma, hipStream_t st) {
   const int64_t rows = (int64_t)a.B * a.Hq * a.T;
-  extend_generic_kernel<T><<<static_cast<unsigned>(rows * a.splits), 64, 0, st>>>(a);
-  const int rc = lc_check_launch(who);
-  if (rc != LC_OK) return rc;
+  int rc;
+  if (!mfma) {
+    extend_generic_kernel<T><<<static_cast<unsigned>(rows * a.splits), 64, 0, st>>>(a);
+    rc = lc_check_launch("lc_paged_extend_fwd (generic)");
+  } else if constexpr (sizeof(T) == 2) {
+    rc = a.D <= 64 ? launch_mfma<T, 64>(a, p, st) : launch_mfma<T, 128>(a, p, st);
+  } else {
+    rc = launch_f32(a, st);
+  }
+  if (rc != LC_OK || (mfma && a.splits == 1)) return rc;
   const unsigned blocks = static_cast<unsigned>(lc_cdiv(rows, 4));
   if (a.D <= 64)
     extend_merge_kernel<T, 1><<<blocks, 256, 0, st>>>(a, rows);
@@ -218,7 +402,7 @@ int launch_extend(const ExtendArgs& a, hipStream_t st) {
     extend_merge_kernel<T, 2><<<blocks, 256, 0, st>>>(a, rows);
   else
     extend_merge_kernel<T, 4><<<blocks, 256, 0, st>>>(a, rows);
-  return lc_check_launch(who);
+  return lc_check_launch("lc_paged_extend_fwd (merge)");
 }
 
 }  // namespace
@@ -228,7 +412,7 @@ extern "C" {
 int64_t lc_paged_extend_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
                                         int64_t capacity, int dtype) {
   if (B < 0 || T < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || D <= 0 || capacity < 0) return -1;
-  return extend_bytes(B * Hq * T, D, extend_plan(B, T, Hq, Hkv, capacity));
+  return extend_bytes(B * Hq * T, D, extend_plan(B, T, Hq, Hkv, capacity, dtype));
 }
 
 int lc_paged_extend_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st,
@@ -258,7 +442,7 @@ int lc_paged_extend_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st,
   LC_REQUIRE(q_sb >= 0 && q_sh >= 0 && q_st >= 0 && o_sb >= 0 && o_sh >= 0 && o_st >= 0 &&
                  kv_s_page >= 0 && kv_s_head >= 0 && kv_s_tok >= 0,
              "%s: negative stride", who);
-  const ExtendPlan plan = extend_plan(B, T, Hq, Hkv, max_pages_per_seq * page_size);
+  const ExtendPlan plan = extend_plan(B, T, Hq, Hkv, max_pages_per_seq * page_size, dtype);
   LC_REQUIRE(B * Hq * T < (1LL << 26) / plan.splits, "%s: %lld query rows", who,
              (long long)(B * Hq * T));
   const int64_t need = extend_bytes(B * Hq * T, D, plan);
@@ -301,16 +485,26 @@ int lc_paged_extend_fwd(const void* q, int64_t q_sb, int64_t q_sh, int64_t q_st,
   a.num_pages = static_cast<int>(num_pages);
   a.pages = static_cast<int>(max_pages_per_seq);
   a.splits = plan.splits;
-  a.tile_rows = plan.tile_rows;
+  a.tile_rows = 32 * plan.wr;
   a.scale_log2 = scale * kLog2e;
+  // The matrix kernels take whole 16-byte vectors of rows, pages of a power of two
+  // from 8 tokens up, and 32-bit strides (a page's rows within 2 GiB).
+  const int64_t vec = 16 / lc_dtype_size(dtype);
+  const bool mfma = D % vec == 0 && D <= 128 && q_sb % vec == 0 && q_sh % vec == 0 &&
+                    q_st % vec == 0 && kv_s_page % vec == 0 && kv_s_head % vec == 0 &&
+                    kv_s_tok % vec == 0 && o_sb % 4 == 0 && o_sh % 4 == 0 && o_st % 4 == 0 &&
+                    a.p_shift >= 3 && kv_s_tok < (1LL << 29) / page_size &&
+                    kv_s_page < (1LL << 32) && scale > 0 && max_pages_per_seq > 0 &&
+                    lc_aligned(q, 16) && lc_aligned(key_pages, 16) &&
+                    lc_aligned(value_pages, 16) && lc_aligned(out, 16);
   hipStream_t st = lc_stream(stream);
   switch (dtype) {
     case LC_DTYPE_F32:
-      return launch_extend<float>(a, st);
+      return launch_extend<float>(a, plan, mfma, st);
     case LC_DTYPE_BF16:
-      return launch_extend<bf16_t>(a, st);
+      return launch_extend<bf16_t>(a, plan, mfma, st);
     default:
-      return launch_extend<f16_t>(a, st);
+      return launch_extend<f16_t>(a, plan, mfma, st);
   }
 }
 

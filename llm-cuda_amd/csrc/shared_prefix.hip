@@ -18,9 +18,8 @@
 // 8.2 us, 400 TFLOP/s of QK and one PV in all).
 #include <math.h>
 
-#include "attn_f32.h"
-#include "attn_tiles.h"
 #include "lc_common.h"
+#include "paged_tiles.h"
 
 namespace {
 
@@ -159,7 +158,7 @@ __global__ __launch_bounds__(64) void shared_generic_kernel(SharedArgs a) {
 // g; a sequence's own rows are its G heads.
 //   S^T[tok x 32 rows] = K Q^T, O^T[d x 32 rows] += V^T P^T   (32x32x16 MFMA)
 // so a byte of K and V is read once for all rows of the workgroup. Up to 32 rows
-// the waves take token steps of their own (shared_stream below). With more, tiles
+// the waves take token steps of their own (paged_stream). With more, tiles
 // of 64 tokens go through LDS (double-buffered, by DMA), which the waves share: with
 // 128 rows each has 32 rows and all tokens, with 64 rows 32 tokens, and the token
 // halves' softmax states are joined through LDS at the end.
@@ -176,111 +175,6 @@ __global__ __launch_bounds__(64) void shared_generic_kernel(SharedArgs a) {
 // 22.2 -> 22.7 us); where a prefix has many rows, PV is twice the matrix work: 64 x
 // (8192 + 625) 52 -> 56 us, 256 x (8192 + 200) 75 -> 86.
 // ---------------------------------------------------------------------------
-constexpr int kTile = 64;  // tokens per tile
-constexpr float kSharedRescaleLog2 = 8.0f;
-
-__device__ __attribute__((aligned(16))) const uint32_t shared_zeros[4] = {0, 0, 0, 0};
-
-// Two weights, each as a value of the data type below it and what is left, rounded.
-// Both parts of a weight above 0 are above 0, so that an infinite V stays infinite (a
-// remainder of 0 or of the other sign would make it NaN).
-template <typename V>
-__device__ __forceinline__ void split_weights(float p0, float p1, V& whole, V& rest, int i) {
-  typedef std::remove_reference_t<decltype(whole[0])> T;
-  // (the next number below; 0 and a remainder of 0 for 0)
-  const uint32_t u0 = __builtin_elementwise_sub_sat(__float_as_uint(p0), 1u),
-                 u1 = __builtin_elementwise_sub_sat(__float_as_uint(p1), 1u);
-  if constexpr (std::is_same_v<T, bf16_t>) {
-    whole[i] = __builtin_bit_cast(T, static_cast<uint16_t>(u0 >> 16));
-    whole[i + 1] = __builtin_bit_cast(T, static_cast<uint16_t>(u1 >> 16));
-    rest[i] = static_cast<T>(p0 - __uint_as_float(u0 & 0xffff0000u));
-    rest[i + 1] = static_cast<T>(p1 - __uint_as_float(u1 & 0xffff0000u));
-  } else {
-    const auto w = __builtin_amdgcn_cvt_pkrtz(__uint_as_float(u0), __uint_as_float(u1));
-    whole[i] = static_cast<T>(w[0]);
-    whole[i + 1] = static_cast<T>(w[1]);
-    rest[i] = static_cast<T>(p0 - static_cast<float>(w[0]));
-    rest[i + 1] = static_cast<T>(p1 - static_cast<float>(w[1]));
-  }
-}
-
-struct RangeItem {
-  const int32_t* table;  // the token range's table row
-  int b0, row0, rows;    // row r is sequence b0 + r / G, head r % G of the kv head
-  int kvh, t_begin, t_end, slot;
-};
-
-// Where the token of each lane lies: its byte offset in the pools, and the bytes of
-// the RPI rows from it on that hold tokens of the range (0: none, or an invalid
-// page). One lane's answer serves a whole DMA instruction, by v_readlane: computed
-// by all lanes at once, it costs a few instructions per tile instead of a 64-bit
-// scalar product and its branches per DMA instruction.
-struct RowPlace {
-  uint32_t lo, hi;
-  int bytes;
-};
-template <int RPI>
-__device__ __forceinline__ RowPlace row_place(const SharedArgs& a, int page, int tok, int t_end,
-                                              int esz) {
-  const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(a.num_pages) && tok < t_end;
-  const uint32_t slot = static_cast<uint32_t>(tok & (a.P - 1)) * static_cast<uint32_t>(a.s_tok);
-  const uint64_t at =
-      (static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(a.s_page) + slot) *
-      static_cast<uint32_t>(esz);
-  RowPlace p;
-  p.lo = ok ? static_cast<uint32_t>(at) : 0;
-  p.hi = ok ? static_cast<uint32_t>(at >> 32) : 0;
-  p.bytes = ok ? ((min(RPI, t_end - tok) - 1) * static_cast<int>(a.s_tok) + a.D) * esz : 0;
-  return p;
-}
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* base, const RowPlace& p,
-                                                             int lane) {
-  const uint64_t at =
-      (static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(p.hi), lane))) << 32) |
-      static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(p.lo), lane));
-  return __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<char*>(static_cast<const char*>(base) + at), 0,
-      __builtin_amdgcn_readlane(p.bytes, lane), 0x00020000);
-}
-
-// Operands of a lane's query row: step s takes the 8 elements of chunk hh CPR / 2 + s
-// (zeros for a row that is none, or past head_dim).
-template <typename T, int DPAD>
-__device__ __forceinline__ void load_rows(const SharedArgs& a, int b, int h, bool row_ok, int hh,
-                                          typename Mfma32<T>::v8 (&qop)[DPAD / 16]) {
-  typedef typename Mfma32<T>::v8 v8;
-  constexpr int CPR = DPAD / 8;
-  const T* qh = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh;
-#pragma unroll
-  for (int s = 0; s < DPAD / 16; ++s) {
-    const int d0 = (hh * (CPR / 2) + s) * 8;
-    const bool ok = row_ok && d0 < a.D;
-    const v8 x = *reinterpret_cast<const v8*>(qh + (ok ? d0 : 0));
-    qop[s] = ok ? x : v8{};
-  }
-}
-
-// LDS addresses of a tile's operands from token row0 on (rows of DPAD, chunks
-// swizzled by pf_swz): K rows for S^T, V columns for O^T by transposed reads.
-template <typename T, int DPAD>
-__device__ __forceinline__ void operand_addresses(int lane, int row0, int (&kaddr)[DPAD / 16],
-                                                  int (&vaddr)[2][DPAD / 32]) {
-  constexpr int CPR = DPAD / 8, ROW_B = DPAD * (int)sizeof(T);
-  const int l32 = lane & 31, hh = lane >> 5;
-#pragma unroll
-  for (int s = 0; s < DPAD / 16; ++s)
-    kaddr[s] = (row0 + l32) * ROW_B + (((hh * (CPR / 2) + s) ^ pf_swz<CPR>(l32)) << 4);
-  const int gq = lane >> 4, te = (lane & 15) >> 2, tc = lane & 3;
-#pragma unroll
-  for (int jj = 0; jj < 2; ++jj)
-#pragma unroll
-    for (int dt = 0; dt < DPAD / 32; ++dt) {
-      const int kr = jj * 8 + hh * 4 + te;
-      const int d = dt * 32 + (gq & 1) * 16 + 4 * tc;
-      vaddr[jj][dt] = (row0 + kr) * ROW_B +
-                      ((((d >> 3) ^ pf_swz<CPR>(kr)) << 4) | ((d & 7) * (int)sizeof(T)));
-    }
-}
 
 // A partial output or logsumexp. Where another workgroup of the same launch reads it
 // (on another XCD, maybe), it is written through to memory by relaxed stores of
@@ -317,502 +211,28 @@ __device__ __forceinline__ f32x4_t got4(const float* from) {
   return f32x4_t{lo[0], lo[1], hi[0], hi[1]};
 }
 
-// Writes columns dt * 32 .. of a row's partial output.
-__device__ __forceinline__ void store_columns(const SharedArgs& a, int64_t pidx, int dt, int hh,
-                                              const f32x16_t& o, float inv_l) {
-  float* po = a.part_o + pidx * a.D;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int d0 = dt * 32 + j * 8 + hh * 4;
-    if (d0 < a.D) {  // (D % 8 == 0: whole groups of 4)
-      f32x4_t w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = o[j * 4 + e] * inv_l;
-      put4(a, po + d0, w);
-    }
+struct RangeItem {
+  static constexpr bool kCausal = false;
+  const int32_t* table;  // the token range's table row
+  int b0, row0, rows;    // row r is sequence b0 + r / G, head r % G of the kv head
+  int kvh, t_begin, t_end, slot;
+
+  template <typename T>
+  __device__ __forceinline__ const T* query(const SharedArgs& a, int r) const {
+    return static_cast<const T*>(a.q) + (int64_t)(b0 + r / a.G) * a.q_sb +
+           (int64_t)(kvh * a.G + r % a.G) * a.q_sh;
   }
-}
-
-template <typename T, int DPAD, int WR>
-__device__ __forceinline__ void shared_range(const SharedArgs& a, const RangeItem& it,
-                                             LC_LDS char* lds_k0, LC_LDS char* lds_k1,
-                                             LC_LDS char* lds_v0, LC_LDS char* lds_v1) {
-  typedef Mfma32<T> Ops;
-  typedef typename Ops::v8 v8;
-  constexpr int KS = DPAD / 16, DTL = DPAD / 32, CPR = DPAD / 8;
-  constexpr int RPI = 64 / CPR;           // token rows per DMA instruction
-  constexpr int NIW = kTile / (RPI * 4);  // DMA instructions per wave and tensor
-  constexpr int ROW_B = DPAD * (int)sizeof(T);
-  constexpr int NKT = WR == 4 ? 2 : 1;  // 32-token blocks per wave and tile
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wave_s = __builtin_amdgcn_readfirstlane(wave);
-  const int l32 = lane & 31, hh = lane >> 5;
-  const int wr = WR == 4 ? wave : (wave & 1);
-  const int wk = WR == 4 ? 0 : (wave >> 1);
-
-  // This lane's query row (a wave whose rows are none computes on zeros: it shares
-  // the others' steps anyway).
-  const int r_abs = it.row0 + wr * 32 + l32;
-  const bool row_ok = r_abs < it.rows;
-  const int r_safe = row_ok ? r_abs : it.row0;
-  const int b = it.b0 + r_safe / a.G;
-  const int h = it.kvh * a.G + r_safe % a.G;
-  v8 qop[KS];
-  load_rows<T, DPAD>(a, b, h, row_ok, hh, qop);
-
-  const T* kp = static_cast<const T*>(a.kp) + (int64_t)it.kvh * a.s_head;
-  const T* vp = static_cast<const T*>(a.vp) + (int64_t)it.kvh * a.s_head;
-  const int last_page = (it.t_end - 1) >> a.p_shift;
-  // Page entry of the tile's token t0 + lane (past the range: one that is not used).
-  auto fetch = [&](int t0) { return it.table[min((t0 + lane) >> a.p_shift, last_page)]; };
-  // DMA of one tensor's tile: this lane's 16-byte chunk of its row.
-  PfLoadOffsets<NIW> off;
-#pragma unroll
-  for (int u = 0; u < NIW; ++u) {
-    const int row = (wave * NIW + u) * RPI + lane / CPR;
-    const int ch = (lane % CPR) ^ pf_swz<CPR>(row);
-    off.o[u] = ch * 8 < a.D ? static_cast<int>(((lane / CPR) * a.s_tok + ch * 8) * sizeof(T)) : -16;
+  // (the row's partial output and logsumexp)
+  __device__ __forceinline__ int64_t row(const SharedArgs& a, int r) const {
+    return ((int64_t)(b0 + r / a.G) * a.Hq + kvh * a.G + r % a.G) * (a.p_splits + a.s_splits) + slot;
   }
-  auto place = [&](int t0, int pages) {
-    return row_place<RPI>(a, pages, t0 + lane, it.t_end, sizeof(T));
-  };
-  auto issue = [&](const T* base, const RowPlace& at, LC_LDS char* dst) {
-#pragma unroll
-    for (int u = 0; u < NIW; ++u) {
-      const int row0 = (wave_s * NIW + u) * RPI;
-      const int vo = off.o[u];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(row_buffer(base, at, row0),
-                                               (LC_LDS void*)(dst + row0 * ROW_B), 16, vo, 0, 0, 0);
-    }
-  };
-
-  // LDS addresses of the operands (see the prefill kernel's).
-  int kaddr[KS], vaddr[2][DTL];
-  operand_addresses<T, DPAD>(lane, wk * 32, kaddr, vaddr);
-
-  f32x16_t o[DTL];
-#pragma unroll
-  for (int i = 0; i < DTL; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-  float m_ref = -INFINITY, l_lane = 0.f, l_tile = 0.f;
-  f32x16_t x[NKT];  // raw scores of the next tile
-  f32x16_t y[NKT];  // exponents of the current tile, relative to m_ref
-  v8 pop[NKT][2], rem[NKT][2];
-
-  auto qk = [&](LC_LDS const char* kt_lds) __attribute__((always_inline)) {
-#pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[kt][r] = 0.f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-        x[kt] = Ops::mma(*reinterpret_cast<LC_LDS const v8*>(kt_lds + kaddr[s] + kt * 32 * ROW_B),
-                         qop[s], x[kt]);
-  };
-  auto pv = [&](LC_LDS const char* vt_lds) __attribute__((always_inline)) {
-#pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-      for (int jp = 0; jp < 2; ++jp)
-#pragma unroll
-        for (int dt = 0; dt < DTL; ++dt) {
-          const int rowoff = (kt * 32 + jp * 16) * ROW_B;
-          const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (LC_LDS i16x4_t*)(vt_lds + vaddr[0][dt] + rowoff));
-          const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (LC_LDS i16x4_t*)(vt_lds + vaddr[1][dt] + rowoff));
-          const i16x8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          o[dt] = Ops::mma(__builtin_bit_cast(v8, both), pop[kt][jp], o[dt]);
-          o[dt] = Ops::mma(__builtin_bit_cast(v8, both), rem[kt][jp], o[dt]);
-        }
-  };
-  // Scores of tokens that are none are masked; rows without a reference max (only
-  // before the first live tile) take the tile's.
-  constexpr uint64_t kAll = NKT == 2 ? ~0ull : 0xffffffffull;
-  auto prepare = [&](uint64_t live) __attribute__((always_inline)) {
-    const uint64_t mine = (live >> (wk * 32)) & kAll;
-    if (mine != kAll) {
-      const uint64_t bits = mine >> (hh * 4);
-#pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!((bits >> (kt * 32 + (r >> 2) * 8 + (r & 3))) & 1)) x[kt][r] = -INFINITY;
-    }
-    if (__ballot(m_ref == -INFINITY)) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, x[kt][r]);
-      mx = pf_half_max(mx) * a.scale_log2;
-      if (m_ref == -INFINITY) m_ref = mx;
-    }
-  };
-  auto shift = [&]() __attribute__((always_inline)) {
-    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) y[kt][r] = fmaf(x[kt][r], a.scale_log2, -m_use);
-  };
-  auto weigh = [&]() __attribute__((always_inline)) {
-    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float p0 = lc_exp2(y[kt][r]), p1 = lc_exp2(y[kt][r + 1]);
-        s0 += p0;
-        s1 += p1;
-        split_weights(p0, p1, pop[kt][r >> 3], rem[kt][r >> 3], r & 7);
-      }
-    l_tile = s0 + s1;
-  };
-  // A weight past 2^8 (then its lane's sum is too): the rows whose max grew move
-  // their reference there, with O and l, and the tile is weighed again.
-  auto settle = [&]() __attribute__((always_inline)) {
-    if (__builtin_expect(__ballot(l_tile > 256.f) != 0, 0)) {
-      float up = 0.f;
-#pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) up = fmaxf(up, y[kt][r]);
-      up = pf_half_max(up);
-      const float alpha = lc_exp2(-up);
-      l_lane *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DTL; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-      m_ref += up;  // (a row without a finite score so far, up 0, stays without a reference)
-#pragma unroll
-      for (int kt = 0; kt < NKT; ++kt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) y[kt][r] -= up;
-      weigh();
-    }
-    l_lane += l_tile;
-  };
-
-  // Step t computes S of tile t + 1 beside the softmax and PV of tile t: K runs a
-  // tile ahead of V. Its DMA (K of tile t + 2, V of t + 1) goes into the buffers that
-  // step t - 1 read; the page entries of tile t + 3 are on their way.
-  const int tb = it.t_begin;
-  const int n_tiles = (it.t_end - tb + kTile - 1) / kTile;
-  int pg3;             // page entries
-  RowPlace at1, at2;   // of tiles t + 1 and t + 2
-  uint64_t live1;
-  {
-    const int pg0 = fetch(tb), pg1 = fetch(tb + kTile), pg2 = fetch(tb + 2 * kTile);
-    pg3 = fetch(tb + 3 * kTile);
-    const RowPlace at0 = place(tb, pg0);
-    at1 = place(tb + kTile, pg1);
-    at2 = place(tb + 2 * kTile, pg2);
-    issue(kp, at0, lds_k0);
-    issue(vp, at0, lds_v0);
-    if (n_tiles > 1) issue(kp, at1, lds_k1);
-    const uint64_t live0 = __ballot(at0.bytes != 0);
-    live1 = __ballot(at1.bytes != 0);
-    pf_barrier<true>();
-    qk(lds_k0);
-    prepare(live0);
-    shift();
+  __device__ __forceinline__ void store4(const SharedArgs& a, int64_t row, int d, f32x4_t x) const {
+    put4(a, a.part_o + row * a.D + d, x);
   }
-  auto step = [&](int t, LC_LDS char* kc, LC_LDS char* vc, LC_LDS char* kn, LC_LDS char* vn)
-      __attribute__((always_inline)) {
-    // Tiles K t + 1 and V t are in LDS; the other buffers' reads are done.
-    pf_barrier<true>();
-    const int t0 = tb + t * kTile;
-    if (t + 2 < n_tiles) issue(kp, at2, kc);
-    issue(vp, at1, vn);
-    const uint64_t live = live1;
-    at1 = at2;
-    live1 = __ballot(at1.bytes != 0);
-    at2 = place(t0 + 3 * kTile, pg3);
-    pg3 = fetch(t0 + 4 * kTile);
-    // One matrix instruction, its operands' reads LA ahead, and vector work.
-    constexpr int NQ = NKT * KS, NP = NKT * 2 * DTL, LA = 4;
-    qk(kn);
-    weigh();
-    __builtin_amdgcn_sched_group_barrier(0x100, LA, 0);
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (j + LA < NQ) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
-    }
-    settle();
-    prepare(live);
-    pv(vc);
-    shift();
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * LA, 0);
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (j + LA < NP) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-    }
-  };
-  int t = 0;
-  for (; t + 2 < n_tiles; t += 2) {
-    step(t, lds_k0, lds_v0, lds_k1, lds_v1);
-    step(t + 1, lds_k1, lds_v1, lds_k0, lds_v0);
+  __device__ __forceinline__ void store_lse(const SharedArgs& a, int64_t row, float x) const {
+    put(a, a.part_lse + row, x);
   }
-  if (t + 1 < n_tiles) step(t, lds_k0, lds_v0, lds_k1, lds_v1);
-  // The last tile.
-  weigh();
-  settle();
-  pf_barrier<true>();
-  pv(n_tiles & 1 ? lds_v0 : lds_v1);
-
-  float l_tot = l_lane;
-  {
-    const unsigned u = __float_as_uint(l_lane);
-    const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    l_tot = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-  }
-  if constexpr (WR != 4) {
-    // The second token half's state goes to the first half's wave: O in the K
-    // buffers, [row tile][register][lane], then m and l.
-    __syncthreads();
-    LC_LDS float* rec = (LC_LDS float*)(wr == 0 ? lds_k0 : lds_k1);
-    LC_LDS float* ml = (LC_LDS float*)lds_v0 + wr * 128;
-    if (wk == 1) {
-#pragma unroll
-      for (int dt = 0; dt < DTL; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) rec[(dt * 16 + r) * 64 + lane] = o[dt][r];
-      ml[lane] = m_ref;
-      ml[64 + lane] = l_tot;
-    }
-    __syncthreads();
-    if (wk != 0) return;
-    const float m2 = ml[lane], l2 = ml[64 + lane];
-    const float m = fmaxf(m_ref, m2);
-    const float w1 = m_ref == -INFINITY ? (l_tot == 0.f ? 0.f : 1.f) : lc_exp2(m_ref - m);
-    const float w2 = m2 == -INFINITY ? (l2 == 0.f ? 0.f : 1.f) : lc_exp2(m2 - m);
-    l_tot = l_tot * w1 + l2 * w2;
-#pragma unroll
-    for (int dt = 0; dt < DTL; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[dt][r] = o[dt][r] * w1 + rec[(dt * 16 + r) * 64 + lane] * w2;
-    m_ref = m;
-  }
-  if (!row_ok) return;
-  const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
-  const float inv_l = l_tot == 0.f ? 0.f : 1.0f / l_tot;
-#pragma unroll
-  for (int dt = 0; dt < DTL; ++dt) store_columns(a, pidx, dt, hh, o[dt], inv_l);
-  if (hh == 0) put(a, a.part_lse + pidx, l_tot == 0.f ? -INFINITY : m_ref + lc_log2(l_tot));
-}
-
-// Up to 32 rows: bound by reading K and V, so the waves stream on their own, without
-// barriers: groups of gw waves (1, 2 or 4) share a range, wave i of a group taking
-// every gw-th 32-token step. `it` may be empty. A step's K and V rows
-// are loaded into registers (16 KB in flight per wave, 8 waves on a CU) while the
-// previous step computes from the wave's LDS. An instruction loads RPI token rows,
-// which share a page (pages of a power of two from RPI up): a scalar base and one
-// lane offset address it.
-template <typename T, int DPAD>
-__device__ __forceinline__ void shared_stream(const SharedArgs& a, const RangeItem& it, int gw,
-                                              LC_LDS char* b0, LC_LDS char* b1, LC_LDS char* b2,
-                                              LC_LDS char* b3, LC_LDS float* ml) {
-  typedef Mfma32<T> Ops;
-  typedef typename Ops::v8 v8;
-  constexpr int KS = DPAD / 16, DTL = DPAD / 32, CPR = DPAD / 8;
-  constexpr int RPI = 64 / CPR, NI = 32 / RPI;
-  constexpr int ROW_B = DPAD * (int)sizeof(T);
-  constexpr int kStep = 32;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wg = wave & (gw - 1);  // this wave in its group
-  const int l32 = lane & 31, hh = lane >> 5;
-  auto buffer = [&](int w) { return w == 0 ? b0 : w == 1 ? b1 : w == 2 ? b2 : b3; };
-  LC_LDS char* lds_k = buffer(wave);
-  LC_LDS char* lds_v = lds_k + kStep * ROW_B;
-
-  const int r_abs = it.row0 + l32;
-  const bool row_ok = r_abs < it.rows;
-  const int r_safe = row_ok ? r_abs : it.row0;
-  const int b = it.b0 + r_safe / a.G;
-  const int h = it.kvh * a.G + r_safe % a.G;
-  v8 qop[KS];
-  load_rows<T, DPAD>(a, b, h, row_ok, hh, qop);
-
-  const T* kp = static_cast<const T*>(a.kp) + (int64_t)it.kvh * a.s_head;
-  const T* vp = static_cast<const T*>(a.vp) + (int64_t)it.kvh * a.s_head;
-  const int last_page = (it.t_end - 1) >> a.p_shift;
-  const int srow = lane / CPR, chunk = lane % CPR;
-  const int lane_off =
-      chunk * 8 < a.D ? static_cast<int>((srow * a.s_tok + chunk * 8) * sizeof(T)) : -16;
-  // Page entry of token t + l32 (past the range: an entry that is not used).
-  auto fetch = [&](int t) { return it.table[min((t + l32) >> a.p_shift, last_page)]; };
-  auto place = [&](int t, int page) {
-    return row_place<RPI>(a, page, t + l32, it.t_end, sizeof(T));
-  };
-  // Rows past the range, of invalid pages or past head_dim lie outside the
-  // instruction's buffer and read zeros (which also keeps 0 x NaN out of the second
-  // product); no branch separates the loads.
-  u32x4_t sk[NI], sv[NI];
-  auto issue = [&](const RowPlace& at) {
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      sk[i] = __builtin_amdgcn_raw_buffer_load_b128(row_buffer(kp, at, i * RPI), lane_off, 0, 2);
-      sv[i] = __builtin_amdgcn_raw_buffer_load_b128(row_buffer(vp, at, i * RPI), lane_off, 0, 2);
-    }
-  };  // (2: non-temporal)
-
-  int kaddr[KS], vaddr[2][DTL];
-  operand_addresses<T, DPAD>(lane, 0, kaddr, vaddr);
-
-  f32x16_t o[DTL];
-#pragma unroll
-  for (int i = 0; i < DTL; ++i)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-  float m_ref = -INFINITY, l_lane = 0.f;
-
-  const int t0 = it.t_begin + wg * kStep;
-  const int next = gw * kStep;
-  // (the places of a step's rows are found a step ahead of its loads, and its page
-  // entries a step before that)
-  RowPlace at_next{};
-  int page_next = 0;
-  uint32_t live_next = 0;
-  if (t0 < it.t_end) {
-    const int page = fetch(t0), page1 = fetch(t0 + next);
-    page_next = fetch(t0 + 2 * next);
-    const RowPlace at = place(t0, page);
-    issue(at);
-    live_next = static_cast<uint32_t>(__ballot(at.bytes != 0));
-    at_next = place(t0 + next, page1);
-  }
-  for (int t = t0; t < it.t_end; t += next) {
-    const uint32_t live = live_next;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int row = i * RPI + srow;
-      const int at = row * ROW_B + ((chunk ^ pf_swz<CPR>(row)) << 4);
-      *reinterpret_cast<LC_LDS u32x4_t*>(lds_k + at) = sk[i];
-      *reinterpret_cast<LC_LDS u32x4_t*>(lds_v + at) = sv[i];
-    }
-    if (t + next < it.t_end) {
-      issue(at_next);
-      live_next = static_cast<uint32_t>(__ballot(at_next.bytes != 0));
-      at_next = place(t + 2 * next, page_next);
-      page_next = fetch(t + 3 * next);
-    }
-    lc_compiler_fence();
-    if (live == 0) continue;
-
-    f32x16_t x;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] = 0.f;
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-      x = Ops::mma(*reinterpret_cast<LC_LDS const v8*>(lds_k + kaddr[s]), qop[s], x);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) x[r] *= a.scale_log2;
-    if (live != 0xffffffffu) {
-      const uint32_t mine = live >> (hh * 4);
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (!((mine >> ((r >> 2) * 8 + (r & 3))) & 1)) x[r] = -INFINITY;
-    }
-    float mx = x[0];
-#pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
-    mx = pf_half_max(mx);
-    if (__ballot(mx > m_ref + kSharedRescaleLog2)) {
-      const float m_new = fmaxf(m_ref, mx);
-      const float alpha = m_new == -INFINITY ? 1.f : lc_exp2(m_ref - m_new);
-      l_lane *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DTL; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-      m_ref = m_new;
-    }
-    const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-    v8 pop[2], rem[2];
-#pragma unroll
-    for (int r = 0; r < 16; r += 2) {
-      const float p0 = lc_exp2(x[r] - m_use), p1 = lc_exp2(x[r + 1] - m_use);
-      l_lane += p0;
-      l_lane += p1;
-      split_weights(p0, p1, pop[r >> 3], rem[r >> 3], r & 7);
-    }
-#pragma unroll
-    for (int jp = 0; jp < 2; ++jp)
-#pragma unroll
-      for (int dt = 0; dt < DTL; ++dt) {
-        const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (LC_LDS i16x4_t*)(lds_v + vaddr[0][dt] + jp * 16 * ROW_B));
-        const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (LC_LDS i16x4_t*)(lds_v + vaddr[1][dt] + jp * 16 * ROW_B));
-        const i16x8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        o[dt] = Ops::mma(__builtin_bit_cast(v8, both), pop[jp], o[dt]);
-        o[dt] = Ops::mma(__builtin_bit_cast(v8, both), rem[jp], o[dt]);
-      }
-    lc_compiler_fence();
-  }
-
-  float l;
-  {
-    const unsigned u = __float_as_uint(l_lane);
-    const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-  }
-  const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
-  if (gw == 1) {
-    if (!row_ok || it.t_begin >= it.t_end) return;
-    const float inv_l = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-    for (int dt = 0; dt < DTL; ++dt) store_columns(a, pidx, dt, hh, o[dt], inv_l);
-    if (hh == 0) a.part_lse[pidx] = l == 0.f ? -INFINITY : m_ref + lc_log2(l);
-    return;
-  }
-  // Join the group's waves: each leaves O in its own buffer, [register][lane], and
-  // takes every gw-th block of 32 columns of all of them.
-  LC_LDS float* rec = (LC_LDS float*)lds_k;
-#pragma unroll
-  for (int dt = 0; dt < DTL; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) rec[(dt * 16 + r) * 64 + lane] = o[dt][r];
-  ml[wave * 128 + lane] = m_ref;
-  ml[wave * 128 + 64 + lane] = l;
-  __syncthreads();
-  if (it.t_begin >= it.t_end) return;
-  const int w0 = wave - wg;
-  float m = -INFINITY;
-  for (int w = w0; w < w0 + gw; ++w) m = fmaxf(m, ml[w * 128 + lane]);
-  // (a wave without tokens has m = -inf, l = 0 and O = 0; NaN passes)
-  auto weight = [&](int w) {
-    const float mw = ml[w * 128 + lane], lw = ml[w * 128 + 64 + lane];
-    return lw == 0.f ? 0.f : mw == -INFINITY ? 1.f : lc_exp2(mw - m);
-  };
-  l = 0.f;
-  for (int w = w0; w < w0 + gw; ++w) l += ml[w * 128 + 64 + lane] * weight(w);
-  const float inv_l = l == 0.f ? 0.f : 1.0f / l;
-  for (int dt = wg; dt < DTL; dt += gw) {
-    f32x16_t sum;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sum[r] = 0.f;
-    for (int w = w0; w < w0 + gw; ++w) {
-      const float f = weight(w);
-      LC_LDS const float* from = (LC_LDS const float*)buffer(w) + dt * 16 * 64 + lane;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sum[r] += from[r * 64] * f;
-    }
-    if (row_ok) store_columns(a, pidx, dt, hh, sum, inv_l);
-  }
-  if (row_ok && wg == 0 && hh == 0)
-    put(a, a.part_lse + pidx, l == 0.f ? -INFINITY : m + lc_log2(l));
-}
+};
 
 // The merge in the same launch, for few rows and ranges: every workgroup of group n
 // and kv head kvh takes a ticket after its partials, and the one with the last joins
@@ -960,166 +380,19 @@ shared_mfma_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups, i
     if (!prefix_item(a, id, row_tiles, 32 * WR, it)) return;
     if (it.t_begin < it.t_end) {
       if constexpr (WR > 1)
-        shared_range<T, DPAD, WR>(a, it, k0, k1, v0, v1);
+        paged_range<T, DPAD, WR>(a, it, k0, k1, v0, v1);
       else
-        shared_stream<T, DPAD>(a, it, 4, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
+        paged_stream<T, DPAD>(a, it, 4, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
     }
   } else {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     own_item(a, (id - p_blocks) * (4 / own_waves) + wave / own_waves, head_groups, it);
     if (own_waves < 4 || it.t_begin < it.t_end)
-      shared_stream<T, DPAD>(a, it, own_waves, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
+      paged_stream<T, DPAD>(a, it, own_waves, k0, k1, v0, v1, (LC_LDS float*)lds_ml);
   }
   if (a.counters != nullptr) join_last<T>(a, it.b0 / a.W, it.kvh);
 }
 
-// ---------------------------------------------------------------------------
-// fp32 on v_mfma_f32_32x32x2_f32 (head_dim a multiple of 4 up to 128, pages of a
-// power of two from 8 up): 32 rows per workgroup, whose 4 waves take every fourth
-// 32-token step of the range and are joined through LDS. Operands come straight
-// from global memory into registers, in the forms of attn_f32.h: a K row per lane,
-// at the lane's own address; V rows in groups of 8 tokens, which share a page.
-// Bound by the fp32 matrix rate where rows fill the tile, else by the start and the
-// latency of few steps.
-// ---------------------------------------------------------------------------
-template <int DPAD>
-__device__ __forceinline__ void shared_f32_range(const SharedArgs& a, const RangeItem& it) {
-  constexpr int DTL = DPAD / 32, LD = DPAD + 4, NC = DPAD / 8;
-  __shared__ __align__(16) float slab[4][32 * LD];
-  __shared__ float ms[4][32], ls[4][32];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int l32 = lane & 31, hh = lane >> 5;
-  const int r_abs = it.row0 + l32;
-  const bool row_ok = r_abs < it.rows;
-  F32Row<DPAD> q, k;
-  {
-    const int r = row_ok ? r_abs : it.row0;
-    const float* qh = static_cast<const float*>(a.q) + (int64_t)(it.b0 + r / a.G) * a.q_sb +
-                      (int64_t)(it.kvh * a.G + r % a.G) * a.q_sh;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int d = i * 8 + hh * 4;
-      const bool ok = row_ok && d < a.D;
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(qh + (ok ? d : 0));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) q.c[i][e] = ok ? x[e] : 0.f;
-    }
-  }
-  const float* kp = static_cast<const float*>(a.kp) + (int64_t)it.kvh * a.s_head;
-  const float* vp = static_cast<const float*>(a.vp) + (int64_t)it.kvh * a.s_head;
-  const int last_page = (it.t_end - 1) >> a.p_shift;
-  auto fetch = [&](int t) { return it.table[min((t + l32) >> a.p_shift, last_page)]; };
-  auto place = [&](int t, int page) { return row_place<8>(a, page, t + l32, it.t_end, 4); };
-  auto load_k = [&](const RowPlace& at) {
-    const char* row = reinterpret_cast<const char*>(kp) +
-                      ((static_cast<uint64_t>(at.hi) << 32) | at.lo) + hh * 16;
-    const char* none = reinterpret_cast<const char*>(shared_zeros);
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const bool ok = at.bytes != 0 && i * 8 + hh * 4 < a.D;
-      k.c[i] = *reinterpret_cast<const f32x4_t*>(ok ? row + i * 32 : none);
-    }
-  };
-  const int row_b = static_cast<int>(a.s_tok * 4);
-  const int v_off = l32 * DTL < a.D ? 4 * hh * row_b + l32 * DTL * 4 : kF32Oob;
-
-  f32x16_t o[DTL];
-#pragma unroll
-  for (int dt = 0; dt < DTL; ++dt) f32_zero(o[dt]);
-  float m = -INFINITY, l = 0.f;
-  constexpr int kNext = 4 * 32;
-  const int t0 = it.t_begin + wave * 32;
-  RowPlace at{};
-  int page_next = 0;
-  if (t0 < it.t_end) {
-    const int page = fetch(t0);
-    page_next = fetch(t0 + kNext);
-    at = place(t0, page);
-    load_k(at);
-  }
-  for (int t = t0; t < it.t_end; t += kNext) {
-    const uint32_t live = static_cast<uint32_t>(__ballot(at.bytes != 0));
-    F32Cols<DTL> v;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const __amdgpu_buffer_rsrc_t rs = row_buffer(vp, at, j * 8);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v.n[j * 4 + i] = f32_load_dims<DTL>(
-            rs, static_cast<int>(static_cast<unsigned>(v_off) + static_cast<unsigned>(i * row_b)));
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    f32x16_t s;
-    f32_zero(s);
-    f32_dot<DPAD>(s, k, q);
-    at = place(t + kNext, page_next);
-    page_next = fetch(t + 2 * kNext);
-    load_k(at);
-    __builtin_amdgcn_sched_barrier(0);
-    float mx = -INFINITY;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] *= a.scale_log2;
-      if (live != 0xffffffffu && !((live >> (8 * (r >> 2) + 4 * hh + (r & 3))) & 1))
-        s[r] = -INFINITY;
-      mx = fmaxf(mx, s[r]);
-    }
-    const float m_new = fmaxf(m, pf_half_max(mx));
-    if (__ballot(m_new > m) != 0) {
-      const float alpha = m_new == -INFINITY ? 1.f : lc_exp2(m - m_new);
-      l *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DTL; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
-      m = m_new;
-    }
-    const float m_use = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = lc_exp2(s[r] - m_use);
-      l += s[r];
-    }
-    f32_outer<DTL>(o, v, s);
-  }
-
-  l += __shfl_xor(l, 32, 64);
-  f32_put<DPAD>(slab[wave], o, l32, hh);
-  if (hh == 0) {
-    ms[wave][l32] = m;
-    ls[wave][l32] = l;
-  }
-  __syncthreads();
-  constexpr int CPR = DPAD / 4;
-#pragma unroll
-  for (int e = tid; e < 32 * CPR; e += 256) {
-    const int row = e / CPR, d = (e - row * CPR) * 4, r = it.row0 + row;
-    if (r >= it.rows || d >= a.D) continue;
-    float mt = -INFINITY, lt = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, ms[w][row]);
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      // (a wave without tokens has m = -inf, l = 0 and O = 0; NaN passes)
-      const float mw = ms[w][row], lw = ls[w][row];
-      const float f = lw == 0.f ? 0.f : mw == -INFINITY ? 1.f : lc_exp2(mw - mt);
-      lt = fmaf(lw, f, lt);
-      const f32x4_t ow = *reinterpret_cast<const f32x4_t*>(&slab[w][row * LD + d]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(ow[i], f, acc[i]);
-    }
-    const float inv = lt == 0.f ? 0.f : 1.0f / lt;
-    const int b = it.b0 + r / a.G, h = it.kvh * a.G + r % a.G;
-    const int64_t pidx = ((int64_t)b * a.Hq + h) * (a.p_splits + a.s_splits) + it.slot;
-    f32x4_t out;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = acc[i] * inv;
-    put4(a, a.part_o + pidx * a.D + d, out);
-    if (d == 0) put(a, a.part_lse + pidx, lt == 0.f ? -INFINITY : mt + lc_log2(lt));
-  }
-}
 
 template <int DPAD>
 __global__ __launch_bounds__(256) __attribute__((
@@ -1132,7 +405,7 @@ shared_f32_kernel(SharedArgs a, int p_blocks, int row_tiles, int head_groups) {
   } else {
     own_item(a, id - p_blocks, head_groups, it);
   }
-  if (it.t_begin < it.t_end) shared_f32_range<DPAD>(a, it);
+  if (it.t_begin < it.t_end) paged_f32_range<DPAD>(a, it);
   if (a.counters != nullptr) join_last<float>(a, it.b0 / a.W, it.kvh);
 }
 
