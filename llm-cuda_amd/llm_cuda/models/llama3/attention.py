@@ -23,6 +23,9 @@ differs only in how the attention itself is computed, all on HIP kernels:
     repeated K/V) and the causal diagonal shifted by the cached prefix length,
     which covers both the reference's fused path (past_len == 0) and its
     `_torch_attention` path with `past_len` (attention.py:63-89,144-147).
+  * Pooled cache (speculative decoding): the prompts as above; then any number of
+    tokens a step, rotated and appended at the sequences' own lengths, which may
+    differ, and attending to the pages in place.
   * An additive attention_mask (broadcastable to [B, H, q_len, kv_len], as the
     reference adds it to the scores, attention.py:85-86) goes into the same
     kernels: the prefill kernel for prompts and chunks, the paged decode
@@ -43,7 +46,7 @@ from llm_cuda.kernels.triton.decode_attention import (
 
 from .config import Llama3Config
 from .fused import FusedLinearWeights
-from .kv_cache import BeamKVLayerCache, PagedKVLayerCache
+from .kv_cache import BeamKVLayerCache, PagedKVLayerCache, PooledKVLayerCache
 from .rotary import apply_rotary, build_inv_freq, build_rope_cache
 
 
@@ -108,7 +111,7 @@ class Llama3Attention(nn.Module):
         return x.view(bsz, seq_len, heads, self.head_dim).transpose(1, 2)
 
     def _project_out(self, out: torch.Tensor, partial_out: bool):
-        """o_proj of a decode step's attention output [B, H, 1, D]."""
+        """o_proj of a decode step's attention output [B, H, tokens, D]."""
         bsz, _, seq_len, _ = out.shape
         out = out.transpose(1, 2).reshape(bsz, seq_len, self.num_heads * self.head_dim)
         wo = self.o_proj.weight
@@ -136,6 +139,25 @@ class Llama3Attention(nn.Module):
             return _ops.project(out, self.o_proj), cache
         own_rows = cache.cache.block_table.shape[1] * cache.cache.page_size
         self._rope_tables(0, cache.prefix_length + own_rows, q.device, q.dtype)
+        q = cache.append_rotated(q, k, v, self._rope_cache[2], self._rope_cache[3])
+        return self._project_out(cache.attend(q), partial_out), cache
+
+    def _pool_forward(self, q, k, v, attention_mask, cache: PooledKVLayerCache, use_cache: bool,
+                      partial_out: bool):
+        """Prompts into an empty pooled cache, or the next tokens of every sequence."""
+        if attention_mask is not None:
+            raise NotImplementedError("attention_mask with a pooled cache")
+        if not use_cache:
+            raise ValueError("a pooled cache needs use_cache=True")
+        bsz, _, seq_len, _ = q.shape
+        if cache.empty:
+            cos, sin = self._rope_tables(0, seq_len, q.device, q.dtype)
+            q, k = apply_rotary(q, k, cos, sin)
+            cache.append_prompt(k, v)
+            out = triton_fused_causal_attention(q, k, v)
+            out = out.transpose(1, 2).reshape(bsz, seq_len, self.num_heads * self.head_dim)
+            return _ops.project(out, self.o_proj), cache
+        self._rope_tables(0, cache.cache.max_pages * cache.cache.page_size, q.device, q.dtype)
         q = cache.append_rotated(q, k, v, self._rope_cache[2], self._rope_cache[3])
         return self._project_out(cache.attend(q), partial_out), cache
 
@@ -167,6 +189,9 @@ class Llama3Attention(nn.Module):
 
         if isinstance(past_key_value, BeamKVLayerCache):
             return self._beam_forward(q, k, v, attention_mask, past_key_value, use_cache,
+                                      partial_out)
+        if isinstance(past_key_value, PooledKVLayerCache):
+            return self._pool_forward(q, k, v, attention_mask, past_key_value, use_cache,
                                       partial_out)
 
         paged = isinstance(past_key_value, PagedKVLayerCache)

@@ -15,7 +15,8 @@ t % page_size of that sequence's pages. What changes:
     instead of a torch.cat of pages. The decode path does not call get_kv at
     all: it reads the pools in place (paged_decode_attention).
 
-`BeamKVCache` is the cache of a beam search (no counterpart in the reference).
+`BeamKVCache` is the cache of a beam search, `PooledKVCache` one whose sequences take,
+share and give back pages of a pool (no counterparts in the reference).
 """
 from __future__ import annotations
 
@@ -341,3 +342,161 @@ class BeamKVCache:
                              f"{tuple(parents.shape)}")
         self.block_table.copy_(_ops.paged_kv_reorder(
             self.key_pages, self.value_pages, self.block_table, self.seq_lens_all[0], parents))
+
+
+class PooledKVLayerCache:
+    """One layer of a PooledKVCache: views of its pools and lengths."""
+
+    def __init__(self, cache: "PooledKVCache", layer: int):
+        self.cache = cache
+        self.layer = layer
+        self.key_pages = cache.key_pages[layer]
+        self.value_pages = cache.value_pages[layer]
+
+    @property
+    def seq_lens(self) -> torch.Tensor:
+        return self.cache.seq_lens_all[self.layer]
+
+    @property
+    def empty(self) -> bool:
+        return self.cache.longest == 0
+
+    def _check(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
+        c = self.cache
+        if k.shape != v.shape or k.dim() != 4 or k.shape[0] != c.batch_size:
+            raise ValueError(f"expected k and v of {c.batch_size} sequences, [batch, kv_heads, "
+                             f"seq, head_dim]; got {tuple(k.shape)} and {tuple(v.shape)}")
+        if k.shape[2] != c.reserved:
+            raise ValueError(f"{k.shape[2]} tokens, {c.reserved} reserved")
+
+    def append_prompt(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The prompts' (rotated) keys and values, into empty sequences."""
+        self._check(k, k, v)
+        _ops.kv_append(k, v, self.key_pages, self.value_pages, self.cache.block_table,
+                       self.seq_lens)
+        self.seq_lens.add_(k.shape[2])
+        self.cache.appended(self.layer, k.shape[2])
+
+    def append_rotated(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                       cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        """Rotates q and k at the sequences' own next positions, appends k and v and returns
+        the rotated q. cos/sin: tables by position that cover the capacity."""
+        self._check(q, k, v)
+        q = _ops.rope_kv_append(q, k, v, cos, sin, self.key_pages, self.value_pages,
+                                self.cache.block_table, self.seq_lens)
+        self.cache.appended(self.layer, k.shape[2])
+        return q
+
+    def attend(self, q: torch.Tensor) -> torch.Tensor:
+        """Attention of the newest tokens' q [batch, heads, tokens, head_dim]."""
+        return _ops.paged_extend(q, self.key_pages, self.value_pages, self.cache.block_table,
+                                 self.seq_lens)
+
+
+class PooledKVCache:
+    """A paged cache whose sequences take pages of one pool as they grow, share them after
+    a fork and give them back. Lengths are the sequences' own (on the device).
+
+    A step is `reserve(n)`, then the layers append n tokens each; `truncate` gives the last
+    ones back, `fork` makes the batch continuations of its sequences, `compact` moves the
+    pages in use to the front. The pools are one tensor [layers, pages, kv_heads, page_size,
+    head_dim] with one block table; page_refs counts the entries that name a page.
+
+    num_pages: by default what `batch_size` sequences of max_seq_len tokens can ever ask for;
+    with fewer, `reserve` and `fork` wait for the GPU and raise where pages are missing (the
+    cache stays as it was).
+    """
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, max_seq_len: int,
+                 page_size: int, device: torch.device, dtype: torch.dtype, batch_size: int = 1,
+                 num_pages: int | None = None):
+        if min(num_layers, max_seq_len, page_size, batch_size) <= 0:
+            raise ValueError("layers, max_seq_len, page_size and batch_size must be > 0")
+        if num_pages is not None and num_pages <= 0:
+            raise ValueError("num_pages must be > 0")
+        device = torch.device(device)
+        self.max_seq_len, self.page_size = max_seq_len, page_size
+        self.batch_size = batch_size
+        self.max_pages = math.ceil(max_seq_len / page_size)
+        # (a sequence that writes into a shared page holds that page and its own for a moment)
+        self._enough = (self.max_pages + 1) * batch_size
+        self.num_pages = self._enough if num_pages is None else num_pages
+        self._rows = batch_size  # of which the pool is known to be large enough
+        self.key_pages = torch.empty(num_layers, self.num_pages, num_kv_heads, page_size, head_dim,
+                                     device=device, dtype=dtype)
+        self.value_pages = torch.empty_like(self.key_pages)
+        self.block_table = torch.full((batch_size, self.max_pages), -1, dtype=torch.int32,
+                                      device=device)
+        self.page_refs = torch.zeros(self.num_pages, dtype=torch.int32, device=device)
+        self.seq_lens_all = torch.zeros(num_layers, batch_size, dtype=torch.int32, device=device)
+        self.longest = 0  # host side: no sequence holds more tokens
+        self.reserved = 0  # tokens of every sequence that pages are held for, not appended yet
+        self.layer_caches = [PooledKVLayerCache(self, i) for i in range(num_layers)]
+
+    def get_layer(self, layer_idx: int) -> PooledKVLayerCache:
+        return self.layer_caches[layer_idx]
+
+    @property
+    def seq_lens(self) -> torch.Tensor:
+        """Tokens of every sequence, int32 [batch]."""
+        return self.seq_lens_all[0]
+
+    def pages_in_use(self) -> int:
+        return int((self.page_refs != 0).sum())
+
+    def _check_missing(self, missing: torch.Tensor, rows: int) -> None:
+        if self.num_pages < self._enough or rows > self._rows:
+            short = int(missing)
+            if short:
+                raise RuntimeError(f"the pool of {self.num_pages} pages is {short} short")
+
+    def reserve(self, tokens: int) -> None:
+        """Pages for `tokens` more tokens of every sequence."""
+        if self.reserved:
+            raise ValueError(f"{self.reserved} reserved tokens are not appended yet")
+        if tokens <= 0 or self.longest + tokens > self.max_seq_len:
+            raise ValueError(f"{tokens} tokens beside up to {self.longest} exceed max_seq_len")
+        table, refs, missing = _ops.paged_kv_resize(
+            self.key_pages, self.value_pages, self.block_table, self.seq_lens,
+            self.seq_lens + tokens, self.page_refs)
+        self._check_missing(missing, self.batch_size)
+        self.block_table, self.page_refs, self.reserved = table, refs, tokens
+
+    def appended(self, layer: int, tokens: int) -> None:
+        """A layer has appended the `tokens` reserved tokens."""
+        if layer == len(self.layer_caches) - 1:
+            self.longest += tokens
+            self.reserved = 0
+
+    def truncate(self, new_lens: torch.Tensor, longest: int) -> None:
+        """Sequences keep their first new_lens (int32 [batch]) tokens at most; `longest`, known
+        on the host: none is longer."""
+        if self.reserved:
+            raise ValueError(f"{self.reserved} reserved tokens are not appended yet")
+        new_lens = torch.minimum(new_lens, self.seq_lens)
+        self.block_table, self.page_refs, _ = _ops.paged_kv_resize(
+            self.key_pages, self.value_pages, self.block_table, self.seq_lens, new_lens,
+            self.page_refs)
+        self.seq_lens_all.copy_(new_lens.clamp(min=0).expand_as(self.seq_lens_all))
+        self.longest = min(self.longest, max(longest, 0))
+
+    def fork(self, parents: torch.Tensor) -> None:
+        """The batch becomes the continuations of sequences parents (int64 [rows])."""
+        if self.reserved:
+            raise ValueError(f"{self.reserved} reserved tokens are not appended yet")
+        table, lens, refs, missing = _ops.paged_kv_fork(
+            self.key_pages, self.value_pages, self.block_table, self.seq_lens, parents,
+            self.page_refs)
+        rows = parents.shape[0]
+        self._check_missing(missing, rows)
+        self.block_table, self.page_refs, self.batch_size = table, refs, rows
+        self.seq_lens_all = lens.repeat(len(self.layer_caches), 1)
+
+    def compact(self) -> torch.Tensor:
+        """The pages in use move to the front of the pool; returns each page's new index (int32
+        [num_pages], -1 for a free one)."""
+        if self.reserved:
+            raise ValueError(f"{self.reserved} reserved tokens are not appended yet")
+        self.block_table, self.page_refs, page_map = _ops.paged_kv_compact(
+            self.key_pages, self.value_pages, self.block_table, self.seq_lens, self.page_refs)
+        return page_map

@@ -19,7 +19,7 @@ from llm_cuda.kernels._ops import add_rms_norm, lm_head_argmax
 
 from .attention import Llama3Attention
 from .config import Llama3Config
-from .kv_cache import BeamKVCache, PagedKVCache, PagedKVLayerCache
+from .kv_cache import BeamKVCache, PagedKVCache, PagedKVLayerCache, PooledKVCache
 from .mlp import Llama3MLP
 from .norm import RMSNorm
 
@@ -94,7 +94,7 @@ class Llama3Model(nn.Module):
         use_cache: bool = False,
     ) -> dict:
         x = self.embed_tokens(input_ids)
-        paged = isinstance(past_key_values, (PagedKVCache, BeamKVCache))
+        paged = isinstance(past_key_values, (PagedKVCache, BeamKVCache, PooledKVCache))
         presents: list[tuple[torch.Tensor, torch.Tensor]] = []
         # Each layer's closing residual add is fused with the next norm (the
         # next layer's input norm, or the final norm): `pending` carries the
@@ -244,6 +244,157 @@ class Llama3ForCausalLM(nn.Module):
             return ids.unsqueeze(-1), out["past_key_values"], best
         return ids.unsqueeze(-1), out["past_key_values"]
 
+    def _logits(self, hidden: torch.Tensor) -> torch.Tensor:
+        """lm_head of a few rows."""
+        if _ops.decode_linear_applies(hidden, self.lm_head.weight):
+            return _ops.decode_linear(hidden, self.lm_head.weight)
+        return self.lm_head(hidden)
+
+    def _pooled_cache(self, batch_size: int, max_seq_len: int, page_size: int,
+                      device: torch.device) -> PooledKVCache:
+        return PooledKVCache(
+            num_layers=self.config.num_hidden_layers,
+            num_kv_heads=self.config.num_key_value_heads,
+            head_dim=self.config.head_dim,
+            max_seq_len=max_seq_len,
+            page_size=page_size,
+            device=device,
+            dtype=self.model.embed_tokens.weight.dtype,
+            batch_size=batch_size,
+        )
+
+    def _pooled_step(self, ids: torch.Tensor, cache: PooledKVCache) -> torch.Tensor:
+        """The next ids [batch, tokens] through the model; their hidden states."""
+        cache.reserve(ids.shape[1])
+        return self.model(ids, past_key_values=cache, use_cache=True)["hidden_states"]
+
+    @torch.no_grad()
+    def speculative_generate(
+        self,
+        input_ids: torch.Tensor,
+        draft_model: "Llama3ForCausalLM",
+        max_new_tokens: int = 16,
+        num_draft_tokens: int = 4,
+        temperature: float = 0.0,
+        num_samples: int = 1,
+        eos_token_id: int | None = None,
+        page_size: int = 64,
+        generator: torch.Generator | None = None,
+    ) -> tuple[torch.Tensor, int]:
+        """Speculative decoding of prompts [N, S]: (ids [N, num_samples, S + max_new_tokens],
+        steps of this model taken). An extension (the reference takes a token a step,
+        model.py:200-218).
+
+        A round drafts num_draft_tokens tokens of every sequence with draft_model (of the same
+        vocabulary), runs this model over all of them in one step and keeps the drafts that its
+        probabilities allow and one token more (`verify_draft_tokens`): the tokens are
+        distributed as this model's own at `temperature` (0: its greedy choices), whatever the
+        draft model is. The num_samples samples of a prompt share its pages; pages of refused
+        tokens and of finished sequences go back to the pool. eos_token_id: a sequence ends
+        with that token and is filled with it. generator: of the random numbers, on the
+        ids' device.
+        """
+        if input_ids.dim() != 2 or input_ids.shape[1] == 0:
+            raise ValueError(f"input_ids must be [prompts, tokens], got {tuple(input_ids.shape)}")
+        N, S = input_ids.shape
+        T, K, W, V = int(max_new_tokens), int(num_draft_tokens), int(num_samples), self.config.vocab_size
+        if T < 1 or W < 1:
+            raise ValueError("max_new_tokens and num_samples must be >= 1")
+        if not 1 <= K <= 255:
+            raise ValueError(f"num_draft_tokens {K} not in [1, 255]")
+        if draft_model.config.vocab_size != V:
+            raise ValueError(f"the draft model's vocabulary of {draft_model.config.vocab_size} is "
+                             f"not this model's ({V})")
+        if eos_token_id is not None and not 0 <= int(eos_token_id) < V:
+            raise ValueError(f"eos_token_id {eos_token_id} outside a vocabulary of {V}")
+        dev = input_ids.device
+        if N == 0:
+            return input_ids.new_empty((0, W, S + T)), 0
+        self.eval()
+        draft_model.eval()
+        fill = 0 if eos_token_id is None else int(eos_token_id)
+        result = torch.full((N * W, S + T), fill, dtype=torch.int64, device=dev)
+        result[:, :S] = input_ids.repeat_interleave(W, 0)
+
+        def uniforms(rows, count):
+            return torch.rand(rows, count, generator=generator, device=dev)
+
+        none = torch.empty((N * W, 0), dtype=torch.int64, device=dev)
+
+        def sample(logits):  # [rows, V] -> [rows, 1]
+            rows = logits.shape[0]
+            return _ops.verify_draft_tokens(logits.unsqueeze(1), none[:rows], uniforms(rows, 1),
+                                            temperature=temperature)[0]
+
+        longest = S + T + K + 1
+        cache = self._pooled_cache(N * W, longest, page_size, dev)
+        drafts = draft_model._pooled_cache(N * W, longest, page_size, dev)
+        samples = torch.arange(N, device=dev).repeat_interleave(W)
+        for c in (cache, drafts):
+            c.fork(samples[::W])
+        hidden = self._pooled_step(input_ids, cache)
+        draft_model._pooled_step(input_ids, drafts)
+        for c in (cache, drafts):
+            c.fork(samples)
+        first = sample(self._logits(hidden[:, -1, :]).repeat_interleave(W, 0))
+        steps = 1
+        # Of the sequences still running: their row of the result, their tokens, and how many
+        # (host: lens; device: n). The target's cache holds all but the last token, the draft
+        # model's may lack one more.
+        ids = torch.zeros((N * W, longest), dtype=torch.int64, device=dev)
+        ids[:, :S] = result[:, :S]
+        ids[:, S:S + 1] = first
+        row, lens = list(range(N * W)), [S + 1] * (N * W)
+        n = torch.full((N * W,), S + 1, dtype=torch.int32, device=dev)
+        new = first.tolist()
+        while True:
+            going = []
+            for r, tokens in enumerate(new):
+                end = lens[r]
+                start = end - len(tokens)
+                done = end >= S + T
+                if eos_token_id is not None and fill in tokens:
+                    end, done = start + tokens.index(fill) + 1, True
+                if done:
+                    end = min(end, S + T)
+                    result[row[r], S:end] = ids[r, S:end]
+                else:
+                    going.append(r)
+            if not going:
+                return result.view(N, W, S + T), steps
+            if len(going) < len(row):
+                keep = torch.tensor(going, device=dev)
+                for c in (cache, drafts):
+                    c.fork(keep)
+                ids, n = ids[keep], n[keep]
+                row, lens = [row[r] for r in going], [lens[r] for r in going]
+            rows, most = len(row), max(lens)
+            at = n.long().unsqueeze(1)
+            # Draft from the last two tokens on: the first of them may not be in the cache.
+            drafts.truncate(n - 2, most - 2)
+            step_ids = torch.gather(ids, 1, torch.cat([at - 2, at - 1], 1))
+            drafted, draft_logits = [], []
+            for _ in range(K):
+                hidden = draft_model._pooled_step(step_ids, drafts)
+                draft_logits.append(draft_model._logits(hidden[:, -1, :]))
+                step_ids = sample(draft_logits[-1])
+                drafted.append(step_ids)
+            drafted = torch.cat(drafted, 1)
+            step_ids = torch.cat([torch.gather(ids, 1, at - 1), drafted], 1)
+            logits = self._logits(self._pooled_step(step_ids, cache))
+            steps += 1
+            tokens, accepted = _ops.verify_draft_tokens(
+                logits, drafted, uniforms(rows, K + 1),
+                draft_logits=torch.stack(draft_logits, 1).to(logits.dtype),
+                temperature=temperature)
+            # (places past the new token are written again by a later round)
+            ids.scatter_(1, at + torch.arange(K + 1, device=dev), tokens.clamp(min=0))
+            n += accepted + 1
+            counts = accepted.tolist()
+            new = [t[:a + 1] for t, a in zip(tokens.tolist(), counts)]
+            lens = [length + a + 1 for length, a in zip(lens, counts)]
+            cache.truncate(n - 1, max(lens) - 1)
+
     @torch.no_grad()
     def beam_search(
         self,
@@ -300,11 +451,7 @@ class Llama3ForCausalLM(nn.Module):
 
         def select(ids, scores, finished):
             hidden = self.model(ids, past_key_values=cache, use_cache=True)["hidden_states"]
-            hidden, weight = hidden[:, -1, :], self.lm_head.weight
-            if _ops.decode_linear_applies(hidden, weight):
-                logits = _ops.decode_linear(hidden, weight)
-            else:
-                logits = self.lm_head(hidden)
+            logits = self._logits(hidden[:, -1, :])
             got = _ops.beam_select(logits.view(N, -1, V), scores, num_candidates=W,
                                    finished=finished, eos_token_id=eos_token_id)
             return got if finished is not None else (*got, None)
