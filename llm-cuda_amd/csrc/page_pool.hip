@@ -20,7 +20,11 @@
 namespace {
 
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-constexpr int kPagesPerThread = 16;  // of a pass over refs
+// Pages of a thread in a pass over refs: 16, or 1 in pools that few passes of that cover
+// (a thread's pages are one after another: 11.2 us for the plan of a compaction of 38 pages
+// with 16, 7.0 with 1).
+constexpr int kManyPages = 16;
+constexpr int64_t kSmallPool = 4 * kPlanThreads;
 constexpr int kApplyThreads = 256;
 constexpr int kCopyBlocks = 2048;
 
@@ -88,33 +92,34 @@ __device__ __forceinline__ int block_scan(int x, int& total, int* sums) {
 
 // A thread's share of a pass over refs, from page p0 on; pages past the pool count as
 // `none`.
-__device__ __forceinline__ void load_refs(const PoolArgs& a, int64_t p0, int none,
-                                          int (&r)[kPagesPerThread]) {
-  if (a.refs_wide && p0 + kPagesPerThread <= a.N) {
+template <int PAGES>
+__device__ __forceinline__ void load_refs(const PoolArgs& a, int64_t p0, int none, int (&r)[PAGES]) {
+  if (PAGES % 4 == 0 && a.refs_wide && p0 + PAGES <= a.N) {
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread; i += 4) {
+    for (int i = 0; i + 4 <= PAGES; i += 4) {
       const u32x4_t x = *reinterpret_cast<const u32x4_t*>(a.refs + p0 + i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) r[i + e] = static_cast<int>(x[e]);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread; ++i) r[i] = p0 + i < a.N ? a.refs[p0 + i] : none;
+    for (int i = 0; i < PAGES; ++i) r[i] = p0 + i < a.N ? a.refs[p0 + i] : none;
   }
 }
 
 // The `want` lowest free pages into list; returns how many there are of them.
+template <int PAGES>
 __device__ __forceinline__ int find_free(const PoolArgs& a, int want, int* sums) {
   int found = 0;
-  for (int64_t p0 = 0; p0 < a.N && found < want; p0 += kPlanThreads * kPagesPerThread) {
-    int r[kPagesPerThread], n = 0, total;
-    const int64_t mine = p0 + threadIdx.x * kPagesPerThread;
+  for (int64_t p0 = 0; p0 < a.N && found < want; p0 += kPlanThreads * PAGES) {
+    int r[PAGES], n = 0, total;
+    const int64_t mine = p0 + threadIdx.x * PAGES;
     load_refs(a, mine, 1, r);
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread; ++i) n += r[i] == 0;
+    for (int i = 0; i < PAGES; ++i) n += r[i] == 0;
     int rank = found + block_scan(n, total, sums);
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread; ++i)
+    for (int i = 0; i < PAGES; ++i)
       if (r[i] == 0) {
         if (rank < want) a.list[rank] = static_cast<int>(mine + i);
         ++rank;
@@ -145,6 +150,7 @@ __device__ __forceinline__ Resized resized(const PoolArgs& a, int b) {
   return s;
 }
 
+template <int PAGES>
 __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PoolArgs a) {
   __shared__ int sums[kPlanWaves];
   if (blockIdx.x > 0) return copy_refs(a);
@@ -162,7 +168,7 @@ __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PoolArgs a) {
     if (copy) a.copies[c] = CopyRec{s.shared, at, s.fill, 0};  // (dst: the rank, for now)
     n_copies += total;
   }
-  const int found = find_free(a, want, sums);
+  const int found = find_free<PAGES>(a, want, sums);
   __syncthreads();
   for (int c = threadIdx.x; c < n_copies; c += kPlanThreads) {
     const int rank = a.copies[c].dst;
@@ -177,8 +183,11 @@ __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(PoolArgs a) {
 
 // The plan's copies, dealt out to `blocks` workgroups of which this is number `block`:
 // a page's K or V of one layer each, or, where these are few, a part of it.
-// U: the unit of a copy, 16 bytes or one element.
-template <typename U>
+// U: the unit of a copy, 16 bytes or one element. kStream: stores past the caches, for
+// copies of whole pages that nobody reads soon (compaction of 445 MB: 107 -> 84 us, 5.3
+// TB/s, the rate of a large copy; loads past them as well: 102). A fork's sources and
+// copies are read next (33 us so, 28 through the caches).
+template <typename U, bool kStream = false>
 __device__ __forceinline__ void copy_slots(const PoolArgs& a, int elem_per_unit, int block,
                                            int blocks) {
   const int n = a.head[1];
@@ -205,7 +214,7 @@ __device__ __forceinline__ void copy_slots(const PoolArgs& a, int elem_per_unit,
     const int run = heads_join && c.slots == a.P ? total : rows_join ? per_head : row_units;
     const int each = ((total + parts - 1) / parts + kApplyThreads - 1) / kApplyThreads * kApplyThreads;
     const int begin = part * each, end = min(total, begin + each);
-    constexpr int kFlight = 4;
+    constexpr int kFlight = kStream ? 8 : 4;
     for (int i0 = begin + static_cast<int>(threadIdx.x); i0 < end; i0 += kApplyThreads * kFlight) {
       U x[kFlight];
       int64_t at[kFlight];
@@ -223,7 +232,12 @@ __device__ __forceinline__ void copy_slots(const PoolArgs& a, int elem_per_unit,
       }
 #pragma unroll
       for (int k = 0; k < kFlight; ++k)
-        if (i0 + k * kApplyThreads < end) to[at[k]] = x[k];
+        if (i0 + k * kApplyThreads < end) {
+          if constexpr (kStream)
+            __builtin_nontemporal_store(x[k], to + at[k]);
+          else
+            to[at[k]] = x[k];
+        }
     }
   }
 }
@@ -263,6 +277,7 @@ __device__ __forceinline__ int got(const int32_t* from) {
   return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+template <int PAGES>
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PoolArgs a) {
   __shared__ int sums[kPlanWaves];
   if (blockIdx.x > 0) return copy_refs(a);
@@ -298,7 +313,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PoolArgs a) {
     if (copy) a.copies[at] = CopyRec{page, at, fill, 0};
     want += total;
   }
-  const int found = find_free(a, want, sums);
+  const int found = find_free<PAGES>(a, want, sums);
   __syncthreads();
   for (int c = threadIdx.x; c < want; c += kPlanThreads)
     a.copies[c].dst = c < found ? a.list[c] : -1;
@@ -342,50 +357,56 @@ __global__ __launch_bounds__(kApplyThreads) void fork_apply_kernel(PoolArgs a, i
 // n pages are in use. Those with an index of n or more move, in order, into the free
 // ones below n, in order: as many of one as of the other. The holes come before the
 // pages that move there, so one pass finds both.
+template <int PAGES>
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PoolArgs a) {
   __shared__ int sums[kPlanWaves];
   __shared__ int live_total;
   if (threadIdx.x == 0) live_total = 0;
   __syncthreads();
-  constexpr int kPass = kPlanThreads * kPagesPerThread;
-  int r[kPagesPerThread];
-  int n = 0;
+  constexpr int kPass = kPlanThreads * PAGES;
+  int r[PAGES], n = 0;
   for (int64_t p0 = 0; p0 < a.N; p0 += kPass) {
-    load_refs(a, p0 + threadIdx.x * kPagesPerThread, 0, r);
+    load_refs(a, p0 + threadIdx.x * PAGES, 0, r);
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread; ++i) n += r[i] != 0;
+    for (int i = 0; i < PAGES; ++i) n += r[i] != 0;
   }
   atomicAdd(&live_total, n);
   __syncthreads();
   n = live_total;
   int holes = 0, moves = 0;
   for (int64_t p0 = 0; p0 < a.N; p0 += kPass) {
-    const int64_t mine = p0 + threadIdx.x * kPagesPerThread;
+    const int64_t mine = p0 + threadIdx.x * PAGES;
     load_refs(a, mine, 0, r);
     int h = 0, m = 0, total;
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread; ++i) {
+    for (int i = 0; i < PAGES; ++i) {
       h += r[i] == 0 && mine + i < n;
       m += r[i] != 0 && mine + i >= n;
     }
     int at_h = holes + block_scan(h, total, sums);
     holes += total;
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread; ++i)
+    for (int i = 0; i < PAGES; ++i)
       if (r[i] == 0 && mine + i < n) a.list[at_h++] = static_cast<int>(mine + i);
     int at_m = moves + block_scan(m, total, sums);  // (its barriers: the holes are written)
     moves += total;
+    // (all loads before the first store)
+    int to[PAGES];
+    int at = at_m;
 #pragma unroll
-    for (int i = 0; i < kPagesPerThread; ++i) {
+    for (int i = 0; i < PAGES; ++i) {
+      to[i] = r[i] == 0 ? -1 : static_cast<int>(mine + i);
+      if (r[i] != 0 && mine + i >= n) to[i] = a.list[at++];
+    }
+#pragma unroll
+    for (int i = 0; i < PAGES; ++i) {
       const int64_t p = mine + i;
       if (p < a.N) {
-        int to = r[i] == 0 ? -1 : static_cast<int>(p);
         if (r[i] != 0 && p >= n) {
-          to = a.list[at_m];
-          a.copies[at_m++] = CopyRec{static_cast<int>(p), to, a.P, 0};
-          a.out_refs[to] = r[i];
+          a.copies[at_m++] = CopyRec{static_cast<int>(p), to[i], a.P, 0};
+          a.out_refs[to[i]] = r[i];
         }
-        a.map[p] = to;
+        a.map[p] = to[i];
         if (p >= n)
           a.out_refs[p] = 0;
         else if (r[i] != 0)
@@ -399,7 +420,7 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PoolArgs a) 
 template <typename U>
 __global__ __launch_bounds__(kApplyThreads) void compact_apply_kernel(PoolArgs a, int elem_per_unit) {
   if (static_cast<int>(blockIdx.x) >= a.table_blocks)
-    return copy_slots<U>(a, elem_per_unit, blockIdx.x - a.table_blocks, gridDim.x - a.table_blocks);
+    return copy_slots<U, true>(a, elem_per_unit, blockIdx.x - a.table_blocks, gridDim.x - a.table_blocks);
   for (int i = blockIdx.x * kApplyThreads + threadIdx.x; i < a.B * a.M;
        i += a.table_blocks * kApplyThreads) {
     const int b = i / a.M, c = i - b * a.M;
@@ -487,12 +508,16 @@ int launch_pool(const char* who, PoolOp op, PoolArgs a, int dtype, hipStream_t s
   const int64_t refs_blocks = lc_cdiv(a.N, kPlanThreads);
   const unsigned plan = op == kCompact ? 1
                                        : 1 + static_cast<unsigned>(refs_blocks < 255 ? refs_blocks : 255);
+  const bool small = a.N <= kSmallPool;
   if (op == kResize)
-    resize_plan_kernel<<<plan, kPlanThreads, 0, st>>>(a);
+    small ? resize_plan_kernel<1><<<plan, kPlanThreads, 0, st>>>(a)
+          : resize_plan_kernel<kManyPages><<<plan, kPlanThreads, 0, st>>>(a);
   else if (op == kFork)
-    fork_plan_kernel<<<plan, kPlanThreads, 0, st>>>(a);
+    small ? fork_plan_kernel<1><<<plan, kPlanThreads, 0, st>>>(a)
+          : fork_plan_kernel<kManyPages><<<plan, kPlanThreads, 0, st>>>(a);
   else
-    compact_plan_kernel<<<plan, kPlanThreads, 0, st>>>(a);
+    small ? compact_plan_kernel<1><<<plan, kPlanThreads, 0, st>>>(a)
+          : compact_plan_kernel<kManyPages><<<plan, kPlanThreads, 0, st>>>(a);
   const int rc = lc_check_launch(who);
   if (rc != LC_OK) return rc;
   const int64_t entries = (int64_t)(a.B > a.R ? a.B : a.R) * a.M;
