@@ -370,6 +370,8 @@ class Llama3ForCausalLM(nn.Module):
                 row, lens = [row[r] for r in going], [lens[r] for r in going]
             rows, most = len(row), max(lens)
             at = n.long().unsqueeze(1)
+            # (after the finished ones left: their drafts may reach past the others' capacity)
+            cache.truncate(n - 1, most - 1)
             # Draft from the last two tokens on: the first of them may not be in the cache.
             drafts.truncate(n - 2, most - 2)
             step_ids = torch.gather(ids, 1, torch.cat([at - 2, at - 1], 1))
@@ -383,9 +385,11 @@ class Llama3ForCausalLM(nn.Module):
             step_ids = torch.cat([torch.gather(ids, 1, at - 1), drafted], 1)
             logits = self._logits(self._pooled_step(step_ids, cache))
             steps += 1
+            draft_logits = torch.stack(draft_logits, 1)
+            if draft_logits.dtype != logits.dtype:  # (both exactly, as they were drawn from)
+                draft_logits, logits = draft_logits.float(), logits.float()
             tokens, accepted = _ops.verify_draft_tokens(
-                logits, drafted, uniforms(rows, K + 1),
-                draft_logits=torch.stack(draft_logits, 1).to(logits.dtype),
+                logits, drafted, uniforms(rows, K + 1), draft_logits=draft_logits,
                 temperature=temperature)
             # (places past the new token are written again by a later round)
             ids.scatter_(1, at + torch.arange(K + 1, device=dev), tokens.clamp(min=0))
@@ -393,7 +397,6 @@ class Llama3ForCausalLM(nn.Module):
             counts = accepted.tolist()
             new = [t[:a + 1] for t, a in zip(tokens.tolist(), counts)]
             lens = [length + a + 1 for length, a in zip(lens, counts)]
-            cache.truncate(n - 1, max(lens) - 1)
 
     @torch.no_grad()
     def beam_search(

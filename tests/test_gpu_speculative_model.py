@@ -53,6 +53,29 @@ def test_a_perfect_draft_needs_few_steps(cuda):
     assert steps == 5  # the prompt's token, then 5 a round
 
 
+@pytest.mark.parametrize("K", [2, 5, 9])
+def test_sequences_that_end_in_different_rounds(cuda, K):
+    """A draft model near the target: sequences overshoot the end by up to K while others go on."""
+    import copy
+
+    model = build(cuda)
+    draft = copy.deepcopy(model)
+    g = torch.Generator(device=cuda).manual_seed(0)
+    with torch.no_grad():
+        for p in draft.parameters():
+            p.add_(0.04 * p.std() * torch.randn(p.shape, generator=g, device=cuda))
+    ids = prompts(cuda, N=9, S=15)
+    got, steps = model.speculative_generate(ids, draft, max_new_tokens=13, num_draft_tokens=K, page_size=16)
+    assert torch.equal(got[:, 0], model.generate(ids, max_new_tokens=13, use_paged_kv=True))
+    assert steps < 13
+
+
+def test_draft_model_of_another_type(cuda):
+    model, draft = build(cuda, BF16), build(cuda, F32, seed=2, layers=1)
+    got, _ = model.speculative_generate(prompts(cuda), draft, max_new_tokens=9, num_draft_tokens=3, temperature=0.8)
+    assert got.shape == (3, 1, 28)
+
+
 def test_one_token_prompts_and_one_new_token(cuda):
     model, draft = build(cuda), build(cuda, seed=3)
     for S, T in ((1, 9), (5, 1), (1, 1)):
