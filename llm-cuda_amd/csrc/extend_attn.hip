@@ -6,7 +6,12 @@
 // into `splits` equal ranges, whose normalised outputs and logsumexps a merge launch
 // joins:
 //   out = sum_i 2^(lse_i - M) o_i / sum_i 2^(lse_i - M),  M = max_i lse_i
-// (lse in log2 units).
+// (lse in log2 units); one range writes the output itself.
+//
+// Bound: reading K and V once (32 sequences of 4096 tokens, 5 queries, 8B heads: 537 MB in
+// 90 us, 5.9 TB/s; 8 of 32768, 70B: 1.07 GB in 194 us + merge 6.7), from some hundred rows a kv
+// head on the matrix and softmax work of the tiles (3 x up to 160 queries behind up to 4000
+// tokens, f16: 63 us + merge 12).
 #include <math.h>
 
 #include "lc_common.h"
@@ -331,6 +336,15 @@ struct ExtendPlan {
   int waves;   // waves that share a range where wr is 1
 };
 
+// Ranges: as many as give the CUs one round of workgroups, two of them each where tiles go
+// through LDS (us at 1 / 2 / 4 / 8 ranges: 32 sequences of 5 queries behind up to 4096
+// tokens, 8B heads 67 / 73 / 77 / 85; 8 behind 32768, 70B 625 / 334 / 198 / 199; one of
+// 256 queries behind 4000, 8B 132 / 87 / 62 / 56). None is shorter than 128 tokens: 5
+// queries behind 1000 take 14.1 us cut in 8, 21 in one piece.
+// Waves that share a range: four where the ranges are at most a round of workgroups (us
+// with 4 / 2 / 1 waves: 64 sequences of 1000 tokens, 8B heads 49 / 51 / 61, 48 of up to 1500
+// 41 / 49 / 79), two above (96 of up to 300 32 / 26 / 29, 128 of 2000 186 / 173 / 173), one
+// for many short ones (256 of 400 101 / 90 / 82, of up to 800 119 / 114 / 117).
 ExtendPlan extend_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t cap, int dtype) {
   const int64_t rows = T * (Hq / Hkv), cus = lc_cu_count();
   ExtendPlan p{1, 1, 4};
@@ -341,8 +355,8 @@ ExtendPlan extend_plan(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t ca
   const int64_t most = lc_cdiv(cap, 2 * kStep);
   s = s < most ? s : most;
   p.splits = static_cast<int>(s < 64 ? s : 64);
-  const int64_t steps = lc_cdiv(lc_cdiv(cap, p.splits), 32);
-  p.waves = units * p.splits < 2 * cus || steps > 40 ? 4 : steps > 12 ? 2 : 1;
+  const int64_t ranges = units * p.splits, steps = lc_cdiv(lc_cdiv(cap, p.splits), 32);
+  p.waves = ranges <= 2 * cus ? 4 : ranges >= 6 * cus && steps <= 20 ? 1 : 2;
   return p;
 }
 int64_t extend_bytes(int64_t rows, int64_t D, const ExtendPlan& p) {
