@@ -293,3 +293,37 @@ def test_whole_pages_of_real_sizes(cuda, Hkv, P, D, layers):
     args = make([150, 150, 90, 300, 64, 1], P, BF16, layers=layers, Hkv=Hkv, D=D, spare=30, share=1, seed=11)
     check("compact", args, cuda)
     check("fork", dict(args, parents=torch.tensor([0, 0, 0, 2, 2, 3, 3, 3, 5, 5])), cuda)
+
+
+def test_counts_that_are_not_aligned(cuda):
+    """page_refs from the second element of a buffer, in a pool of several passes."""
+    from llm_cuda.kernels import page_pool
+
+    g = torch.Generator().manual_seed(3)
+    N = 20011
+    refs = (torch.rand(N, generator=g) < 0.9).to(I32)
+    live = refs.nonzero().view(-1).to(I32)
+    pages = torch.arange(N, dtype=F32).view(1, N, 1, 1, 1)
+    base = dict(key_pages=pages.clone(), value_pages=-pages, block_table=live[:600].view(2, 300).contiguous(),
+                seq_lens=torch.tensor([100, 300], dtype=I32), page_refs=refs)
+    now = torch.tensor([300, 20], dtype=I32)
+    for name, want, more in (("resize", oracle.kv_resize(**base, new_lens=now), dict(new_lens=now)),
+                             ("compact", oracle.kv_compact(**base), {})):
+        args = on(cuda, dict(base, **more))
+        args["page_refs"] = torch.cat([refs[:1], refs]).to(cuda)[1:]
+        got = getattr(page_pool, f"paged_kv_{name}")(**args)
+        same((*got, args["key_pages"], args["value_pages"]), want, ("table", "refs", "third", "k", "v"))
+
+
+def test_a_pool_without_pages(cuda):
+    from llm_cuda.kernels import page_pool
+
+    pool = torch.empty(2, 0, 1, 4, 8, device=cuda)
+    none = torch.zeros(0, dtype=I32, device=cuda)
+    table, lens = torch.full((3, 5), -1, dtype=I32, device=cuda), torch.zeros(3, dtype=I32, device=cuda)
+    t, refs, missing = page_pool.paged_kv_resize(pool, pool, table, lens, lens + 7, none)
+    assert (t == -1).all() and refs.numel() == 0 and int(missing) == 6
+    t, n, refs, missing = page_pool.paged_kv_fork(pool, pool, table, lens, torch.tensor([0, 0], device=cuda), none)
+    assert t.shape == (2, 5) and not n.any() and int(missing) == 0
+    t, refs, page_map = page_pool.paged_kv_compact(pool, pool, table, lens, none)
+    assert (t == -1).all() and page_map.numel() == 0
