@@ -402,9 +402,9 @@ class PooledKVCache:
     pages in use to the front. The pools are one tensor [layers, pages, kv_heads, page_size,
     head_dim] with one block table; page_refs counts the entries that name a page.
 
-    num_pages: by default what `batch_size` sequences of max_seq_len tokens can ever ask for;
-    with fewer, `reserve` and `fork` wait for the GPU and raise where pages are missing (the
-    cache stays as it was).
+    num_pages: by default what `batch_size` sequences of max_seq_len tokens can ever ask for.
+    With fewer, and while a fork has made more than `batch_size` sequences, `reserve` and `fork`
+    wait for the GPU and raise where pages are missing (the cache stays as it was).
     """
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, max_seq_len: int,
@@ -488,7 +488,8 @@ class PooledKVCache:
             self.key_pages, self.value_pages, self.block_table, self.seq_lens, parents,
             self.page_refs)
         rows = parents.shape[0]
-        self._check_missing(missing, rows)
+        # (the old rows hold their pages until the new ones have theirs)
+        self._check_missing(missing, max(rows, self.batch_size))
         self.block_table, self.page_refs, self.batch_size = table, refs, rows
         self.seq_lens_all = lens.repeat(len(self.layer_caches), 1)
 
