@@ -541,8 +541,10 @@ __device__ __forceinline__ void paged_range(const A& a, const Item& it, LC_LDS c
     if (wk != 0) return;
     const float m2 = ml[lane], l2 = ml[64 + lane];
     const float m = fmaxf(m_ref, m2);
-    const float w1 = m_ref == -INFINITY ? (l_tot == 0.f ? 0.f : 1.f) : lc_exp2(m_ref - m);
-    const float w2 = m2 == -INFINITY ? (l2 == 0.f ? 0.f : 1.f) : lc_exp2(m2 - m);
+    // (by l first: a row that sees nothing has l = 0 and any reference, +inf among them; NaN
+    // passes)
+    const float w1 = l_tot == 0.f ? 0.f : m_ref == -INFINITY ? 1.f : lc_exp2(m_ref - m);
+    const float w2 = l2 == 0.f ? 0.f : m2 == -INFINITY ? 1.f : lc_exp2(m2 - m);
     l_tot = l_tot * w1 + l2 * w2;
 #pragma unroll
     for (int dt = 0; dt < DTL; ++dt)

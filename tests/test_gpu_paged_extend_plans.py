@@ -1,6 +1,6 @@
 """Attention of the newest tokens in every form that a call's sizes choose, with ranges of
-several whole tiles: rows that see unequal numbers of tokens, and a maximum that moves all
-along. Tolerances: see test_gpu_paged_extend.py."""
+several whole tiles: rows that see unequal numbers of tokens, a maximum that moves all along,
+and queries that are none. Tolerances: see test_gpu_paged_extend.py."""
 import math
 
 import pytest
@@ -110,3 +110,19 @@ def test_every_form_with_rising_scores(cuda, form):
     assert torch.equal(torch.isneginf(lse), empty) and not out[empty].any()
     assert ((out - ref).abs() <= half * ref.abs() + (2 * d + weight) * size + least).all()
     assert ((lse - ref_lse)[~empty].abs() <= d + 2 ** -21 * ref_lse[~empty].abs()).all()
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan, "largest"])
+@pytest.mark.parametrize("form", FORMS, ids=IDS)
+def test_rows_that_are_no_queries_may_hold_anything(cuda, form, bad):
+    """Rows past a sequence's queries, and queries before its first token: zeros, lse -inf."""
+    args = build(form, 3)
+    T = form[2]
+    i = torch.arange(T)
+    n = args["query_lens"].clamp(0, T).view(-1, 1)
+    dead = (i >= n) | (args["seq_lens"].view(-1, 1) - n + i < 0)
+    assert dead.any() and not dead.all()
+    want = whole(args)
+    bad = torch.finfo(form[0]).max if bad == "largest" else bad
+    args["q"] = torch.where(dead.view(len(n), 1, T, 1), torch.tensor(bad, dtype=form[0]), args["q"])
+    check(args, run(args, cuda), want=want)
