@@ -645,7 +645,8 @@ LC_API int64_t lc_verify_draft_tokens_workspace_bytes(int64_t B, int64_t drafts,
  * draft_tokens int64 [B, drafts] (one outside the vocabulary is refused); uniforms
  * fp32 [B, drafts + 1] in [0, 1); draft_lens int32 [B] (clamped to [0, drafts]) or
  * NULL (drafts for all); temperatures fp32 [B] or NULL: `temperature` for all.
- * drafts < 256. workspace: 256-byte aligned; calls that may overlap need their own.
+ * drafts < 256, B < 2^22. workspace: 256-byte aligned; calls that may overlap need
+ * their own.
  * No counterpart in the reference (models/llama3/model.py:200-218). */
 LC_API int lc_verify_draft_tokens(const void* logits, int64_t l_sb, int64_t l_si,
                                   const void* draft_logits, int64_t d_sb, int64_t d_si,

@@ -632,6 +632,8 @@ int lc_verify_draft_tokens(const void* logits, int64_t l_sb, int64_t l_si, const
   static const char* who = "lc_verify_draft_tokens";
   LC_REQUIRE(B >= 0 && drafts >= 0 && drafts <= kMaxDrafts, "%s: %lld sequences of %lld drafts (below 256)",
              who, (long long)B, (long long)drafts);
+  // (a launch has fewer than 2^32 threads)
+  LC_REQUIRE(B < (1LL << 32) / kDecideThreads, "%s: %lld sequences (below 2^22)", who, (long long)B);
   LC_REQUIRE(vocab > 0 && vocab < (1LL << 31) - 4 * kBlock, "%s: vocabulary of %lld", who,
              (long long)vocab);
   LC_REQUIRE(dtype == LC_DTYPE_F32 || dtype == LC_DTYPE_F16 || dtype == LC_DTYPE_BF16,
