@@ -637,7 +637,8 @@ LC_API int64_t lc_verify_draft_tokens_workspace_bytes(int64_t B, int64_t drafts,
  * less than 2^-32: then p and q agree). A temperature t that is not a positive finite
  * number, or a row whose largest logit is not finite, stands for all mass on the row's
  * first largest logit (NaN is the largest). Sums that choose a token are formed in 64
- * bits; those of p_i(d_i) and q_i(d_i) from fp32 terms (to 1e-6 relative).
+ * bits; those of p_i(d_i) and q_i(d_i) from fp32 terms (to some 1e-7 relative, 2.2e-6 at
+ * worst).
  *   tokens int64 [B, drafts + 1]: the drafts that stand, the new token, then -1
  *   accepted int32 [B]: a
  * logits [B, drafts + 1, vocab], draft_logits [B, drafts, vocab], unit stride over

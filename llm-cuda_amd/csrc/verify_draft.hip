@@ -12,8 +12,8 @@
 // draws from 128256 tokens. The sums that choose a token are therefore formed in 64
 // bits from 64-bit exponentials; they concern one row of a sequence (two with a refused
 // draft). Whether a draft stands is one comparison, for which sums of fp32 terms
-// (added in 64 bits from a wave's on) do: off by 1e-7, it falls otherwise in as
-// many of ten million.
+// (added in 64 bits from a wave's on) do: a sum off by some 1e-7, at worst 2.2e-6 (see
+// verify_stats_kernel), turns as large a part of the comparisons.
 //
 // Launches: statistics of every chunk of every row; decisions, a workgroup per sequence; the
 // 64-bit sums of the chosen rows; the residual's, where drafts have logits; the token. 64
@@ -138,9 +138,11 @@ __device__ __forceinline__ double last_lane(double x) {
 }
 __device__ __forceinline__ double wave_sum_f64(double x) { return last_lane(wave_scan_f64(x)); }
 
-// e^y for y <= 0 to 2^-47: y = k ln 2 + z with |z| <= ln 2 / 2, and the power series of
-// e^z up to z^11 (the next term is below 2^-47). k, found by adding 1.5 * 2^52, goes into
-// the exponent's bits; below -700 the term is 0.
+// e^y for y <= 0, off by at most 2^-46.6 + |y| 2^-54.7 relatively (2^-44.8 at -700): y =
+// k ln 2 + z with |z| <= ln 2 / 2, and the power series of e^z up to z^11. The next term
+// is 2^-46.7 of e^z where z is -ln 2 / 2; one double for ln 2 is off by 2^-55.3, k times
+// (a large |y| means a small term). k, found by adding 1.5 * 2^52, goes into the
+// exponent's bits; below -700 the term is 0.
 __device__ __forceinline__ double exp_f64(double y) {
   constexpr double kShift = 6755399441055744.0;
   const double t = fma(y, 1.4426950408889634, kShift);
@@ -166,8 +168,12 @@ __device__ __forceinline__ double exp_f64(double y) {
 
 // Chunk statistics: one workgroup per (chunk, row); rows are a sequence's K + 1 target
 // rows, then its K draft rows. Rows past the sequence's drafts are not read. Bound by
-// reading the logits once (64 sequences of up to 5 drafts, 128256 fp32 logits: 240 MB in 38
-// us, 6.3 TB/s).
+// reading the logits once (64 sequences of up to 5 drafts, 128256 fp32 logits: 240 MB in 37
+// us, 6.5 TB/s).
+// How far a chunk's sum may be off: three roundings of a term's exponent (the difference, the
+// scale, the product), 3 * 2^-24 times the terms' mean exponent, which is at most 6.2 (8191
+// equal logits under one that is larger by 7.2 temperatures); the exponential, 2^-23; 16
+// additions, 2^-24 each. Together 2.2e-6; the roundings of other rows mostly cancel.
 template <typename T, int BLOCKS>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyArgs a) {
   const int rows = 2 * a.K + 1;
@@ -355,7 +361,9 @@ __device__ __forceinline__ double* plane(const VerifyArgs& a, int which, int b) 
   return a.sums + ((int64_t)which * a.B + b) * a.chunks;
 }
 
-// 64-bit sums of a chunk's terms. Bound by the 64-bit exponentials.
+// 64-bit sums of a chunk's terms. One round of workgroups, which load and then compute: of 21
+// us (64 rows and the refused drafts', 128256 fp32 logits) the vector units issue for 14
+// (7.3 million instructions in 4096 waves, mostly 64-bit exponentials).
 template <typename T, int BLOCKS>
 __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   __shared__ double sums[kWaves];
@@ -567,8 +575,10 @@ __global__ __launch_bounds__(kThreads * BLOCKS) void verify_token_kernel(VerifyA
     a.tokens[(int64_t)b * (a.K + 1) + v.accepted] = pick != 0x7fffffff ? pick : last;
 }
 
-// Elements of a row per workgroup: 8192 where that still gives every CU one, else 2048,
-// for the latency of a few rows.
+// Elements of a row per workgroup: 8192 where that still gives every CU one in the first
+// pass, else 2048, for the latency of a few rows. The workspace's size does not depend on
+// which drafts have logits, so all 2 K + 1 rows of a sequence count, whether they are read
+// or not.
 int blocks_per_chunk(int64_t B, int64_t K, int64_t V) {
   return B * (2 * K + 1) * lc_cdiv(V, 4 * kBlock) >= lc_cu_count() ? 4 : 1;
 }
