@@ -11,7 +11,8 @@
 // Bound: reading K and V once (32 sequences of 4096 tokens, 5 queries, 8B heads: 537 MB in
 // 90 us, 5.9 TB/s; 8 of 32768, 70B: 1.07 GB in 194 us + merge 6.7), from some hundred rows a kv
 // head on the matrix and softmax work of the tiles (3 x up to 160 queries behind up to 4000
-// tokens, f16: 63 us + merge 12).
+// tokens, f16: 63 us + merge 12: the matrix units are busy a quarter of it, the vector units
+// a third; two waves a SIMD, and a second round of 88 workgroups). fp32: see paged_f32_range.
 #include <math.h>
 
 #include "lc_common.h"
@@ -336,11 +337,15 @@ struct ExtendPlan {
   int waves;   // waves that share a range where wr is 1
 };
 
-// Ranges: as many as give the CUs one round of workgroups, two of them each where tiles go
-// through LDS (us at 1 / 2 / 4 / 8 ranges: 32 sequences of 5 queries behind up to 4096
-// tokens, 8B heads 67 / 73 / 77 / 85; 8 behind 32768, 70B 625 / 334 / 198 / 199; one of
-// 256 queries behind 4000, 8B 132 / 87 / 62 / 56). None is shorter than 128 tokens: 5
-// queries behind 1000 take 14.1 us cut in 8, 21 in one piece.
+// Ranges of a full table: as many as give the CUs one round of workgroups, two of them each
+// where tiles go through LDS, rounded up (us at 1 / 2 / 4 / 8 ranges: 32 sequences of 5
+// queries behind up to 4096 tokens, 8B heads 67 / 73 / 77 / 85; 8 behind 32768, 70B 625 / 334
+// / 198 / 199; one of 256 queries behind 4000, 8B 132 / 87 / 62 / 56). None is shorter than
+// 128 tokens there: 5 queries behind 1000 take 14.1 us cut in 8, 21 in one piece. The rule
+// goes by the table's width, which the host knows; a sequence that leaves most of its row
+// unused is cut into as many, of 64 tokens or more (us in tables 1 / 8 / 64 times as wide as
+// the longest sequence: one of 1000 tokens 14.2 / 15.0 / 14.9; 256 of 400, whose ranges then
+// get two waves, 84 / 91 / 91; 32 of 4096, and chunks of 160 behind 4000, within 1%).
 // Waves that share a range: four where the ranges are at most a round of workgroups (us
 // with 4 / 2 / 1 waves: 64 sequences of 1000 tokens, 8B heads 49 / 51 / 61, 48 of up to 1500
 // 41 / 49 / 79), two above (96 of up to 300 32 / 26 / 29, 128 of 2000 186 / 173 / 173), one

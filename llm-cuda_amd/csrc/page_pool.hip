@@ -524,7 +524,7 @@ int launch_pool(const char* who, PoolOp op, PoolArgs a, int dtype, hipStream_t s
   const int64_t entries = (int64_t)(a.B > a.R ? a.B : a.R) * a.M;
   const int64_t tb = lc_cdiv(entries, kApplyThreads);
   a.table_blocks = static_cast<int>(tb < 1 ? 1 : tb > 1024 ? 1024 : tb);
-  // (a slot row of 16 bytes or more is worth a workgroup to 4 KB of a page)
+  // (at most a workgroup to 16 KB of a page's K or V, the least part of copy_slots)
   const int64_t most = needs.copies * a.layers * 2 *
                        lc_cdiv((int64_t)a.Hkv * a.P * a.D * lc_dtype_size(dtype), 16384);
   const int64_t cb = a.N == 0 ? 0 : most < kCopyBlocks ? most : kCopyBlocks;
